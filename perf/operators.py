@@ -307,8 +307,8 @@ def _quantized(x):
     lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
     edge, span = torch.where(lo.abs() > hi.abs(), lo, hi), hi - lo
     flat = span == 0
-    count = _away(15 * edge / torch.where(flat, torch.ones_like(span), span))
-    scale = torch.where(flat, torch.zeros_like(edge), edge / torch.where(flat, torch.ones_like(count), count)).bfloat16()
+    count = _away(15 * edge.abs() / torch.where(flat, torch.ones_like(span), span))
+    scale = torch.where(flat, torch.zeros_like(edge), -edge / torch.where(flat, torch.ones_like(count), count)).bfloat16()
     codes = _away((x - edge) / torch.where(flat, torch.ones_like(edge), scale.float()))
     return codes.clamp(0, 15), scale, edge.bfloat16()
 
@@ -465,9 +465,8 @@ def _exact_append(s):
         x = x.unflatten(-1, (-1, GROUP))
         low, high = torch.aminmax(x, dim=-1)
         end = low.where(low.abs() > high.abs(), high)
-        n = 15 * end / (high - low)
-        n = torch.trunc(n + 0.5 * torch.sign(n))
-        step = _nearest((end / n).where(high > low, 0 * end))[..., None]
+        n = torch.trunc(15 * end.abs() / (high - low) + 0.5)
+        step = _nearest((-end / n).where(high > low, 0 * end))[..., None]
         code = ((x - end[..., None]) / step.where(step != 0, step + 1)).add(0.5).floor().clamp(0, 15)
         return _nearest(code * step + end[..., None]).flatten(-2)
 
