@@ -139,6 +139,44 @@ int32_t b2_paged_attn_prefill(b2_ctx* ctx, const uint16_t* q_dev, const uint16_t
                               const int32_t* ctx_lens_host, int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim,
                               int32_t page_size, float scale, uint16_t* out_dev);
 
+/* ---- 4-bit key/value cache --------------------------------------------------------------------
+ * The same cache in 4-bit codes with a bf16 scale and bias for each 64 dims of a token's head: 144 bytes per token and kv
+ * head at head size 128, 72 at 64, against 512 and 256 (the reference caches bf16 only, src/primitives/kv_cache.rs:30-64).
+ * A code c stands for bf16(c * scale + bias).
+ * Pool: [n_pages, hkv, page_size / 16, record] bytes, a record being the keys and values of 16 tokens of one kv head:
+ *   K codes  [16 tokens][head_dim / 2] bytes: a token's dims in order, the lower of two in the low nibble
+ *   V codes  u32 [2][8][4][head_dim / 32]: word (h, g, c, d) holds token 8h + 2c in its low and token 8h + 2c + 1 in its high
+ *            half, each the dims g * head_dim / 8 + 4d .. + 3 from the lowest nibble on
+ *   K, then V scales and biases: u32 [head_dim / 64][16 tokens], scale in the low half, bias in the high one (both bf16)
+ * b2_kv_q4_pool_bytes gives the pool's size; a pool needs no initial contents.  Any hq / hkv that is whole, head_dim 64 or 128,
+ * page_size a multiple of 16, pool 16-byte aligned.  A block table may name pages in any order; a page number outside of
+ * 0 .. n_pages - 1 reads nothing (decode and short queries leave its tokens out, long ones see zeros there). */
+int64_t b2_kv_q4_pool_bytes(int64_t n_pages, int32_t hkv, int32_t head_dim, int32_t page_size); /* 0 for sizes that are refused */
+/* b2_rope_kv_append into such a pool: [per-head q/k RMSNorm ->] NeoX RoPE -> quantization -> append.  The rotation and its
+ * roundings are the same.  Per 64 values: e = the one farthest from zero (the largest in a tie), n = round(15 |e| / (max - min)),
+ * scale = bf16(-e / n), bias = e, code = clamp(round((x - bias) / scale), 0, 15), halves away from zero; equal values: scale 0.
+ * Values that are infinite, NaN or beyond 2^100 make their group NaN.  A slot outside of the pool skips the cache write; of
+ * tokens with the same slot in one call the last write is any of them.  k_out_dev / v_out_dev (nullable) [T, hkv, head_dim]
+ * receive the bf16 values that the codes stand for, for a caller that goes on with them. */
+int32_t b2_rope_kv_append_q4(b2_ctx* ctx, const uint16_t* qkv_dev, int32_t T, int32_t hq, int32_t hkv, int32_t head_dim,
+                             const int32_t* positions_dev, const int32_t* slot_mapping_dev, const uint16_t* cos_dev,
+                             const uint16_t* sin_dev, const uint16_t* q_norm_dev, const uint16_t* k_norm_dev, float eps,
+                             int32_t page_size, uint8_t* kv_pool_dev, int32_t n_pages, uint16_t* q_out_dev,
+                             uint16_t* k_out_dev, uint16_t* v_out_dev);
+/* b2_paged_attn_decode over such a pool: one query token per sequence.  Work is split evenly over the GPU whatever the
+ * lengths; the results do not depend on timing.  A ctx_lens[i] above max_blocks * page_size is read as that maximum; 0 gives
+ * rows of zeros.  What a page holds behind a sequence's end is not looked at. */
+int32_t b2_paged_attn_decode_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_t* kv_pool_dev, int32_t n_pages,
+                                const int32_t* block_tables_dev, int32_t max_blocks, const int32_t* ctx_lens_dev,
+                                int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size, float scale,
+                                uint16_t* out_dev);
+/* b2_paged_attn_prefill over such a pool: any number of query tokens per sequence, causal as there.  Sequences with many query
+ * tokens are widened to bf16 in a workspace of the context (up to 1 GiB, or what the longest sequence needs). */
+int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_t* kv_pool_dev, int32_t n_pages,
+                                 const int32_t* block_tables_dev, int32_t max_blocks, const int32_t* cu_seqlens_host,
+                                 const int32_t* ctx_lens_host, int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim,
+                                 int32_t page_size, float scale, uint16_t* out_dev);
+
 /* ---- MLX-format group-wise affine quantization (src/primitives/quant.rs:20-82,
  *      src/primitives/projection.rs:15-102) ------------------------------------------------------
  * Weight W [out, in]; packed [out, in*bits/32] u32 with codes along `in`, lowest bits first
@@ -190,6 +228,31 @@ int32_t b2_embed(b2_ctx* ctx, const uint16_t* table_dev, const int32_t* ids_dev,
                  uint16_t* out_dev);
 /* greedy argmax per row, ties -> lowest index (src/primitives/sampler.rs:221-241). */
 int32_t b2_argmax(b2_ctx* ctx, const uint16_t* logits_dev, int32_t rows, int32_t vocab, int32_t* out_dev);
+/* Rules on logits before a token is chosen (the host-side path of src/primitives/sampler.rs:160-219: repetition penalty,
+ * constraint mask; presence and frequency penalties and biases beside them).  All arrays are on the device; a null one means
+ * that the rule is not used, and its row of `rows`:
+ *   history: the tokens before this one, all rows one after the other, row i history_off[i] .. history_off[i+1] - 1; the first
+ *     n_prompt[i] of a row are its prompt (none: all of it is answer).  Tokens outside of the vocabulary do not count.
+ *   v seen in the history: v > 0 ? v / repetition : v * repetition;  n > 0 times in the answer: (v - n * frequency) - presence
+ *   bias: row i bias_off[i] .. bias_off[i+1] - 1 of (id, value), ids ascending; v + value (the first of equal ids counts)
+ *   mask: rows of mask_words words, bit t % 32 of word t / 32 says that token t is allowed; row mask_row[i] of them for row i
+ *     (none: row i; negative: everything is allowed).  What is not allowed becomes -inf.
+ * In f32, every step rounded once, in this order. */
+typedef struct {
+    const int32_t *history_dev, *history_off_dev /* [rows + 1] */, *n_prompt_dev /* [rows] */;
+    const float *repetition_dev, *presence_dev, *frequency_dev; /* [rows] each */
+    const int32_t* bias_id_dev;
+    const float* bias_value_dev;
+    const int32_t* bias_off_dev; /* [rows + 1] */
+    const uint32_t* mask_dev;
+    int64_t mask_words;
+    const int32_t* mask_row_dev; /* [rows] */
+} b2_logit_rules;
+/* logits_dev [rows] rows of vocab bf16 (f32 != 0: f32) values, ld apart.  out_dev (nullable; may be logits_dev): the adjusted
+ * logits, rounded to the same type, same ld.  argmax_dev (nullable): the greedy choice among the unrounded ones, ties -> lowest
+ * index, -1 where no token is above -inf (b2_argmax says 0 there; a token that is not allowed is never chosen here). */
+int32_t b2_logits_adjust(b2_ctx* ctx, const void* logits_dev, int32_t f32, int32_t rows, int32_t vocab, int64_t ld,
+                         const b2_logit_rules* rules, void* out_dev, int32_t* argmax_dev);
 /* RoPE inverse frequencies: kind 0 = Rope::standard (src/primitives/rope.rs:42-52), 1 = Rope::llama3
  * (rope.rs:125-156); host computation, f32 powf as the reference. */
 int32_t b2_rope_inv_freq(int32_t head_dim, float theta, int32_t kind, float factor, float low_freq_factor,

@@ -3,6 +3,10 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <vector>
+
+#include "../../include/b200llm.h"
+
 struct b2_ctx;
 
 // Paged-attention decode (paged_attn_decode.cu).  All pointers are device pointers.
@@ -205,3 +209,64 @@ int b2_prefill_q_tile(const b2_ctx* ctx, int head_dim);
 int32_t b2_prefill_attn_launch(b2_ctx* ctx, const PrefillAttnParams& p, int head_dim, int grid_work);
 bool b2_prefill_attn_tc_eligible(const PrefillAttnParams& p, int head_dim);
 int32_t b2_prefill_attn_tc_launch(b2_ctx* ctx, const PrefillAttnParams& p, int grid_work);
+
+// ---- 4-bit key/value cache (kv_q4_append.cu, kv_q4_attn.cu, kv_q4_prefill.cu; the records: kv_q4.cuh) -----------------------
+// What every entry point over such a pool refuses.
+int32_t b2_kv_q4_check(const char* who, const void* pool, int64_t n_pages, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size);
+struct RopeKvQ4Params {
+    RopeKvParams rope;   // (its pools are not used)
+    uint8_t* pool;       // [pages, hkv, page_size / 16, record]
+    int64_t n_slots;     // tokens of the pool; a slot outside of 0 .. n_slots - 1 skips the cache write
+    uint16_t *k_out, *v_out;  // [T, hkv, hd] bf16 values that the codes stand for, nullable
+};
+int32_t b2_rope_kv_q4_launch(b2_ctx* ctx, const RopeKvQ4Params& p);
+struct Q4AttnParams {
+    const uint16_t* q;            // [rows, hq, hd] bf16; sequence i's first row is q_rows[i] (or i)
+    const uint8_t* pool;
+    int64_t n_pages;              // a page number outside of 0 .. n_pages - 1 reads nothing: its tokens are left out
+    const int32_t* block_tables;  // [rows, max_blocks]; row of sequence i is bt_rows[i] (or i)
+    int max_blocks;
+    const int32_t* bt_rows;       // nullable
+    const int32_t* q_rows;        // nullable
+    const int32_t* ctx_lens;      // [num_seqs] tokens in the cache, the queries' own included
+    const int32_t* q_lens;        // [num_seqs] query tokens, the last of the context; null: one each
+    int num_seqs, hq, hkv, page_tiles;
+    float scale_log2;             // softmax scale * log2(e)
+    uint16_t* out;                // [rows, hq, hd] bf16
+    float* parts;                 // (filled in by the launch)
+    int* counters;
+};
+int32_t b2_kv_q4_attn_launch(b2_ctx* ctx, const Q4AttnParams& p, int head_dim);
+// Any number of query tokens per sequence, lengths known on the host: a plan (integers that have to be on the device before the launch,
+// `at` says where each list begins), made once for all layers of a step.
+struct Q4Seq {
+    int32_t bt_row, q_row, q_len, ctx;  // block-table row, first query row, query tokens (the last ones of the context), tokens in the cache
+};
+struct Q4Pass {  // sequences whose keys and values are widened to bf16 together
+    int seqs, work, max_ctx;
+    int64_t tiles;        // 16-token tiles of all of them
+    int max_tiles;        // of the longest
+    size_t list, cu;      // list: [seqs] block-table row, context, first tile; cu: rows, contexts and work items as the prefill kernels take them
+};
+struct Q4Plan {
+    std::vector<int32_t> host;
+    int few = 0;          // sequences that kv_q4_attn.cu takes: [few] of each of Q4Seq's numbers, from host[0] on
+    std::vector<Q4Pass> passes;
+};
+struct Q4PrefillParams {
+    const uint16_t* q;
+    int q_rows;                   // rows of the q allocation
+    const uint8_t* pool;
+    int64_t n_pages;
+    const int32_t* block_tables;
+    int max_blocks;
+    int hq, hkv, page_tiles;
+    float scale_log2;
+    uint16_t* out;
+};
+int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int hkv, int head_dim, Q4Plan& plan);
+// `plan_dev`: plan.host on the device
+int32_t b2_kv_q4_prefill_launch(b2_ctx* ctx, const Q4PrefillParams& p, int head_dim, const Q4Plan& plan, const int32_t* plan_dev);
+
+// ---- rules on logits (logits_adjust.cu): `rows` rows of `vocab` bf16 or f32 logits, `ld` apart; out and argmax nullable
+int32_t b2_logits_adjust_launch(b2_ctx* ctx, const b2_logit_rules& rules, const void* logits, bool f32, int rows, int vocab, int64_t ld, void* out, int32_t* argmax);

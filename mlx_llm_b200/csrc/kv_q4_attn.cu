@@ -1,0 +1,512 @@
+// Attention over a 4-bit paged cache for few query tokens per sequence: single-token decode, and the short runs of tokens that a
+// verification step checks.
+//
+// HBM-bound byte streaming, 144 bytes per token and kv head (head size 128), with the conversion of 32 codes a lane close behind it.
+//
+//   unit    = (sequence, kv head, block of 8 columns); a column is one (query token, q head of the group).  Its work is the sequence's
+//             16-token records.
+//   split   = all units' records form one line, which is cut into equal runs, one per warp: every warp streams the same number of
+//             records whatever the lengths of the sequences, and no warp of a block waits for another before its run is done.
+//             A unit inside one run is written out at once.  Runs that share a unit leave (maximum, sum, unnormalised output): first
+//             in shared memory, where the block adds up its warps', then in global memory, where the block that arrives last adds up
+//             the blocks', both in the order of the line, so that results do not depend on timing.
+//   tensor  = mma.sync m16n8k16 with the record's 16 tokens on M and the columns on N: S^T = K Q^T, then O^T += V^T P^T.  Codes become
+//             A operands in place (9 instructions for 8 codes, kv_q4.cuh); the order of dims inside a product is free, so Q is read in
+//             the order that the nibbles come out.  P^T reaches the B layout with one movmatrix per 8 tokens; it is split into a bf16
+//             head and remainder, so that P V keeps ~16 bits.
+//   softmax = in the log2 domain against a running reference that is raised only when a score exceeds it by more than 2^8.
+#include <algorithm>
+
+#include "kernels.h"
+#include "kv_q4.cuh"
+
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kWarps = 8, kStages = 3;
+constexpr int kEntries = 1024;       // entries of the line's index in shared memory; each covers num_seqs / kEntries sequences
+constexpr float kFloor = -1e30f;     // reference of a column that has seen nothing: exp2(-inf - floor) is 0
+constexpr float kSlack = 8.f;
+constexpr int kMinRun = 4;           // records of a run at least
+constexpr int kBlocksPerSm = 2;
+
+template <int HD>
+constexpr int part_floats() {
+    return 8 * HD + 16;  // [8 columns][HD] outputs, 8 maxima, 8 sums
+}
+template <int HD>
+constexpr int ring_bytes() {
+    return kWarps * kStages * q4::Record<HD>::kBytes;
+}
+template <int HD>
+constexpr int smem_bytes() {
+    return ring_bytes<HD>() + kWarps * part_floats<HD>() * 4;
+}
+
+struct Lengths {  // of one sequence
+    int ctx, queries, tiles, blocks;
+};
+__device__ __forceinline__ Lengths lengths_of(const Q4AttnParams& p, int seq) {
+    Lengths l;
+    l.ctx = min(max(p.ctx_lens[seq], 0), p.max_blocks * p.page_tiles * 16);
+    l.queries = p.q_lens ? p.q_lens[seq] : 1;
+    l.tiles = (l.ctx + 15) >> 4;
+    l.blocks = (l.queries * (p.hq / p.hkv) + 7) >> 3;
+    return l;
+}
+// A place on the line.
+struct Cursor {
+    int seq, kvh, block, tile;
+    Lengths len;
+    __device__ __forceinline__ void at_seq(const Q4AttnParams& p, int s) {  // the first sequence from s on that has work
+        kvh = block = tile = 0;
+        for (seq = s; seq < p.num_seqs; seq++) {
+            len = lengths_of(p, seq);
+            if (len.tiles * len.blocks > 0) return;
+        }
+    }
+    __device__ __forceinline__ void next_unit(const Q4AttnParams& p) {
+        tile = 0;
+        if (++block < len.blocks) return;
+        block = 0;
+        if (++kvh < p.hkv) return;
+        at_seq(p, seq + 1);
+    }
+};
+struct Part {  // what a run leaves of a unit that it shares with others
+    int seq, kvh, block, start, tiles, first, last;  // start: the unit's place on the line; records first .. last - 1 of its `tiles`
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(const Q4AttnParams p) {
+    using Rec = q4::Record<HD>;
+    constexpr int W = HD / 32;       // words of a lane per token (K) or token pair (V)
+    constexpr int KS = HD / 16, MT = HD / 16;
+    constexpr int kChunks = Rec::kBytes / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int s_off[kEntries + 1], s_warp[kWarps], s_last;
+    __shared__ Part s_part[2 * kWarps];
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int group = p.hq / p.hkv;
+    const int per = (p.num_seqs + kEntries - 1) / kEntries;  // sequences per entry
+    const int entries = (p.num_seqs + per - 1) / per;
+
+    // the line: first record of every entry
+    {
+        int carry = 0;
+        for (int base = 0; base < entries; base += kWarps * 32) {
+            const int e = base + threadIdx.x;
+            int n = 0;
+            for (int s = e * per; s < min(p.num_seqs, (e + 1) * per); s++) {
+                const Lengths l = lengths_of(p, s);
+                n += l.tiles * l.blocks * p.hkv;
+            }
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(kFull, incl, o);
+                if (lane >= o) incl += v;
+            }
+            if (lane == 31) s_warp[warp] = incl;
+            __syncthreads();
+            int before = carry;
+            for (int w = 0; w < warp; w++) before += s_warp[w];
+            if (e < entries) s_off[e] = before + incl - n;
+            for (int w = 0; w < kWarps; w++) carry += s_warp[w];
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) s_off[entries] = carry;
+        if (threadIdx.x < 2 * kWarps) s_part[threadIdx.x].tiles = 0;
+        __syncthreads();
+    }
+    // an empty context attends to nothing: rows of zeros
+    for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
+        const Lengths l = lengths_of(p, s);
+        if (l.tiles > 0) continue;
+        const size_t row = p.q_rows ? p.q_rows[s] : s;
+        for (int e = threadIdx.x; e < l.queries * p.hq * HD; e += kWarps * 32) p.out[row * p.hq * HD + e] = 0;
+    }
+    const int total = s_off[entries];
+    const int run = max(kMinRun, (total + (int)gridDim.x * kWarps - 1) / ((int)gridDim.x * kWarps));
+    const int block_start = blockIdx.x * kWarps * run;
+    if (block_start >= total) return;
+    int pos = min(block_start + warp * run, total);
+    const int end = min(pos + run, total);
+
+    const uint32_t ring = smem_u32(smem) + warp * kStages * Rec::kBytes;
+    float* const parts = reinterpret_cast<float*>(smem + ring_bytes<HD>());
+    const float to_log2 = p.scale_log2 * q4::kUnscale;
+
+    // writes a unit's finished columns: this lane's 16 (8) dims of columns 2c and 2c + 1, or nothing
+    auto out_row = [&](int seq, int kvh, int col) {
+        const int row = (p.q_rows ? p.q_rows[seq] : seq) + col / group;
+        return p.out + ((size_t)row * p.hq + (size_t)kvh * group + col % group) * HD;
+    };
+
+    if (pos < end) {
+        Cursor use, ask;
+        {
+            int lo = 0, hi = entries - 1;  // the last entry that begins at or before pos; of equal ones all but the last are empty
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (s_off[mid] <= pos)
+                    lo = mid;
+                else
+                    hi = mid - 1;
+            }
+            int left = pos - s_off[lo];
+            use.at_seq(p, lo * per);
+            while (left >= use.len.tiles * use.len.blocks * p.hkv) {
+                left -= use.len.tiles * use.len.blocks * p.hkv;
+                use.at_seq(p, use.seq + 1);
+            }
+            const int unit = left / use.len.tiles;
+            use.tile = left - unit * use.len.tiles;
+            use.kvh = unit / use.len.blocks;
+            use.block = unit - use.kvh * use.len.blocks;
+        }
+        ask = use;
+        int asked = pos, window = -1, record = -1;  // lane i holds the record number of tile window + i of ask's unit, -1 for none
+        uint32_t absent = 0;                         // bit s: the record of stage s lies on a page outside of the pool
+        auto issue = [&](int stage) {
+            if (asked < end) {
+                if (window < 0 || ask.tile - window >= 32) {
+                    window = ask.tile;
+                    const int tile = window + lane, index = tile / p.page_tiles;
+                    record = -1;
+                    if (tile < ask.len.tiles) {
+                        const int page = p.block_tables[(size_t)(p.bt_rows ? p.bt_rows[ask.seq] : ask.seq) * p.max_blocks + index];
+                        if (page >= 0 && page < p.n_pages) record = (page * p.hkv + ask.kvh) * p.page_tiles + tile - index * p.page_tiles;
+                    }
+                }
+                const int rec = __shfl_sync(kFull, record, ask.tile - window);
+                absent = (absent & ~(1u << stage)) | (rec < 0 ? 1u << stage : 0u);
+                if (rec >= 0) {
+                    const uint8_t* src = p.pool + (size_t)rec * Rec::kBytes;
+                    const uint32_t dst = ring + stage * Rec::kBytes;
+#pragma unroll
+                    for (int i = 0; i < kChunks; i += 32)
+                        if (i + 32 <= kChunks || i + lane < kChunks) cp_async16(dst + (i + lane) * 16, src + (i + lane) * 16);
+                }
+                asked++;
+                if (++ask.tile == ask.len.tiles) {
+                    ask.next_unit(p);
+                    window = -1;
+                }
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < kStages - 1; s++) issue(s);
+        int stage = 0;
+        bool first_of_run = true;
+        while (pos < end) {
+            const int t0 = use.tile, t1 = min(use.len.tiles, t0 + end - pos);
+            const int start = pos - t0;
+            // Q as the B operand, in the order of the nibbles; columns past the last are zeros
+            uint32_t qf[KS][2];
+            const int cols = min(8, use.len.queries * group - use.block * 8);
+            {
+                const int col = use.block * 8 + min(g, cols - 1);
+                const size_t row = (p.q_rows ? p.q_rows[use.seq] : use.seq) + col / group;
+                const uint16_t* q = p.q + (row * p.hq + (size_t)use.kvh * group + col % group) * HD + c * (HD / 4);
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    uint4 u = *reinterpret_cast<const uint4*>(q + 8 * w);
+                    if (g >= cols) u = make_uint4(0, 0, 0, 0);
+                    qf[2 * w][0] = prmt(u.x, u.z, 0x5410u);
+                    qf[2 * w][1] = prmt(u.x, u.z, 0x7632u);
+                    qf[2 * w + 1][0] = prmt(u.y, u.w, 0x5410u);
+                    qf[2 * w + 1][1] = prmt(u.y, u.w, 0x7632u);
+                }
+            }
+            // keys that columns 2c and 2c + 1 see; all columns see those before `sure`
+            const int hidden = use.len.ctx - use.len.queries + 1;
+            const int lim0 = hidden + (use.block * 8 + 2 * c) / group, lim1 = hidden + (use.block * 8 + 2 * c + 1) / group;
+            const int sure = hidden + use.block * 8 / group;
+            float m0 = kFloor, m1 = kFloor, l0 = 0.f, l1 = 0.f;
+            float o[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
+
+            for (int t = t0; t < t1; t++) {
+                cp_async_wait<kStages - 2>();
+                __syncwarp();  // everyone's copies have landed, and everyone is done with the stage that is asked into now
+                issue(stage == 0 ? kStages - 1 : stage - 1);
+                const uint8_t* rec = smem + (warp * kStages + stage) * Rec::kBytes;
+                const bool there = !(absent >> stage & 1);
+                stage = stage + 1 == kStages ? 0 : stage + 1;
+                if (!there) continue;
+                const int tok0 = t * 16;
+                // S^T[token, column]
+                float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+                {
+                    const uint32_t* sb = reinterpret_cast<const uint32_t*>(rec + Rec::kKsb) + (c * (HD / 4) / 64) * 16 + g;
+                    const q4::Scales qa = q4::scales_twice(sb[0]), qb = q4::scales_twice(sb[8]);
+                    uint32_t ka[W], kb[W];
+                    if constexpr (W == 4) {
+                        const uint4 a = *reinterpret_cast<const uint4*>(rec + lane * 16), b = *reinterpret_cast<const uint4*>(rec + 512 + lane * 16);
+                        ka[0] = a.x, ka[1] = a.y, ka[2] = a.z, ka[3] = a.w, kb[0] = b.x, kb[1] = b.y, kb[2] = b.z, kb[3] = b.w;
+                    } else {
+                        const uint2 a = *reinterpret_cast<const uint2*>(rec + lane * 8), b = *reinterpret_cast<const uint2*>(rec + 256 + lane * 8);
+                        ka[0] = a.x, ka[1] = a.y, kb[0] = b.x, kb[1] = b.y;
+                    }
+#pragma unroll
+                    for (int w = 0; w < W; w++) {
+                        uint32_t va[4], vb[4];
+                        q4::values(ka[w], qa, va);
+                        q4::values(kb[w], qb, vb);
+                        const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
+                        mma_bf16_16816(s, a0, qf[2 * w]);
+                        mma_bf16_16816(s2, a1, qf[2 * w + 1]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[j] = (s[j] + s2[j]) * to_log2;
+                const uint32_t* vsb = reinterpret_cast<const uint32_t*>(rec + Rec::kVsb) + (g * (HD / 8) / 64) * 16 + 2 * c;
+                uint2 sb0 = *reinterpret_cast<const uint2*>(vsb), sb1 = *reinterpret_cast<const uint2*>(vsb + 8);
+                if (tok0 + 16 > sure) {
+                    if (tok0 + g >= lim0) s[0] = -INFINITY;
+                    if (tok0 + g >= lim1) s[1] = -INFINITY;
+                    if (tok0 + g + 8 >= lim0) s[2] = -INFINITY;
+                    if (tok0 + g + 8 >= lim1) s[3] = -INFINITY;
+                    // what lies behind the context may be anything, and 0 * NaN is NaN
+                    if (tok0 + 2 * c >= use.len.ctx) sb0.x = 0;
+                    if (tok0 + 2 * c + 1 >= use.len.ctx) sb0.y = 0;
+                    if (tok0 + 2 * c + 8 >= use.len.ctx) sb1.x = 0;
+                    if (tok0 + 2 * c + 9 >= use.len.ctx) sb1.y = 0;
+                }
+                float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
+                if (__any_sync(kFull, mx0 > m0 + kSlack || mx1 > m1 + kSlack)) {
+#pragma unroll
+                    for (int sh = 4; sh <= 16; sh <<= 1) {
+                        mx0 = fmaxf(mx0, __shfl_xor_sync(kFull, mx0, sh));
+                        mx1 = fmaxf(mx1, __shfl_xor_sync(kFull, mx1, sh));
+                    }
+                    mx0 = fmaxf(m0, mx0), mx1 = fmaxf(m1, mx1);
+                    const float a0 = fast_exp2(m0 - mx0), a1 = fast_exp2(m1 - mx1);
+                    m0 = mx0, m1 = mx1;
+                    l0 *= a0, l1 *= a1;
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) o[mt][0] *= a0, o[mt][1] *= a1, o[mt][2] *= a0, o[mt][3] *= a1;
+                }
+                const float p0 = fast_exp2(s[0] - m0), p1 = fast_exp2(s[1] - m1), p2 = fast_exp2(s[2] - m0), p3 = fast_exp2(s[3] - m1);
+                l0 += p0 + p2;
+                l1 += p1 + p3;
+                uint32_t pb[2], pl[2];
+                {
+                    const uint32_t h01 = pack_bf2(p0, p1), h23 = pack_bf2(p2, p3);
+                    const uint32_t r01 = pack_bf2(p0 - bflo(h01), p1 - bfhi(h01)), r23 = pack_bf2(p2 - bflo(h23), p3 - bfhi(h23));
+                    pb[0] = movmatrix_trans(h01), pb[1] = movmatrix_trans(h23);
+                    pl[0] = movmatrix_trans(r01), pl[1] = movmatrix_trans(r23);
+                }
+                // O^T[dim, column]: rows g and g + 8 of tile mt are dims 2 mt and 2 mt + 1 of this lane's block
+                {
+                    const q4::Scales qa = q4::scales_pair(sb0.x, sb0.y), qb = q4::scales_pair(sb1.x, sb1.y);
+                    const uint8_t* v = rec + Rec::kV;
+                    uint32_t wa[W], wb[W];
+                    if constexpr (W == 4) {
+                        const uint4 a = *reinterpret_cast<const uint4*>(v + lane * 16), b = *reinterpret_cast<const uint4*>(v + 512 + lane * 16);
+                        wa[0] = a.x, wa[1] = a.y, wa[2] = a.z, wa[3] = a.w, wb[0] = b.x, wb[1] = b.y, wb[2] = b.z, wb[3] = b.w;
+                    } else {
+                        const uint2 a = *reinterpret_cast<const uint2*>(v + lane * 8), b = *reinterpret_cast<const uint2*>(v + 256 + lane * 8);
+                        wa[0] = a.x, wa[1] = a.y, wb[0] = b.x, wb[1] = b.y;
+                    }
+#pragma unroll
+                    for (int w = 0; w < W; w++) {
+                        uint32_t va[4], vb[4];
+                        q4::values(wa[w], qa, va);
+                        q4::values(wb[w], qb, vb);
+                        const uint32_t a0[4] = {va[0], va[1], vb[0], vb[1]}, a1[4] = {va[2], va[3], vb[2], vb[3]};
+                        mma_bf16_16816(o[2 * w], a0, pb);
+                        mma_bf16_16816(o[2 * w + 1], a1, pb);
+                        mma_bf16_16816(o[2 * w], a0, pl);
+                        mma_bf16_16816(o[2 * w + 1], a1, pl);
+                    }
+                }
+            }
+            pos += t1 - t0;
+#pragma unroll
+            for (int sh = 4; sh <= 16; sh <<= 1) {
+                l0 += __shfl_xor_sync(kFull, l0, sh);
+                l1 += __shfl_xor_sync(kFull, l1, sh);
+            }
+            if (t0 == 0 && t1 == use.len.tiles) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int col = 2 * c + h;
+                    if (col >= cols) continue;
+                    const float l = h ? l1 : l0, f = l == 0.f ? 0.f : q4::kUnscale / l;
+                    uint32_t v[MT];
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) v[mt] = pack_bf2(o[mt][h] * f, o[mt][h + 2] * f);
+                    uint4* dst = reinterpret_cast<uint4*>(out_row(use.seq, use.kvh, use.block * 8 + col) + g * (HD / 8));
+#pragma unroll
+                    for (int i = 0; i < MT / 4; i++) dst[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+            } else {
+                // the first part of a run has a place of its own; the last one lies where the run's records were
+                if (!first_of_run) __syncwarp();
+                float* dst = first_of_run ? parts + warp * part_floats<HD>() : reinterpret_cast<float*>(smem + warp * kStages * Rec::kBytes);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    const int d = g * (HD / 8) + 2 * mt;
+                    *reinterpret_cast<float2*>(dst + (2 * c) * HD + d) = make_float2(o[mt][0], o[mt][2]);
+                    *reinterpret_cast<float2*>(dst + (2 * c + 1) * HD + d) = make_float2(o[mt][1], o[mt][3]);
+                }
+                if (g == 0) {
+                    dst[8 * HD + 2 * c] = m0, dst[8 * HD + 2 * c + 1] = m1;
+                    dst[8 * HD + 8 + 2 * c] = l0, dst[8 * HD + 8 + 2 * c + 1] = l1;
+                }
+                if (lane == 0) s_part[2 * warp + !first_of_run] = Part{use.seq, use.kvh, use.block, start, use.len.tiles, t0, t1};
+            }
+            first_of_run = false;
+            use.tile = t1;
+            if (t1 == use.len.tiles) use.next_unit(p);
+        }
+    }
+    __syncthreads();
+
+    // ---- the block's parts, unit by unit in the order of the line
+    auto part_at = [&](int i) { return (i & 1) ? reinterpret_cast<const float*>(smem + (i >> 1) * kStages * Rec::kBytes) : parts + (i >> 1) * part_floats<HD>(); };
+    constexpr int kPer = 8 * HD / (kWarps * 32);  // outputs of a thread
+    int crossing[2] = {-1, -1};                   // parts of the units that other blocks share: this block's first and its last one
+    for (int i = 0; i < 2 * kWarps;) {
+        if (s_part[i].tiles == 0) {
+            i++;
+            continue;
+        }
+        const Part u = s_part[i];
+        int n = i + 1, last = u.last;
+        for (; n < 2 * kWarps && (s_part[n].tiles == 0 || s_part[n].start == u.start); n++)
+            if (s_part[n].tiles) last = s_part[n].last;
+        const bool whole = u.first == 0 && last == u.tiles;
+        const int cols = min(8, (p.q_lens ? p.q_lens[u.seq] : 1) * group - u.block * 8);
+        const int side = u.start <= block_start ? 0 : 1;
+        float* const dst = p.parts + (size_t)(blockIdx.x * 2 + side) * part_floats<HD>();
+#pragma unroll
+        for (int k = 0; k < kPer; k++) {
+            const int e = threadIdx.x + k * kWarps * 32, col = e / HD;
+            if (col >= cols) break;
+            float m = kFloor, l = 0.f, sum = 0.f;
+            for (int j = i; j < n; j++)
+                if (s_part[j].tiles) m = fmaxf(m, part_at(j)[8 * HD + col]);
+            for (int j = i; j < n; j++)
+                if (s_part[j].tiles) {
+                    const float* part = part_at(j);
+                    const float f = fast_exp2(part[8 * HD + col] - m);
+                    l += part[8 * HD + 8 + col] * f;
+                    sum += part[e] * f;
+                }
+            if (whole) {
+                out_row(u.seq, u.kvh, u.block * 8 + col)[e % HD] = f2bf(l == 0.f ? 0.f : sum * (q4::kUnscale / l));
+            } else {
+                dst[e] = sum;
+                if (e % HD == 0) dst[8 * HD + col] = m, dst[8 * HD + 8 + col] = l;
+            }
+        }
+        if (!whole) crossing[side] = i;
+        i = n;
+    }
+    // ---- units of several blocks: whoever arrives last adds up their parts
+    const int block_run = kWarps * run;
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+        if (crossing[side] < 0) continue;
+        const Part u = s_part[crossing[side]];
+        const int from = u.start / block_run, to = (u.start + u.tiles - 1) / block_run;
+        __threadfence();  // this block's part is visible before its arrival is counted
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            s_last = atomicAdd(p.counters + from, 1) == to - from;
+            if (s_last) p.counters[from] = 0;
+        }
+        __syncthreads();
+        if (!s_last) continue;
+        __threadfence();
+        const int cols = min(8, (p.q_lens ? p.q_lens[u.seq] : 1) * group - u.block * 8);
+        auto part = [&](int b) { return p.parts + (size_t)(b * 2 + (u.start <= b * block_run ? 0 : 1)) * part_floats<HD>(); };
+#pragma unroll
+        for (int k = 0; k < kPer; k++) {
+            const int e = threadIdx.x + k * kWarps * 32, col = e / HD;
+            if (col >= cols) break;
+            float m = kFloor, l = 0.f, sum = 0.f;
+            for (int b = from; b <= to; b++) m = fmaxf(m, __ldcg(part(b) + 8 * HD + col));
+#pragma unroll 4
+            for (int b = from; b <= to; b++) {
+                const float f = fast_exp2(__ldcg(part(b) + 8 * HD + col) - m);
+                l += __ldcg(part(b) + 8 * HD + 8 + col) * f;
+                sum += __ldcg(part(b) + e) * f;
+            }
+            out_row(u.seq, u.kvh, u.block * 8 + col)[e % HD] = f2bf(l == 0.f ? 0.f : sum * (q4::kUnscale / l));
+        }
+    }
+}
+
+template <int HD>
+int32_t launch(b2_ctx* ctx, Q4AttnParams p) {
+    const int grid = kBlocksPerSm * ctx->sm_count;
+    if (!ctx->q4_parts) {  // two parts per block, and an arrival counter each (zero between launches)
+        const size_t bytes = (size_t)grid * (2 * part_floats<128>() + 1) * 4;
+        B2_CUDA(cudaMalloc((void**)&ctx->q4_parts, bytes));
+        B2_CUDA(cudaMemsetAsync(ctx->q4_parts, 0, bytes, ctx->stream));
+    }
+    p.parts = ctx->q4_parts;
+    p.counters = reinterpret_cast<int*>(ctx->q4_parts + (size_t)grid * 2 * part_floats<128>());
+    B2_SMEM_ONCE(ctx, kv_q4_attn_kernel<HD>, smem_bytes<HD>());
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_attn_kernel<HD>, dim3(grid), dim3(kWarps * 32), (size_t)smem_bytes<HD>(), ctx->stream, p));
+    B2_LAUNCHED(ctx);
+    B2_CUDA(cudaGetLastError());
+    return B2_OK;
+}
+
+}  // namespace
+
+int32_t b2_kv_q4_check(const char* who, const void* pool, int64_t n_pages, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size) {
+    const std::string name = who;
+    B2_REQUIRE(hkv > 0 && hq > 0 && hq % hkv == 0, B2_ERR_MSG, name + ": hq must be a multiple of hkv");
+    B2_REQUIRE(head_dim == 64 || head_dim == 128, B2_ERR_UNSUPPORTED, name + ": head_dim must be 64 or 128");
+    B2_REQUIRE(page_size > 0 && page_size % 16 == 0, B2_ERR_UNSUPPORTED, name + ": page_size must be a multiple of 16");
+    B2_REQUIRE(n_pages > 0 && n_pages * page_size < (1ll << 31) && n_pages * hkv * (page_size / 16) < (1ll << 31), B2_ERR_MSG,
+               name + ": the pool must have pages, and fewer than 2^31 tokens and records");
+    B2_REQUIRE(((uintptr_t)pool & 15) == 0, B2_ERR_UNSUPPORTED, name + ": the pool must be 16-byte aligned");
+    return B2_OK;
+}
+
+int32_t b2_kv_q4_attn_launch(b2_ctx* ctx, const Q4AttnParams& p, int head_dim) {
+    if (p.num_seqs <= 0) return B2_OK;
+    return head_dim == 128 ? launch<128>(ctx, p) : launch<64>(ctx, p);
+}
+
+extern "C" int64_t b2_kv_q4_pool_bytes(int64_t n_pages, int32_t hkv, int32_t head_dim, int32_t page_size) {
+    if (b2_kv_q4_check("b2_kv_q4_pool_bytes", nullptr, n_pages, hkv, hkv, head_dim, page_size) != B2_OK) return 0;
+    return n_pages * hkv * (page_size / 16) * q4::record_bytes(head_dim);
+}
+
+extern "C" int32_t b2_paged_attn_decode_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_t* kv_pool_dev, int32_t n_pages, const int32_t* block_tables_dev,
+                                           int32_t max_blocks, const int32_t* ctx_lens_dev, int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim,
+                                           int32_t page_size, float scale, uint16_t* out_dev) {
+    B2_REQUIRE(ctx && q_dev && kv_pool_dev && block_tables_dev && ctx_lens_dev && out_dev, B2_ERR_MSG, "b2_paged_attn_decode_q4: null argument");
+    B2_CHECK(b2_kv_q4_check("b2_paged_attn_decode_q4", kv_pool_dev, n_pages, hq, hkv, head_dim, page_size));
+    B2_REQUIRE(num_seqs >= 0 && max_blocks > 0, B2_ERR_MSG, "b2_paged_attn_decode_q4: bad sizes");
+    B2_REQUIRE((double)num_seqs * max_blocks * (page_size / 16) * hkv * ((hq / hkv + 7) / 8) < 1073741824.0, B2_ERR_UNSUPPORTED,
+               "b2_paged_attn_decode_q4: the block tables reach more than 2^30 records; make fewer sequences a call");
+    B2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & 15) == 0, B2_ERR_UNSUPPORTED, "b2_paged_attn_decode_q4: q and out must be 16-byte aligned");
+    B2_CUDA(cudaSetDevice(ctx->device));
+    Q4AttnParams p{};
+    p.q = q_dev;
+    p.pool = kv_pool_dev;
+    p.n_pages = n_pages;
+    p.block_tables = block_tables_dev;
+    p.max_blocks = max_blocks;
+    p.ctx_lens = ctx_lens_dev;
+    p.num_seqs = num_seqs;
+    p.hq = hq;
+    p.hkv = hkv;
+    p.page_tiles = page_size / 16;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.out = out_dev;
+    return b2_kv_q4_attn_launch(ctx, p, head_dim);
+}

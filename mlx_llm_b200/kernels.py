@@ -29,6 +29,31 @@ def paged_attn_prefill(ctx, q, k_pool, v_pool, block_tables, max_blocks, cu_seql
                                        int(cl.size), int(hq), int(hkv), int(head_dim), int(page_size), C.c_float(scale), ptr(out)))
 
 
+def kv_q4_pool_bytes(n_pages, hkv, head_dim, page_size):
+    lib = load()
+    lib.b2_kv_q4_pool_bytes.restype = C.c_int64
+    return lib.b2_kv_q4_pool_bytes(C.c_int64(n_pages), int(hkv), int(head_dim), int(page_size))
+
+
+def rope_kv_append_q4(ctx, qkv, T, hq, hkv, head_dim, positions, slot_mapping, cos, sin, q_norm, k_norm, eps, page_size, kv_pool, n_pages, q_out,
+                      k_out=None, v_out=None):
+    check(load().b2_rope_kv_append_q4(ctx.h, ptr(qkv), int(T), int(hq), int(hkv), int(head_dim), ptr(positions), ptr(slot_mapping), ptr(cos), ptr(sin),
+                                      ptr(q_norm), ptr(k_norm), C.c_float(eps), int(page_size), ptr(kv_pool), int(n_pages), ptr(q_out), ptr(k_out),
+                                      ptr(v_out)))
+
+
+def paged_attn_decode_q4(ctx, q, kv_pool, n_pages, block_tables, ctx_lens, num_seqs, hq, hkv, head_dim, page_size, scale, out, max_blocks):
+    check(load().b2_paged_attn_decode_q4(ctx.h, ptr(q), ptr(kv_pool), int(n_pages), ptr(block_tables), int(max_blocks), ptr(ctx_lens), int(num_seqs),
+                                         int(hq), int(hkv), int(head_dim), int(page_size), C.c_float(scale), ptr(out)))
+
+
+def paged_attn_prefill_q4(ctx, q, kv_pool, n_pages, block_tables, max_blocks, cu_seqlens, ctx_lens, hq, hkv, head_dim, page_size, scale, out):
+    cu = np.ascontiguousarray(cu_seqlens, np.int32)
+    cl = np.ascontiguousarray(ctx_lens, np.int32)
+    check(load().b2_paged_attn_prefill_q4(ctx.h, ptr(q), ptr(kv_pool), int(n_pages), ptr(block_tables), int(max_blocks), ptr(cu), ptr(cl), int(cl.size),
+                                          int(hq), int(hkv), int(head_dim), int(page_size), C.c_float(scale), ptr(out)))
+
+
 def quantize(ctx, w, out_dim, in_dim, bits, packed, scales, biases, group=64):
     check(load().b2_quantize(ctx.h, ptr(w), C.c_int64(out_dim), C.c_int64(in_dim), int(group), int(bits), ptr(packed), ptr(scales),
                              ptr(biases)))
@@ -88,6 +113,24 @@ def embed(ctx, table, ids, n, dim, vocab, out):
 
 def argmax(ctx, logits, rows, vocab, out):
     check(load().b2_argmax(ctx.h, ptr(logits), int(rows), int(vocab), ptr(out)))
+
+
+class LogitRules(C.Structure):
+    """b2_logit_rules: device pointers, null where a rule is not used."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("history", "history_off", "n_prompt", "repetition", "presence", "frequency", "bias_id", "bias_value", "bias_off",
+                                          "mask")] + [("mask_words", C.c_int64), ("mask_row", C.c_void_p)]
+
+
+def logit_rules(mask_words=0, **arrays):
+    """Rules for logits_adjust: history, history_off, n_prompt, repetition, presence, frequency, bias_id, bias_value, bias_off, mask, mask_row as device
+    buffers (None: not used), and the words of a mask's row."""
+    return LogitRules(mask_words=int(mask_words), **{n: ptr(a) for n, a in arrays.items()})
+
+
+def logits_adjust(ctx, logits, rows, vocab, rules, f32=False, ld=None, out=None, argmax=None):
+    check(load().b2_logits_adjust(ctx.h, ptr(logits), int(f32), int(rows), int(vocab), C.c_int64(vocab if ld is None else ld), C.byref(rules), ptr(out),
+                                  ptr(argmax)))
 
 
 def rope_inv_freq(head_dim, theta, kind=0, factor=1.0, low=1.0, high=4.0, orig=8192.0):
