@@ -6,24 +6,81 @@
 // (e the maximum in a tie; halves away from zero).  Codes are taken for the scale as it is stored, so that its rounding costs nothing
 // again; all values equal: scale 0.  A NaN or an infinity makes the scale a NaN, and with it the group's values, as they would be in bf16.
 //
-// One warp per (token, head); a lane owns HD/64 adjacent elements of each half.
+// Bound by HBM (6151 tokens of 64 + 16 heads: 261 MB) once the instructions are few: HD / 16 lanes take a head, each 8 adjacent dims of
+// either half, so that reads and writes are 16 bytes, the rotation's roundings come with bf16x2 instructions (a product or a sum of two
+// bf16 numbers rounded once is what they give), a lane's codes of a group are one word, and a warp has HD 128: 4, HD 64: 8 heads.
+// Queries, keys and values are warps of their own.
 #include "kernels.h"
 #include "kv_q4.cuh"
 
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
+constexpr int kWarps = 4;
 
-__device__ __forceinline__ float warp_min_nan(float v) {
-    float r;
-    asm("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;\n" : "=f"(r) : "f"(v));
-    return r;
+__device__ __forceinline__ uint32_t add_bf2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.bf16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
+    return d;
 }
-__device__ __forceinline__ float warp_max_nan(float v) {
-    float r;
-    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;\n" : "=f"(r) : "f"(v));
-    return r;
+__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
+    return d;
 }
+struct Eight {
+    uint32_t w[4];
+    __device__ __forceinline__ float operator[](int i) const { return i & 1 ? bfhi(w[i >> 1]) : bflo(w[i >> 1]); }
+};
+__device__ __forceinline__ Eight load8(const uint16_t* p) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    return {{v.x, v.y, v.z, v.w}};
+}
+__device__ __forceinline__ void store8(uint16_t* p, const Eight& v) { *reinterpret_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]); }
+
+// Per-head RMSNorm of queries: rope_kv.cu's sum, term for term (its lane l has dims HD/32 l of either half, and it adds lanes 16, 8, ... 1
+// apart), so that a model's queries do not depend on what holds its cache.
+template <int HD>
+__device__ __forceinline__ void norm_query(Eight& a, Eight& b, const Eight& wa, const Eight& wb, float eps) {
+    constexpr int L = HD / 16, V = HD / 64, P = 8 / V;  // lanes of a head, elements and lanes of the other kernel
+    float ss[P];
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        ss[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; j++) ss[i] += a[i * V + j] * a[i * V + j] + b[i * V + j] * b[i * V + j];
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < P; i++) ss[i] += __shfl_xor_sync(kFull, ss[i], o);
+#pragma unroll
+    for (int o = P / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; i++) ss[i] += ss[i + o];
+    const float inv = 1.0f / sqrtf(ss[0] / (float)HD + eps);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        a.w[i] = pack_bf2(a[2 * i] * inv * wa[2 * i], a[2 * i + 1] * inv * wa[2 * i + 1]);
+        b.w[i] = pack_bf2(b[2 * i] * inv * wb[2 * i], b[2 * i + 1] * inv * wb[2 * i + 1]);
+    }
+}
+// ... of keys: in f64, since one bit of a group's farthest value moves its scale, and with it the whole group.
+template <int HD>
+__device__ __forceinline__ void norm_key(Eight& a, Eight& b, const Eight& wa, const Eight& wb, float eps) {
+    double ss = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) ss += (double)a[i] * a[i] + (double)b[i] * b[i];
+#pragma unroll
+    for (int o = HD / 32; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+    const double inv = 1.0 / sqrt(ss / HD + (double)eps);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        a.w[i] = pack_bf2((float)(a[2 * i] * wa[2 * i] * inv), (float)(a[2 * i + 1] * wa[2 * i + 1] * inv));
+        b.w[i] = pack_bf2((float)(b[2 * i] * wb[2 * i] * inv), (float)(b[2 * i + 1] * wb[2 * i + 1] * inv));
+    }
+}
+
 struct Group {
     float scale, edge;  // (the scale as stored)
 };
@@ -31,122 +88,131 @@ __device__ __forceinline__ Group group_of(float lo, float hi) {
     const float edge = fabsf(lo) > fabsf(hi) ? lo : hi, span = hi - lo;
     if (span == 0.f) return {0.f, edge};
     const float scale = rbf(__fdiv_rn(-edge, roundf(__fdiv_rn(15.f * fabsf(edge), span))));
-    // a bias of infinity is a NaN too: 0 scale + bias would keep it
     return {isfinite(span) ? scale : __int_as_float(0x7fc00000), edge};
 }
-__device__ __forceinline__ uint32_t code_of(float x, const Group& q) {
-    return q.scale == 0.f ? 0u : (uint32_t)fminf(fmaxf(roundf(__fdiv_rn(x - q.edge, q.scale)), 0.f), 15.f);
+// smallest and largest of a lane's eight; NaN where one is NaN or infinite (0 x is, then)
+__device__ __forceinline__ void ends_of(const Eight& v, float& lo, float& hi) {
+    lo = hi = v[0];
+    float bad = 0.f * v[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        lo = fminf(lo, v[i]), hi = fmaxf(hi, v[i]);
+        bad = fmaf(0.f, v[i], bad);
+    }
+    lo += bad, hi += bad;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The eight codes of a lane, lowest nibble first.  The quotient comes from a reciprocal; what it misses is put right by the sign of an fma:
+// (x - edge) / scale is never negative, and halves go up.
+__device__ __forceinline__ uint32_t codes_of(const Eight& v, const Group& q) {
+    const float s = fabsf(q.scale), inv = s > 0.f ? __fdividef(1.f, s) : 0.f, half = 0.5f * s;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float d = fabsf(v[i] - q.edge);
+        const float magic = fminf(d * inv, 15.f) + 8388608.f;  // 2^23: the sum's low bits are the whole number
+        const float r = fmaf(8388608.f - magic, s, d);         // d - code s
+        int code = (__float_as_int(magic) & 31) + (r >= half) - (r < -half);
+        code = s > 0.f ? min(max(code, 0), 15) : 0;
+        word |= (uint32_t)code << (4 * i);
+    }
+    return word;
+}
+// the values that codes stand for
+__device__ __forceinline__ Eight values_of(uint32_t word, const Group& q) {
+    const uint32_t s2 = pack_bf2(q.scale, q.scale), e2 = pack_bf2(q.edge, q.edge);
+    Eight v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v.w[i] = fma_bf2(pack_bf2((float)(word >> (8 * i) & 15), (float)(word >> (8 * i + 4) & 15)), s2, e2);
+    return v;
 }
 
 template <int HD>
-__global__ void rope_kv_q4_kernel(const RopeKvQ4Params a) {
-    constexpr int V = HD / 64;  // elements per lane per half (1 or 2)
+__global__ void __launch_bounds__(kWarps * 32) rope_kv_q4_kernel(const RopeKvQ4Params a, int q_blocks, int kv_blocks) {
     using Rec = q4::Record<HD>;
+    constexpr int L = HD / 16;  // lanes of a head
     const RopeKvParams& p = a.rope;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     pdl_wait();
-    const int heads_total = p.hq + 2 * p.hkv;
-    const int wid = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (wid >= p.T * heads_total) return;
-    const int lane = threadIdx.x & 31;
-    const int tok = wid / heads_total, head = wid % heads_total;
-    const uint16_t* src = p.qkv + (size_t)tok * p.ld + (size_t)head * HD;
-    const bool is_q = head < p.hq, is_k = !is_q && head < p.hq + p.hkv;
-    float x1[V], x2[V];  // first-half and second-half elements of this lane
-    if (V == 2) {
-        const uint32_t lo = reinterpret_cast<const uint32_t*>(src)[lane], hi = reinterpret_cast<const uint32_t*>(src)[32 + lane];
-        x1[0] = bflo(lo), x1[V - 1] = bfhi(lo);
-        x2[0] = bflo(hi), x2[V - 1] = bfhi(hi);
-    } else {
-        x1[0] = bf2f(src[lane]);
-        x2[0] = bf2f(src[32 + lane]);
-    }
-    if (is_q || is_k) {
-        const uint16_t* nw = is_q ? p.q_norm : p.k_norm;
+    const int kind = blockIdx.x < q_blocks ? 0 : blockIdx.x < q_blocks + kv_blocks ? 1 : 2;  // queries, keys, values
+    const int block = blockIdx.x - (kind == 0 ? 0 : kind == 1 ? q_blocks : q_blocks + kv_blocks);
+    const int lane = threadIdx.x & 31, j = lane % L;
+    const int heads = kind == 0 ? p.hq : p.hkv;
+    const int item = (block * kWarps + (threadIdx.x >> 5)) * (32 / L) + lane / L;
+    const bool real = item < p.T * heads;  // (lanes without a head go through the motions of the last one)
+    const int tok = (real ? item : p.T * heads - 1) / heads, head = (real ? item : p.T * heads - 1) - tok * heads;
+    const uint16_t* src = p.qkv + (size_t)tok * p.ld + (size_t)(head + (kind == 0 ? 0 : kind == 1 ? p.hq : p.hq + p.hkv)) * HD + 8 * j;
+    Eight x = load8(src), y = load8(src + HD / 2);
+    if (kind < 2) {
+        const size_t at = (size_t)p.positions[tok] * (HD / 2) + 8 * j;
+        const Eight c = load8(p.cos_table + at), s = load8(p.sin_table + at);
+        const uint16_t* nw = kind == 0 ? p.q_norm : p.k_norm;
         if (nw) {
-            float ss = 0.f;
-#pragma unroll
-            for (int j = 0; j < V; j++) ss += x1[j] * x1[j] + x2[j] * x2[j];
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-            const float inv = 1.0f / sqrtf(ss / (float)HD + p.eps);
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                x1[j] = rbf(x1[j] * inv * bf2f(nw[lane * V + j]));
-                x2[j] = rbf(x2[j] * inv * bf2f(nw[HD / 2 + lane * V + j]));
-            }
+            const Eight wa = load8(nw + 8 * j), wb = load8(nw + HD / 2 + 8 * j);
+            if (kind == 0)
+                norm_query<HD>(x, y, wa, wb, p.eps);
+            else
+                norm_key<HD>(x, y, wa, wb, p.eps);
         }
-        const int pos = p.positions[tok];
-        const uint16_t* ct = p.cos_table + (size_t)pos * (HD / 2);
-        const uint16_t* st = p.sin_table + (size_t)pos * (HD / 2);
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            const float c = bf2f(ct[lane * V + j]), s = bf2f(st[lane * V + j]);
-            const float y1 = rbf(rbf(x1[j] * c) + rbf(-x2[j] * s)), y2 = rbf(rbf(x2[j] * c) + rbf(x1[j] * s));
-            x1[j] = y1, x2[j] = y2;
+        for (int i = 0; i < 4; i++) {
+            const uint32_t u = sub_bf2(mul_bf2(x.w[i], c.w[i]), mul_bf2(y.w[i], s.w[i])), v = add_bf2(mul_bf2(y.w[i], c.w[i]), mul_bf2(x.w[i], s.w[i]));
+            x.w[i] = u, y.w[i] = v;
         }
     }
-    if (is_q) {
-        uint16_t* dst = p.q_out + ((size_t)tok * p.hq + head) * HD;
-        if (V == 2) {
-            reinterpret_cast<uint32_t*>(dst)[lane] = pack_bf2(x1[0], x1[V - 1]);
-            reinterpret_cast<uint32_t*>(dst)[32 + lane] = pack_bf2(x2[0], x2[V - 1]);
-        } else {
-            dst[lane] = f2bf(x1[0]);
-            dst[32 + lane] = f2bf(x2[0]);
+    if (kind == 0) {
+        if (real) {
+            uint16_t* dst = p.q_out + ((size_t)tok * p.hq + head) * HD + 8 * j;
+            store8(dst, x);
+            store8(dst + HD / 2, y);
         }
         return;
     }
-    const int kvh = head - p.hq - (is_k ? 0 : p.hkv);
-    Group q1, q2;  // of the first and the second half; one group for both at head size 64
-    if (V == 2) {
-        q1 = group_of(warp_min_nan(fminf(x1[0], x1[V - 1]) + 0.f * (x1[0] + x1[V - 1])), warp_max_nan(fmaxf(x1[0], x1[V - 1])));
-        q2 = group_of(warp_min_nan(fminf(x2[0], x2[V - 1]) + 0.f * (x2[0] + x2[V - 1])), warp_max_nan(fmaxf(x2[0], x2[V - 1])));
-    } else {
-        q1 = q2 = group_of(warp_min_nan(fminf(x1[0], x2[0]) + 0.f * (x1[0] + x2[0])), warp_max_nan(fmaxf(x1[0], x2[0])));
+    const bool is_k = kind == 1;
+    float lo1, hi1, lo2, hi2;
+    ends_of(x, lo1, hi1);
+    ends_of(y, lo2, hi2);
+    if (Rec::kGroups == 1) lo1 = lo2 = min_nan(lo1, lo2), hi1 = hi2 = max_nan(hi1, hi2);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+        lo1 = min_nan(lo1, __shfl_xor_sync(kFull, lo1, o)), hi1 = max_nan(hi1, __shfl_xor_sync(kFull, hi1, o));
+        if (Rec::kGroups == 2) lo2 = min_nan(lo2, __shfl_xor_sync(kFull, lo2, o)), hi2 = max_nan(hi2, __shfl_xor_sync(kFull, hi2, o));
     }
-    uint32_t c1[V], c2[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) c1[j] = code_of(x1[j], q1), c2[j] = code_of(x2[j], q2);
+    const Group q1 = group_of(lo1, hi1), q2 = Rec::kGroups == 2 ? group_of(lo2, hi2) : q1;
+    const uint32_t c1 = codes_of(x, q1), c2 = codes_of(y, q2);
     const int slot = p.slot_mapping[tok];
-    if (slot >= 0 && slot < a.n_slots) {
-        const int page = slot / p.page_size, off = slot % p.page_size, t = off & 15;
-        uint8_t* rec = a.pool + (((size_t)page * p.hkv + kvh) * (p.page_size >> 4) + (off >> 4)) * Rec::kBytes;
-        // a byte of a token's row holds dims 2b, 2b + 1: this lane's of either half, or, at head size 64, a pair of lanes'
-        uint32_t b1, b2;
-        if (V == 2) {
-            b1 = c1[0] | c1[V - 1] << 4, b2 = c2[0] | c2[V - 1] << 4;
-        } else {
-            b1 = c1[0] | __shfl_down_sync(kFull, c1[0], 1) << 4, b2 = c2[0] | __shfl_down_sync(kFull, c2[0], 1) << 4;
-        }
-        if (V == 2 || (lane & 1) == 0) {
-            const int at = V == 2 ? lane : lane >> 1;
+    if (real && slot >= 0 && slot < a.n_slots) {
+        const int page = slot / p.page_size, off = slot - page * p.page_size, t = off & 15;
+        uint8_t* rec = a.pool + (((size_t)page * p.hkv + head) * (p.page_size >> 4) + (off >> 4)) * Rec::kBytes;
+        if (is_k) {  // a word has eight dims
+            uint32_t* row = reinterpret_cast<uint32_t*>(rec) + t * (HD / 8) + j;
+            row[0] = c1;
+            row[HD / 16] = c2;
+        } else {  // a half word has four: word d of block g, for dims 8 j + 4 i and HD/2 + 8 j + 4 i
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const int b = at + half * (HD / 4);
-                int where = t * (HD / 2) + b;
-                if (!is_k) {
-                    constexpr int per = HD / 16;  // bytes of a token in a block
-                    where = Rec::kV + ((((t >> 3) * 8 + b / per) * 4 + ((t & 7) >> 1)) * (HD / 32) + (b % per >> 1)) * 4 + (t & 1) * 2 + (b & 1);
-                }
-                rec[where] = (uint8_t)(half ? b2 : b1);
+            for (int i = 0; i < 4; i++) {
+                const int d = (i >> 1) * (HD / 2) + 8 * j + 4 * (i & 1);
+                const int word = (((t >> 3) * 8 + d / (HD / 8)) * 4 + ((t & 7) >> 1)) * (HD / 32) + d % (HD / 8) / 4;
+                reinterpret_cast<uint16_t*>(rec + Rec::kV)[2 * word + (t & 1)] = (uint16_t)((i >> 1 ? c2 : c1) >> (16 * (i & 1)));
             }
         }
-        if (lane < Rec::kGroups)
-            reinterpret_cast<uint32_t*>(rec + (is_k ? Rec::kKsb : Rec::kVsb))[lane * 16 + t] = pack_bf2(lane ? q2.scale : q1.scale, lane ? q2.edge : q1.edge);
+        if (j < Rec::kGroups)
+            reinterpret_cast<uint32_t*>(rec + (is_k ? Rec::kKsb : Rec::kVsb))[j * 16 + t] = pack_bf2(j ? q2.scale : q1.scale, j ? q2.edge : q1.edge);
     }
     uint16_t* dst = is_k ? a.k_out : a.v_out;
-    if (dst) {
-        dst += ((size_t)tok * p.hkv + kvh) * HD;
-        const uint32_t s1 = pack_bf2(q1.scale, q1.scale), e1 = pack_bf2(q1.edge, q1.edge), s2 = pack_bf2(q2.scale, q2.scale), e2 = pack_bf2(q2.edge, q2.edge);
-        const uint32_t v1 = fma_bf2(pack_bf2((float)c1[0], (float)c1[V - 1]), s1, e1), v2 = fma_bf2(pack_bf2((float)c2[0], (float)c2[V - 1]), s2, e2);
-        if (V == 2) {
-            reinterpret_cast<uint32_t*>(dst)[lane] = v1;
-            reinterpret_cast<uint32_t*>(dst)[32 + lane] = v2;
-        } else {
-            dst[lane] = (uint16_t)v1;
-            dst[32 + lane] = (uint16_t)v2;
-        }
+    if (dst && real) {
+        dst += ((size_t)tok * p.hkv + head) * HD + 8 * j;
+        store8(dst, values_of(c1, q1));
+        store8(dst + HD / 2, values_of(c2, q2));
     }
 }
 
@@ -155,11 +221,10 @@ __global__ void rope_kv_q4_kernel(const RopeKvQ4Params a) {
 int32_t b2_rope_kv_q4_launch(b2_ctx* ctx, const RopeKvQ4Params& a) {
     const RopeKvParams& p = a.rope;
     if (p.T <= 0) return B2_OK;
-    const long warps = (long)p.T * (p.hq + 2 * p.hkv);
-    const int wpb = 8;
-    const unsigned grid = (unsigned)((warps + wpb - 1) / wpb);
+    const int per = kWarps * 512 / p.hd;  // heads of a block
+    const int q_blocks = (int)(((long)p.T * p.hq + per - 1) / per), kv_blocks = (int)(((long)p.T * p.hkv + per - 1) / per);
     auto kernel = p.hd == 128 ? rope_kv_q4_kernel<128> : rope_kv_q4_kernel<64>;
-    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kernel, dim3(grid), dim3(wpb * 32), 0, ctx->stream, a));
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kernel, dim3(q_blocks + 2 * kv_blocks), dim3(kWarps * 32), 0, ctx->stream, a, q_blocks, kv_blocks));
     B2_LAUNCHED(ctx);
     B2_CUDA(cudaGetLastError());
     return B2_OK;
@@ -173,8 +238,9 @@ extern "C" int32_t b2_rope_kv_append_q4(b2_ctx* ctx, const uint16_t* qkv_dev, in
                "b2_rope_kv_append_q4: null argument");
     B2_CHECK(b2_kv_q4_check("b2_rope_kv_append_q4", kv_pool_dev, n_pages, hq, hkv, head_dim, page_size));
     B2_REQUIRE((long)T * (hq + 2 * hkv) < (1l << 31), B2_ERR_UNSUPPORTED, "b2_rope_kv_append_q4: too many tokens for one call");
-    B2_REQUIRE((((uintptr_t)qkv_dev | (uintptr_t)q_out_dev | (uintptr_t)k_out_dev | (uintptr_t)v_out_dev) & 3) == 0, B2_ERR_UNSUPPORTED,
-               "b2_rope_kv_append_q4: qkv, q_out, k_out and v_out must be 4-byte aligned");
+    B2_REQUIRE((((uintptr_t)qkv_dev | (uintptr_t)q_out_dev | (uintptr_t)k_out_dev | (uintptr_t)v_out_dev | (uintptr_t)cos_dev | (uintptr_t)sin_dev |
+                 (uintptr_t)q_norm_dev | (uintptr_t)k_norm_dev) & 15) == 0,
+               B2_ERR_UNSUPPORTED, "b2_rope_kv_append_q4: bf16 arrays must be 16-byte aligned");
     RopeKvQ4Params a{};
     RopeKvParams& p = a.rope;
     p.qkv = const_cast<uint16_t*>(qkv_dev);

@@ -23,7 +23,8 @@
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kWarps = 8, kStages = 3;
+constexpr int kWarps = 8;
+constexpr int kStages = 4;             // records of a warp in shared memory: the two that it works on, the two that are on their way
 constexpr int kEntries = 1024;       // entries of the line's index in shared memory; each covers num_seqs / kEntries sequences
 constexpr float kFloor = -1e30f;     // reference of a column that has seen nothing: exp2(-inf - floor) is 0
 constexpr float kSlack = 8.f;
@@ -77,15 +78,89 @@ struct Part {  // what a run leaves of a unit that it shares with others
     int seq, kvh, block, start, tiles, first, last;  // start: the unit's place on the line; records first .. last - 1 of its `tiles`
 };
 
+// W words of this lane
+template <int W>
+__device__ __forceinline__ void lane_words(const uint8_t* at, int lane, uint32_t (&w)[W]) {
+    if constexpr (W == 4) {
+        const uint4 v = reinterpret_cast<const uint4*>(at)[lane];
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+        const uint2 v = reinterpret_cast<const uint2*>(at)[lane];
+        w[0] = v.x, w[1] = v.y;
+    }
+}
+// S^T[token, column] of a record: tokens g and g + 8, columns 2c and 2c + 1
+template <int HD>
+__device__ __forceinline__ void scores(const uint8_t* rec, int lane, const uint32_t (&qf)[HD / 16][2], float to_log2, float (&s)[4]) {
+    using Rec = q4::Record<HD>;
+    constexpr int W = HD / 32;
+    const int g = lane >> 2, c = lane & 3;
+    const uint32_t* sb = reinterpret_cast<const uint32_t*>(rec + Rec::kKsb) + (c * (HD / 4) / 64) * 16 + g;
+    const q4::Scales qa = q4::scales_twice(sb[0]), qb = q4::scales_twice(sb[8]);
+    uint32_t ka[W], kb[W];
+    lane_words<W>(rec, lane, ka);
+    lane_words<W>(rec + 4 * HD, lane, kb);
+    float s2[4] = {0.f, 0.f, 0.f, 0.f};
+    s[0] = s[1] = s[2] = s[3] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        uint32_t va[4], vb[4];
+        q4::values(ka[w], qa, va);
+        q4::values(kb[w], qb, vb);
+        const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
+        mma_bf16_16816(s, a0, qf[2 * w]);
+        mma_bf16_16816(s2, a1, qf[2 * w + 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) s[j] = (s[j] + s2[j]) * to_log2;
+}
+// O^T[dim, column] += V^T P^T of a record; rows g and g + 8 of tile mt are dims 2 mt and 2 mt + 1 of this lane's block.  `left`: tokens of
+// the record that belong to the context; what lies behind them may be anything, and 0 * NaN is NaN
+template <int HD>
+__device__ __forceinline__ void add_values(const uint8_t* rec, int lane, const float (&p)[4], int left, float (&o)[HD / 16][4]) {
+    using Rec = q4::Record<HD>;
+    constexpr int W = HD / 32;
+    const int g = lane >> 2, c = lane & 3;
+    const uint32_t* vsb = reinterpret_cast<const uint32_t*>(rec + Rec::kVsb) + (g * (HD / 8) / 64) * 16 + 2 * c;
+    uint2 sb0 = *reinterpret_cast<const uint2*>(vsb), sb1 = *reinterpret_cast<const uint2*>(vsb + 8);
+    if (left < 16) {
+        if (2 * c >= left) sb0.x = 0;
+        if (2 * c + 1 >= left) sb0.y = 0;
+        if (2 * c + 8 >= left) sb1.x = 0;
+        if (2 * c + 9 >= left) sb1.y = 0;
+    }
+    uint32_t pb[2], pl[2];
+    const uint32_t h01 = pack_bf2(p[0], p[1]), h23 = pack_bf2(p[2], p[3]);
+    const uint32_t r01 = pack_bf2(p[0] - bflo(h01), p[1] - bfhi(h01)), r23 = pack_bf2(p[2] - bflo(h23), p[3] - bfhi(h23));
+    pb[0] = movmatrix_trans(h01), pb[1] = movmatrix_trans(h23);
+    pl[0] = movmatrix_trans(r01), pl[1] = movmatrix_trans(r23);
+    const q4::Scales qa = q4::scales_pair(sb0.x, sb0.y), qb = q4::scales_pair(sb1.x, sb1.y);
+    uint32_t wa[W], wb[W];
+    lane_words<W>(rec + Rec::kV, lane, wa);
+    lane_words<W>(rec + Rec::kV + 4 * HD, lane, wb);
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        uint32_t va[4], vb[4];
+        q4::values(wa[w], qa, va);
+        q4::values(wb[w], qb, vb);
+        const uint32_t a0[4] = {va[0], va[1], vb[0], vb[1]}, a1[4] = {va[2], va[3], vb[2], vb[3]};
+        mma_bf16_16816(o[2 * w], a0, pb);
+        mma_bf16_16816(o[2 * w + 1], a1, pb);
+        mma_bf16_16816(o[2 * w], a0, pl);
+        mma_bf16_16816(o[2 * w + 1], a1, pl);
+    }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(const Q4AttnParams p) {
     using Rec = q4::Record<HD>;
-    constexpr int W = HD / 32;       // words of a lane per token (K) or token pair (V)
+    constexpr int W = HD / 32;  // words of a lane per token (K) or token pair (V)
     constexpr int KS = HD / 16, MT = HD / 16;
     constexpr int kChunks = Rec::kBytes / 16;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int s_off[kEntries + 1], s_warp[kWarps], s_last;
     __shared__ Part s_part[2 * kWarps];
+    __shared__ float s_weight[2 * kWarps][8], s_max[2 * kWarps][8], s_sum[2 * kWarps][8];
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -168,10 +243,11 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
             use.block = unit - use.kvh * use.len.blocks;
         }
         ask = use;
+        const int begin = pos;
         int asked = pos, window = -1, record = -1;  // lane i holds the record number of tile window + i of ask's unit, -1 for none
         uint32_t absent = 0;                         // bit s: the record of stage s lies on a page outside of the pool
-        auto issue = [&](int stage) {
-            if (asked < end) {
+        auto ask_until = [&](int upto) {
+            for (; asked < upto; asked++) {
                 if (window < 0 || ask.tile - window >= 32) {
                     window = ask.tile;
                     const int tile = window + lane, index = tile / p.page_tiles;
@@ -181,16 +257,15 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
                         if (page >= 0 && page < p.n_pages) record = (page * p.hkv + ask.kvh) * p.page_tiles + tile - index * p.page_tiles;
                     }
                 }
-                const int rec = __shfl_sync(kFull, record, ask.tile - window);
+                const int rec = __shfl_sync(kFull, record, ask.tile - window), stage = (asked - begin) % kStages;
                 absent = (absent & ~(1u << stage)) | (rec < 0 ? 1u << stage : 0u);
                 if (rec >= 0) {
-                    const uint8_t* src = p.pool + (size_t)rec * Rec::kBytes;
-                    const uint32_t dst = ring + stage * Rec::kBytes;
+                    const uint8_t* src = p.pool + (size_t)rec * Rec::kBytes + lane * 16;
+                    const uint32_t dst = ring + stage * Rec::kBytes + lane * 16;
 #pragma unroll
                     for (int i = 0; i < kChunks; i += 32)
-                        if (i + 32 <= kChunks || i + lane < kChunks) cp_async16(dst + (i + lane) * 16, src + (i + lane) * 16);
+                        if (i + 32 <= kChunks || i + lane < kChunks) cp_async16(dst + i * 16, src + i * 16);
                 }
-                asked++;
                 if (++ask.tile == ask.len.tiles) {
                     ask.next_unit(p);
                     window = -1;
@@ -198,9 +273,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
             }
             cp_async_commit();
         };
-#pragma unroll
-        for (int s = 0; s < kStages - 1; s++) issue(s);
-        int stage = 0;
+        ask_until(min(end, pos + kStages));
         bool first_of_run = true;
         while (pos < end) {
             const int t0 = use.tile, t1 = min(use.len.tiles, t0 + end - pos);
@@ -231,54 +304,34 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
 
-            for (int t = t0; t < t1; t++) {
-                cp_async_wait<kStages - 2>();
-                __syncwarp();  // everyone's copies have landed, and everyone is done with the stage that is asked into now
-                issue(stage == 0 ? kStages - 1 : stage - 1);
-                const uint8_t* rec = smem + (warp * kStages + stage) * Rec::kBytes;
-                const bool there = !(absent >> stage & 1);
-                stage = stage + 1 == kStages ? 0 : stage + 1;
-                if (!there) continue;
+            for (int t = t0; t < t1; t += 2) {
+                // two records at a time, so that their chains of instructions overlap; at an odd end the second is left out
+                const int at = pos + t - t0;
+                cp_async_wait<0>();
+                __syncwarp();  // everyone's copies have landed, and everyone is done with the records that are overwritten now
+                ask_until(min(end, at + kStages));
+                const int st0 = (at - begin) % kStages, st1 = (st0 + 1) % kStages;
+                const bool one = !(absent >> st0 & 1), two = t + 1 < t1 && !(absent >> st1 & 1);
+                const uint8_t *rec0 = smem + (warp * kStages + st0) * Rec::kBytes, *rec1 = smem + (warp * kStages + st1) * Rec::kBytes;
+                float s0[4], s1[4];
+                if (one)
+                    scores<HD>(rec0, lane, qf, to_log2, s0);
+                else
+                    s0[0] = s0[1] = s0[2] = s0[3] = -INFINITY;
+                if (two)
+                    scores<HD>(rec1, lane, qf, to_log2, s1);
+                else
+                    s1[0] = s1[1] = s1[2] = s1[3] = -INFINITY;
                 const int tok0 = t * 16;
-                // S^T[token, column]
-                float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
-                {
-                    const uint32_t* sb = reinterpret_cast<const uint32_t*>(rec + Rec::kKsb) + (c * (HD / 4) / 64) * 16 + g;
-                    const q4::Scales qa = q4::scales_twice(sb[0]), qb = q4::scales_twice(sb[8]);
-                    uint32_t ka[W], kb[W];
-                    if constexpr (W == 4) {
-                        const uint4 a = *reinterpret_cast<const uint4*>(rec + lane * 16), b = *reinterpret_cast<const uint4*>(rec + 512 + lane * 16);
-                        ka[0] = a.x, ka[1] = a.y, ka[2] = a.z, ka[3] = a.w, kb[0] = b.x, kb[1] = b.y, kb[2] = b.z, kb[3] = b.w;
-                    } else {
-                        const uint2 a = *reinterpret_cast<const uint2*>(rec + lane * 8), b = *reinterpret_cast<const uint2*>(rec + 256 + lane * 8);
-                        ka[0] = a.x, ka[1] = a.y, kb[0] = b.x, kb[1] = b.y;
-                    }
+                if (tok0 + 32 > sure) {
 #pragma unroll
-                    for (int w = 0; w < W; w++) {
-                        uint32_t va[4], vb[4];
-                        q4::values(ka[w], qa, va);
-                        q4::values(kb[w], qb, vb);
-                        const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
-                        mma_bf16_16816(s, a0, qf[2 * w]);
-                        mma_bf16_16816(s2, a1, qf[2 * w + 1]);
+                    for (int j = 0; j < 4; j++) {
+                        const int lim = j & 1 ? lim1 : lim0, tok = tok0 + g + (j >> 1) * 8;
+                        if (tok >= lim) s0[j] = -INFINITY;
+                        if (tok + 16 >= lim) s1[j] = -INFINITY;
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 4; j++) s[j] = (s[j] + s2[j]) * to_log2;
-                const uint32_t* vsb = reinterpret_cast<const uint32_t*>(rec + Rec::kVsb) + (g * (HD / 8) / 64) * 16 + 2 * c;
-                uint2 sb0 = *reinterpret_cast<const uint2*>(vsb), sb1 = *reinterpret_cast<const uint2*>(vsb + 8);
-                if (tok0 + 16 > sure) {
-                    if (tok0 + g >= lim0) s[0] = -INFINITY;
-                    if (tok0 + g >= lim1) s[1] = -INFINITY;
-                    if (tok0 + g + 8 >= lim0) s[2] = -INFINITY;
-                    if (tok0 + g + 8 >= lim1) s[3] = -INFINITY;
-                    // what lies behind the context may be anything, and 0 * NaN is NaN
-                    if (tok0 + 2 * c >= use.len.ctx) sb0.x = 0;
-                    if (tok0 + 2 * c + 1 >= use.len.ctx) sb0.y = 0;
-                    if (tok0 + 2 * c + 8 >= use.len.ctx) sb1.x = 0;
-                    if (tok0 + 2 * c + 9 >= use.len.ctx) sb1.y = 0;
-                }
-                float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
+                float mx0 = fmaxf(fmaxf(s0[0], s0[2]), fmaxf(s1[0], s1[2])), mx1 = fmaxf(fmaxf(s0[1], s0[3]), fmaxf(s1[1], s1[3]));
                 if (__any_sync(kFull, mx0 > m0 + kSlack || mx1 > m1 + kSlack)) {
 #pragma unroll
                     for (int sh = 4; sh <= 16; sh <<= 1) {
@@ -292,40 +345,12 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) o[mt][0] *= a0, o[mt][1] *= a1, o[mt][2] *= a0, o[mt][3] *= a1;
                 }
-                const float p0 = fast_exp2(s[0] - m0), p1 = fast_exp2(s[1] - m1), p2 = fast_exp2(s[2] - m0), p3 = fast_exp2(s[3] - m1);
-                l0 += p0 + p2;
-                l1 += p1 + p3;
-                uint32_t pb[2], pl[2];
-                {
-                    const uint32_t h01 = pack_bf2(p0, p1), h23 = pack_bf2(p2, p3);
-                    const uint32_t r01 = pack_bf2(p0 - bflo(h01), p1 - bfhi(h01)), r23 = pack_bf2(p2 - bflo(h23), p3 - bfhi(h23));
-                    pb[0] = movmatrix_trans(h01), pb[1] = movmatrix_trans(h23);
-                    pl[0] = movmatrix_trans(r01), pl[1] = movmatrix_trans(r23);
-                }
-                // O^T[dim, column]: rows g and g + 8 of tile mt are dims 2 mt and 2 mt + 1 of this lane's block
-                {
-                    const q4::Scales qa = q4::scales_pair(sb0.x, sb0.y), qb = q4::scales_pair(sb1.x, sb1.y);
-                    const uint8_t* v = rec + Rec::kV;
-                    uint32_t wa[W], wb[W];
-                    if constexpr (W == 4) {
-                        const uint4 a = *reinterpret_cast<const uint4*>(v + lane * 16), b = *reinterpret_cast<const uint4*>(v + 512 + lane * 16);
-                        wa[0] = a.x, wa[1] = a.y, wa[2] = a.z, wa[3] = a.w, wb[0] = b.x, wb[1] = b.y, wb[2] = b.z, wb[3] = b.w;
-                    } else {
-                        const uint2 a = *reinterpret_cast<const uint2*>(v + lane * 8), b = *reinterpret_cast<const uint2*>(v + 256 + lane * 8);
-                        wa[0] = a.x, wa[1] = a.y, wb[0] = b.x, wb[1] = b.y;
-                    }
 #pragma unroll
-                    for (int w = 0; w < W; w++) {
-                        uint32_t va[4], vb[4];
-                        q4::values(wa[w], qa, va);
-                        q4::values(wb[w], qb, vb);
-                        const uint32_t a0[4] = {va[0], va[1], vb[0], vb[1]}, a1[4] = {va[2], va[3], vb[2], vb[3]};
-                        mma_bf16_16816(o[2 * w], a0, pb);
-                        mma_bf16_16816(o[2 * w + 1], a1, pb);
-                        mma_bf16_16816(o[2 * w], a0, pl);
-                        mma_bf16_16816(o[2 * w + 1], a1, pl);
-                    }
-                }
+                for (int j = 0; j < 4; j++) s0[j] = fast_exp2(s0[j] - (j & 1 ? m1 : m0)), s1[j] = fast_exp2(s1[j] - (j & 1 ? m1 : m0));
+                l0 += (s0[0] + s0[2]) + (s1[0] + s1[2]);
+                l1 += (s0[1] + s0[3]) + (s1[1] + s1[3]);
+                if (one) add_values<HD>(rec0, lane, s0, use.len.ctx - tok0, o);
+                if (two) add_values<HD>(rec1, lane, s1, use.len.ctx - tok0 - 16, o);
             }
             pos += t1 - t0;
 #pragma unroll
@@ -369,53 +394,70 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     }
     __syncthreads();
 
-    // ---- the block's parts, unit by unit in the order of the line
+    // ---- the block's parts, unit by unit in the order of the line.  A thread has four dims of a column.
+    static_assert(8 * HD <= kWarps * 32 * 4, "a thread has one piece of a unit's output");
     auto part_at = [&](int i) { return (i & 1) ? reinterpret_cast<const float*>(smem + (i >> 1) * kStages * Rec::kBytes) : parts + (i >> 1) * part_floats<HD>(); };
-    constexpr int kPer = 8 * HD / (kWarps * 32);  // outputs of a thread
-    int crossing[2] = {-1, -1};                   // parts of the units that other blocks share: this block's first and its last one
-    for (int i = 0; i < 2 * kWarps;) {
-        if (s_part[i].tiles == 0) {
-            i++;
-            continue;
+    const int my_start = lane < 2 * kWarps ? s_part[lane].start : 0;
+    const unsigned there = __ballot_sync(kFull, lane < 2 * kWarps && s_part[lane < 2 * kWarps ? lane : 0].tiles > 0);
+    unsigned heads;  // the first part of every unit
+    {
+        const unsigned before = there & ((1u << lane) - 1);
+        const int prev_start = __shfl_sync(kFull, my_start, before ? 31 - __clz(before) : 0);
+        heads = __ballot_sync(kFull, (there >> lane & 1) && (!before || prev_start != my_start));
+    }
+    auto unit_parts = [&](int head) {  // the parts of the unit that begins with part `head`
+        const unsigned later = heads & ~((2u << head) - 1);
+        return there & ~((1u << head) - 1) & (later ? (later & -later) - 1 : ~0u);
+    };
+    if (threadIdx.x < 16 * kWarps && (heads >> (threadIdx.x >> 3) & 1)) {  // maximum and sum of a unit's column, and its parts' weights
+        const int head = threadIdx.x >> 3, col = threadIdx.x & 7;
+        float m = kFloor, l = 0.f;
+        for (unsigned u = unit_parts(head); u; u &= u - 1) m = fmaxf(m, part_at(__ffs(u) - 1)[8 * HD + col]);
+        for (unsigned u = unit_parts(head); u; u &= u - 1) {
+            const int i = __ffs(u) - 1;
+            const float f = fast_exp2(part_at(i)[8 * HD + col] - m);
+            l += part_at(i)[8 * HD + 8 + col] * f;
+            s_weight[i][col] = f;
         }
-        const Part u = s_part[i];
-        int n = i + 1, last = u.last;
-        for (; n < 2 * kWarps && (s_part[n].tiles == 0 || s_part[n].start == u.start); n++)
-            if (s_part[n].tiles) last = s_part[n].last;
-        const bool whole = u.first == 0 && last == u.tiles;
-        const int cols = min(8, (p.q_lens ? p.q_lens[u.seq] : 1) * group - u.block * 8);
-        const int side = u.start <= block_start ? 0 : 1;
-        float* const dst = p.parts + (size_t)(blockIdx.x * 2 + side) * part_floats<HD>();
-#pragma unroll
-        for (int k = 0; k < kPer; k++) {
-            const int e = threadIdx.x + k * kWarps * 32, col = e / HD;
-            if (col >= cols) break;
-            float m = kFloor, l = 0.f, sum = 0.f;
-            for (int j = i; j < n; j++)
-                if (s_part[j].tiles) m = fmaxf(m, part_at(j)[8 * HD + col]);
-            for (int j = i; j < n; j++)
-                if (s_part[j].tiles) {
-                    const float* part = part_at(j);
-                    const float f = fast_exp2(part[8 * HD + col] - m);
-                    l += part[8 * HD + 8 + col] * f;
-                    sum += part[e] * f;
-                }
+        s_max[head][col] = m, s_sum[head][col] = l;
+    }
+    __syncthreads();
+    const int e = threadIdx.x * 4, col = e / HD;
+    auto store = [&](const Part& u, const float4& v, float l) {
+        const float f = l == 0.f ? 0.f : q4::kUnscale / l;
+        *reinterpret_cast<uint2*>(out_row(u.seq, u.kvh, u.block * 8 + col) + e % HD) = make_uint2(pack_bf2(v.x * f, v.y * f), pack_bf2(v.z * f, v.w * f));
+    };
+    auto add = [](float4& sum, const float4& v, float f) { sum.x += v.x * f, sum.y += v.y * f, sum.z += v.z * f, sum.w += v.w * f; };
+    int crossing[2] = {-1, -1};  // parts of the units that other blocks share: this block's first and its last one
+    for (unsigned h = heads; h; h &= h - 1) {
+        const int head = __ffs(h) - 1;
+        const unsigned mine = unit_parts(head);
+        const Part u = s_part[head];
+        const bool whole = u.first == 0 && s_part[31 - __clz(mine)].last == u.tiles;
+        const int cols = min(8, (p.q_lens ? p.q_lens[u.seq] : 1) * group - u.block * 8), side = u.start <= block_start ? 0 : 1;
+        if (!whole) crossing[side] = head;
+        if (col < cols) {
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (unsigned r = mine; r; r &= r - 1) {
+                const int i = __ffs(r) - 1;
+                add(sum, *reinterpret_cast<const float4*>(part_at(i) + e), s_weight[i][col]);
+            }
             if (whole) {
-                out_row(u.seq, u.kvh, u.block * 8 + col)[e % HD] = f2bf(l == 0.f ? 0.f : sum * (q4::kUnscale / l));
+                store(u, sum, s_sum[head][col]);
             } else {
-                dst[e] = sum;
-                if (e % HD == 0) dst[8 * HD + col] = m, dst[8 * HD + 8 + col] = l;
+                float* dst = p.parts + (size_t)(blockIdx.x * 2 + side) * part_floats<HD>();
+                *reinterpret_cast<float4*>(dst + e) = sum;
+                if (e % HD == 0) dst[8 * HD + col] = s_max[head][col], dst[8 * HD + 8 + col] = s_sum[head][col];
             }
         }
-        if (!whole) crossing[side] = i;
-        i = n;
     }
     // ---- units of several blocks: whoever arrives last adds up their parts
     const int block_run = kWarps * run;
-#pragma unroll
+    float* const weight = reinterpret_cast<float*>(smem);  // [blocks][8]
     for (int side = 0; side < 2; side++) {
-        if (crossing[side] < 0) continue;
-        const Part u = s_part[crossing[side]];
+        const int head = side ? crossing[1] : crossing[0];
+        if (head < 0) continue;
+        const Part u = s_part[head];
         const int from = u.start / block_run, to = (u.start + u.tiles - 1) / block_run;
         __threadfence();  // this block's part is visible before its arrival is counted
         __syncthreads();
@@ -426,22 +468,29 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         __syncthreads();
         if (!s_last) continue;
         __threadfence();
-        const int cols = min(8, (p.q_lens ? p.q_lens[u.seq] : 1) * group - u.block * 8);
         auto part = [&](int b) { return p.parts + (size_t)(b * 2 + (u.start <= b * block_run ? 0 : 1)) * part_floats<HD>(); };
+        {  // a warp per column: weights of the blocks' parts, and their sum
+            float m = kFloor, l = 0.f;
+            for (int b = from + lane; b <= to; b += 32) m = fmaxf(m, __ldcg(part(b) + 8 * HD + warp));
 #pragma unroll
-        for (int k = 0; k < kPer; k++) {
-            const int e = threadIdx.x + k * kWarps * 32, col = e / HD;
-            if (col >= cols) break;
-            float m = kFloor, l = 0.f, sum = 0.f;
-            for (int b = from; b <= to; b++) m = fmaxf(m, __ldcg(part(b) + 8 * HD + col));
-#pragma unroll 4
-            for (int b = from; b <= to; b++) {
-                const float f = fast_exp2(__ldcg(part(b) + 8 * HD + col) - m);
-                l += __ldcg(part(b) + 8 * HD + 8 + col) * f;
-                sum += __ldcg(part(b) + e) * f;
+            for (int sh = 1; sh <= 16; sh <<= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, sh));
+            for (int b = from + lane; b <= to; b += 32) {
+                const float f = fast_exp2(__ldcg(part(b) + 8 * HD + warp) - m);
+                l += __ldcg(part(b) + 8 * HD + 8 + warp) * f;
+                weight[(b - from) * 8 + warp] = f;
             }
-            out_row(u.seq, u.kvh, u.block * 8 + col)[e % HD] = f2bf(l == 0.f ? 0.f : sum * (q4::kUnscale / l));
+#pragma unroll
+            for (int sh = 1; sh <= 16; sh <<= 1) l += __shfl_xor_sync(kFull, l, sh);
+            if (lane == 0) s_sum[0][warp] = l;
         }
+        __syncthreads();
+        if (col < min(8, (p.q_lens ? p.q_lens[u.seq] : 1) * group - u.block * 8)) {
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int b = from; b <= to; b++) add(sum, __ldcg(reinterpret_cast<const float4*>(part(b) + e)), weight[(b - from) * 8 + col]);
+            store(u, sum, s_sum[0][col]);
+        }
+        __syncthreads();  // the weights and the sums are written again
     }
 }
 

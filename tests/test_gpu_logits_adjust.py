@@ -160,3 +160,12 @@ def test_same_as_argmax_without_rules(env):
     K.logits_adjust(ctx, dev, 7, 5001, K.logit_rules(), argmax=b)
     ctx.sync()
     assert np.array_equal(a.download(), b.download())
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_more_named_tokens_than_are_kept_at_a_time(env, f32, in_place):
+    rng, c = case(31, 2, 90000, 60000, 4000)
+    c["history"] = [rng.permutation(90000)[:70000], rng.integers(0, 9000, 50000)]  # ... in every slice, and in one
+    c["n_prompt"] = [35000, 20000]
+    check(env, f32=f32, in_place=in_place, allowed=rng.random((2, 90000)) < 0.5, **c)
