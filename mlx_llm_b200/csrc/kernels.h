@@ -233,7 +233,9 @@ struct Q4AttnParams {
     int num_seqs, hq, hkv, page_tiles;
     float scale_log2;             // softmax scale * log2(e)
     uint16_t* out;                // [rows, hq, hd] bf16
-    float* parts;                 // (filled in by the launch)
+    // filled in by the launch
+    int group, max_ctx, entries, per_entry;
+    float* parts;
     int* counters;
 };
 int32_t b2_kv_q4_attn_launch(b2_ctx* ctx, const Q4AttnParams& p, int head_dim);

@@ -25,10 +25,11 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 8;
 constexpr int kStages = 4;             // records of a warp in shared memory: the two that it works on, the two that are on their way
-constexpr int kEntries = 1024;       // entries of the line's index in shared memory; each covers num_seqs / kEntries sequences
+constexpr int kEntries = 512;        // entries of the line's index in shared memory; each covers num_seqs / kEntries sequences
 constexpr float kFloor = -1e30f;     // reference of a column that has seen nothing: exp2(-inf - floor) is 0
 constexpr float kSlack = 8.f;
 constexpr int kMinRun = 4;           // records of a run at least
+constexpr int kUnitRun = 8;          // ... and at most, where a block has a unit of its own
 constexpr int kBlocksPerSm = 2;
 
 template <int HD>
@@ -45,14 +46,14 @@ constexpr int smem_bytes() {
 }
 
 struct Lengths {  // of one sequence
-    int ctx, queries, tiles, blocks;
+    int ctx, tiles, columns, blocks;
 };
 __device__ __forceinline__ Lengths lengths_of(const Q4AttnParams& p, int seq) {
     Lengths l;
-    l.ctx = min(max(p.ctx_lens[seq], 0), p.max_blocks * p.page_tiles * 16);
-    l.queries = p.q_lens ? p.q_lens[seq] : 1;
+    l.ctx = min(max(p.ctx_lens[seq], 0), p.max_ctx);
+    l.columns = p.q_lens ? p.q_lens[seq] * p.group : p.group;
     l.tiles = (l.ctx + 15) >> 4;
-    l.blocks = (l.queries * (p.hq / p.hkv) + 7) >> 3;
+    l.blocks = l.tiles ? (l.columns + 7) >> 3 : 0;
     return l;
 }
 // A place on the line.
@@ -63,8 +64,12 @@ struct Cursor {
         kvh = block = tile = 0;
         for (seq = s; seq < p.num_seqs; seq++) {
             len = lengths_of(p, seq);
-            if (len.tiles * len.blocks > 0) return;
+            if (len.blocks > 0) return;
         }
+    }
+    __device__ __forceinline__ void at_unit(int unit) {
+        kvh = unit / len.blocks;
+        block = unit - kvh * len.blocks;
     }
     __device__ __forceinline__ void next_unit(const Q4AttnParams& p) {
         tile = 0;
@@ -75,7 +80,7 @@ struct Cursor {
     }
 };
 struct Part {  // what a run leaves of a unit that it shares with others
-    int seq, kvh, block, start, tiles, first, last;  // start: the unit's place on the line; records first .. last - 1 of its `tiles`
+    int seq, kvh, block, start, tiles, first, last, cols;  // start: the unit's place on the line; records first .. last - 1 of its `tiles`
 };
 
 // W words of this lane
@@ -157,91 +162,110 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     constexpr int W = HD / 32;  // words of a lane per token (K) or token pair (V)
     constexpr int KS = HD / 16, MT = HD / 16;
     constexpr int kChunks = Rec::kBytes / 16;
+    constexpr int kThreads = kWarps * 32, kParts = 2 * kWarps;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int s_off[kEntries + 1], s_warp[kWarps], s_last;
-    __shared__ Part s_part[2 * kWarps];
-    __shared__ float s_weight[2 * kWarps][8], s_max[2 * kWarps][8], s_sum[2 * kWarps][8];
+    __shared__ int s_off[kEntries + 1], s_unit[kEntries + 1];  // first record, first unit of every entry
+    __shared__ int4 s_scan[kWarps];
+    __shared__ Part s_part[kParts];
+    __shared__ float s_m[kParts][8], s_l[kParts][8], s_weight[kParts][8], s_sum[kParts][8], s_max[kParts][8];
+    __shared__ int s_last;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int group = p.hq / p.hkv;
-    const int per = (p.num_seqs + kEntries - 1) / kEntries;  // sequences per entry
-    const int entries = (p.num_seqs + per - 1) / per;
+    const int group = p.group;
 
-    // the line: first record of every entry
-    {
-        int carry = 0;
-        for (int base = 0; base < entries; base += kWarps * 32) {
-            const int e = base + threadIdx.x;
-            int n = 0;
-            for (int s = e * per; s < min(p.num_seqs, (e + 1) * per); s++) {
-                const Lengths l = lengths_of(p, s);
-                n += l.tiles * l.blocks * p.hkv;
-            }
-            int incl = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(kFull, incl, o);
-                if (lane >= o) incl += v;
-            }
-            if (lane == 31) s_warp[warp] = incl;
-            __syncthreads();
-            int before = carry;
-            for (int w = 0; w < warp; w++) before += s_warp[w];
-            if (e < entries) s_off[e] = before + incl - n;
-            for (int w = 0; w < kWarps; w++) carry += s_warp[w];
-            __syncthreads();
+    // the line: first record and unit of every entry, the longest unit, and whether there are empty contexts
+    int total = 0, units = 0, longest = 0, empty = 0;
+    for (int base = 0; base < p.entries; base += kThreads) {
+        const int e = base + threadIdx.x;
+        int n = 0, u = 0, most = 0, none = 0;
+        for (int s = e * p.per_entry; s < min(p.num_seqs, (e + 1) * p.per_entry); s++) {
+            const Lengths l = lengths_of(p, s);
+            u += l.blocks * p.hkv;
+            n += l.tiles * l.blocks * p.hkv;
+            most = max(most, l.tiles);
+            none |= l.tiles == 0;
         }
-        if (threadIdx.x == 0) s_off[entries] = carry;
-        if (threadIdx.x < 2 * kWarps) s_part[threadIdx.x].tiles = 0;
+        int ni = n, ui = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int a = __shfl_up_sync(kFull, ni, o), b = __shfl_up_sync(kFull, ui, o);
+            if (lane >= o) ni += a, ui += b;
+        }
+        most = __reduce_max_sync(kFull, most);
+        none = __any_sync(kFull, none);
+        if (lane == 31) s_scan[warp] = make_int4(ni, ui, most, none);
+        if (base == 0 && threadIdx.x < kParts) s_part[threadIdx.x].tiles = 0;
+        __syncthreads();
+        int nb = total, ub = units;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const int4 v = s_scan[w];
+            if (w < warp) nb += v.x, ub += v.y;
+            total += v.x, units += v.y, longest = max(longest, v.z), empty |= v.w;
+        }
+        if (e < p.entries) s_off[e] = nb + ni - n, s_unit[e] = ub + ui - u;
         __syncthreads();
     }
-    // an empty context attends to nothing: rows of zeros
-    for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
-        const Lengths l = lengths_of(p, s);
-        if (l.tiles > 0) continue;
-        const size_t row = p.q_rows ? p.q_rows[s] : s;
-        for (int e = threadIdx.x; e < l.queries * p.hq * HD; e += kWarps * 32) p.out[row * p.hq * HD + e] = 0;
-    }
-    const int total = s_off[entries];
+    if (empty)  // an empty context attends to nothing: rows of zeros
+        for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
+            if (lengths_of(p, s).tiles > 0) continue;
+            const size_t row = p.q_rows ? p.q_rows[s] : s;
+            const int n = (p.q_lens ? p.q_lens[s] : 1) * p.hq * HD;
+            for (int e = threadIdx.x; e < n; e += kThreads) p.out[row * p.hq * HD + e] = 0;
+        }
+    // few short units: each is a block's, and no block shares one with another.  Else equal runs.
+    const bool by_unit = units <= (int)gridDim.x && longest <= kWarps * kUnitRun;
     const int run = max(kMinRun, (total + (int)gridDim.x * kWarps - 1) / ((int)gridDim.x * kWarps));
     const int block_start = blockIdx.x * kWarps * run;
-    if (block_start >= total) return;
-    int pos = min(block_start + warp * run, total);
-    const int end = min(pos + run, total);
-
+    if (by_unit ? blockIdx.x >= units : block_start >= total) return;
     const uint32_t ring = smem_u32(smem) + warp * kStages * Rec::kBytes;
-    float* const parts = reinterpret_cast<float*>(smem + ring_bytes<HD>());
+    float4* const parts = reinterpret_cast<float4*>(smem + ring_bytes<HD>());
     const float to_log2 = p.scale_log2 * q4::kUnscale;
 
-    // writes a unit's finished columns: this lane's 16 (8) dims of columns 2c and 2c + 1, or nothing
+    // row of the output that a unit's column belongs to
     auto out_row = [&](int seq, int kvh, int col) {
-        const int row = (p.q_rows ? p.q_rows[seq] : seq) + col / group;
-        return p.out + ((size_t)row * p.hq + (size_t)kvh * group + col % group) * HD;
+        const int query = col / group;
+        const int row = (p.q_rows ? p.q_rows[seq] : seq) + query;
+        return p.out + ((size_t)row * p.hq + (size_t)kvh * group + (col - query * group)) * HD;
     };
 
-    if (pos < end) {
-        Cursor use, ask;
-        {
-            int lo = 0, hi = entries - 1;  // the last entry that begins at or before pos; of equal ones all but the last are empty
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (s_off[mid] <= pos)
-                    lo = mid;
-                else
-                    hi = mid - 1;
-            }
-            int left = pos - s_off[lo];
-            use.at_seq(p, lo * per);
-            while (left >= use.len.tiles * use.len.blocks * p.hkv) {
-                left -= use.len.tiles * use.len.blocks * p.hkv;
-                use.at_seq(p, use.seq + 1);
-            }
+    Cursor use, ask;
+    int pos, end;
+    {
+        const int want = by_unit ? blockIdx.x : min(block_start + warp * run, total - 1);
+        const int* first = by_unit ? s_unit : s_off;
+        int lo = 0, hi = p.entries - 1;  // the last entry that begins at or before it; of equal ones all but the last are empty
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first[mid] <= want)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        int left = want - first[lo];
+        use.at_seq(p, lo * p.per_entry);
+        while (true) {  // (sequences of the entry)
+            const int all = (by_unit ? 1 : use.len.tiles) * use.len.blocks * p.hkv;
+            if (left < all) break;
+            left -= all;
+            use.at_seq(p, use.seq + 1);
+        }
+        if (by_unit) {
+            use.at_unit(left);
+            const int each = (use.len.tiles + kWarps - 1) / kWarps;
+            use.tile = min(warp * each, use.len.tiles);
+            pos = use.tile;  // (the unit's own line)
+            end = min(pos + each, use.len.tiles);
+        } else {
             const int unit = left / use.len.tiles;
             use.tile = left - unit * use.len.tiles;
-            use.kvh = unit / use.len.blocks;
-            use.block = unit - use.kvh * use.len.blocks;
+            use.at_unit(unit);
+            pos = min(block_start + warp * run, total);
+            end = min(pos + run, total);
         }
+    }
+    if (pos < end) {
         ask = use;
         const int begin = pos;
         int asked = pos, window = -1, record = -1;  // lane i holds the record number of tile window + i of ask's unit, -1 for none
@@ -280,11 +304,11 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
             const int start = pos - t0;
             // Q as the B operand, in the order of the nibbles; columns past the last are zeros
             uint32_t qf[KS][2];
-            const int cols = min(8, use.len.queries * group - use.block * 8);
+            const int cols = min(8, use.len.columns - use.block * 8);
             {
-                const int col = use.block * 8 + min(g, cols - 1);
-                const size_t row = (p.q_rows ? p.q_rows[use.seq] : use.seq) + col / group;
-                const uint16_t* q = p.q + (row * p.hq + (size_t)use.kvh * group + col % group) * HD + c * (HD / 4);
+                const int col = use.block * 8 + min(g, cols - 1), query = col / group;
+                const size_t row = (p.q_rows ? p.q_rows[use.seq] : use.seq) + query;
+                const uint16_t* q = p.q + (row * p.hq + (size_t)use.kvh * group + (col - query * group)) * HD + c * (HD / 4);
 #pragma unroll
                 for (int w = 0; w < W; w++) {
                     uint4 u = *reinterpret_cast<const uint4*>(q + 8 * w);
@@ -296,9 +320,12 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
                 }
             }
             // keys that columns 2c and 2c + 1 see; all columns see those before `sure`
-            const int hidden = use.len.ctx - use.len.queries + 1;
-            const int lim0 = hidden + (use.block * 8 + 2 * c) / group, lim1 = hidden + (use.block * 8 + 2 * c + 1) / group;
-            const int sure = hidden + use.block * 8 / group;
+            int lim0 = use.len.ctx, lim1 = lim0, sure = lim0;
+            if (p.q_lens) {
+                const int hidden = use.len.ctx - p.q_lens[use.seq] + 1;
+                lim0 = hidden + (use.block * 8 + 2 * c) / group, lim1 = hidden + (use.block * 8 + 2 * c + 1) / group;
+                sure = hidden + use.block * 8 / group;
+            }
             float m0 = kFloor, m1 = kFloor, l0 = 0.f, l1 = 0.f;
             float o[MT][4];
 #pragma unroll
@@ -372,20 +399,14 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
                     for (int i = 0; i < MT / 4; i++) dst[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                 }
             } else {
-                // the first part of a run has a place of its own; the last one lies where the run's records were
-                if (!first_of_run) __syncwarp();
-                float* dst = first_of_run ? parts + warp * part_floats<HD>() : reinterpret_cast<float*>(smem + warp * kStages * Rec::kBytes);
+                // as it lies in the lanes.  The first part of a run has a place of its own; the last one lies where the run's records were
+                __syncwarp();
+                const int i = 2 * warp + !first_of_run;
+                float4* dst = first_of_run ? parts + warp * MT * 32 : reinterpret_cast<float4*>(smem + warp * kStages * Rec::kBytes);
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    const int d = g * (HD / 8) + 2 * mt;
-                    *reinterpret_cast<float2*>(dst + (2 * c) * HD + d) = make_float2(o[mt][0], o[mt][2]);
-                    *reinterpret_cast<float2*>(dst + (2 * c + 1) * HD + d) = make_float2(o[mt][1], o[mt][3]);
-                }
-                if (g == 0) {
-                    dst[8 * HD + 2 * c] = m0, dst[8 * HD + 2 * c + 1] = m1;
-                    dst[8 * HD + 8 + 2 * c] = l0, dst[8 * HD + 8 + 2 * c + 1] = l1;
-                }
-                if (lane == 0) s_part[2 * warp + !first_of_run] = Part{use.seq, use.kvh, use.block, start, use.len.tiles, t0, t1};
+                for (int mt = 0; mt < MT; mt++) dst[mt * 32 + lane] = make_float4(o[mt][0], o[mt][1], o[mt][2], o[mt][3]);
+                if (g == 0) s_m[i][2 * c] = m0, s_m[i][2 * c + 1] = m1, s_l[i][2 * c] = l0, s_l[i][2 * c + 1] = l1;
+                if (lane == 0) s_part[i] = Part{use.seq, use.kvh, use.block, start, use.len.tiles, t0, t1, cols};
             }
             first_of_run = false;
             use.tile = t1;
@@ -394,101 +415,117 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     }
     __syncthreads();
 
-    // ---- the block's parts, unit by unit in the order of the line.  A thread has four dims of a column.
-    static_assert(8 * HD <= kWarps * 32 * 4, "a thread has one piece of a unit's output");
-    auto part_at = [&](int i) { return (i & 1) ? reinterpret_cast<const float*>(smem + (i >> 1) * kStages * Rec::kBytes) : parts + (i >> 1) * part_floats<HD>(); };
-    const int my_start = lane < 2 * kWarps ? s_part[lane].start : 0;
-    const unsigned there = __ballot_sync(kFull, lane < 2 * kWarps && s_part[lane < 2 * kWarps ? lane : 0].tiles > 0);
-    unsigned heads;  // the first part of every unit
+    // ---- the block's parts, unit by unit in the order of the line.  A thread has what a lane had of one tile: 2 dims of 2 columns.
+    const Part mine = s_part[lane % kParts];
+    const unsigned there = __ballot_sync(kFull, lane < kParts && mine.tiles > 0);
+    unsigned heads, unit;  // the first part of every unit; the parts of this lane's
     {
         const unsigned before = there & ((1u << lane) - 1);
-        const int prev_start = __shfl_sync(kFull, my_start, before ? 31 - __clz(before) : 0);
-        heads = __ballot_sync(kFull, (there >> lane & 1) && (!before || prev_start != my_start));
+        const int prev_start = __shfl_sync(kFull, mine.start, before ? 31 - __clz(before) : 0);
+        heads = __ballot_sync(kFull, (there >> lane & 1) && (!before || prev_start != mine.start));
+        const unsigned up_to = (2u << lane) - 1, head = heads & up_to, later = heads & ~up_to;
+        unit = there & (later ? (later & -later) - 1 : ~0u) & ~(head ? (1u << (31 - __clz(head))) - 1 : ~0u);
     }
-    auto unit_parts = [&](int head) {  // the parts of the unit that begins with part `head`
-        const unsigned later = heads & ~((2u << head) - 1);
-        return there & ~((1u << head) - 1) & (later ? (later & -later) - 1 : ~0u);
-    };
-    if (threadIdx.x < 16 * kWarps && (heads >> (threadIdx.x >> 3) & 1)) {  // maximum and sum of a unit's column, and its parts' weights
-        const int head = threadIdx.x >> 3, col = threadIdx.x & 7;
+    for (int i = threadIdx.x >> 3; i < kParts; i += kThreads / 8) {  // weight of a part's column, and its unit's maximum and sum
+        const unsigned u = __shfl_sync(kFull, unit, i);
+        const int col = threadIdx.x & 7;
         float m = kFloor, l = 0.f;
-        for (unsigned u = unit_parts(head); u; u &= u - 1) m = fmaxf(m, part_at(__ffs(u) - 1)[8 * HD + col]);
-        for (unsigned u = unit_parts(head); u; u &= u - 1) {
-            const int i = __ffs(u) - 1;
-            const float f = fast_exp2(part_at(i)[8 * HD + col] - m);
-            l += part_at(i)[8 * HD + 8 + col] * f;
-            s_weight[i][col] = f;
-        }
-        s_max[head][col] = m, s_sum[head][col] = l;
+#pragma unroll
+        for (int j = 0; j < kParts; j++) m = fmaxf(m, u >> j & 1 ? s_m[j][col] : kFloor);
+#pragma unroll
+        for (int j = 0; j < kParts; j++) l += u >> j & 1 ? s_l[j][col] * fast_exp2(s_m[j][col] - m) : 0.f;
+        if (there >> i & 1) s_weight[i][col] = fast_exp2(s_m[i][col] - m), s_max[i][col] = m, s_sum[i][col] = l;
     }
     __syncthreads();
-    const int e = threadIdx.x * 4, col = e / HD;
-    auto store = [&](const Part& u, const float4& v, float l) {
-        const float f = l == 0.f ? 0.f : q4::kUnscale / l;
-        *reinterpret_cast<uint2*>(out_row(u.seq, u.kvh, u.block * 8 + col) + e % HD) = make_uint2(pack_bf2(v.x * f, v.y * f), pack_bf2(v.z * f, v.w * f));
+    const int mt = warp;
+    auto store = [&](const Part& u, const float4& v, float l0, float l1) {
+        const float f0 = l0 == 0.f ? 0.f : q4::kUnscale / l0, f1 = l1 == 0.f ? 0.f : q4::kUnscale / l1;
+        const int d = g * (HD / 8) + 2 * mt;
+        if (2 * c < u.cols) *reinterpret_cast<uint32_t*>(out_row(u.seq, u.kvh, u.block * 8 + 2 * c) + d) = pack_bf2(v.x * f0, v.z * f0);
+        if (2 * c + 1 < u.cols) *reinterpret_cast<uint32_t*>(out_row(u.seq, u.kvh, u.block * 8 + 2 * c + 1) + d) = pack_bf2(v.y * f1, v.w * f1);
     };
-    auto add = [](float4& sum, const float4& v, float f) { sum.x += v.x * f, sum.y += v.y * f, sum.z += v.z * f, sum.w += v.w * f; };
+    auto add = [](float4& sum, const float4& v, float f0, float f1) { sum.x += v.x * f0, sum.y += v.y * f1, sum.z += v.z * f0, sum.w += v.w * f1; };
+    static_assert(MT <= kWarps, "a warp has a tile of the output");
     int crossing[2] = {-1, -1};  // parts of the units that other blocks share: this block's first and its last one
     for (unsigned h = heads; h; h &= h - 1) {
         const int head = __ffs(h) - 1;
-        const unsigned mine = unit_parts(head);
+        const unsigned all = __shfl_sync(kFull, unit, head);
         const Part u = s_part[head];
-        const bool whole = u.first == 0 && s_part[31 - __clz(mine)].last == u.tiles;
-        const int cols = min(8, (p.q_lens ? p.q_lens[u.seq] : 1) * group - u.block * 8), side = u.start <= block_start ? 0 : 1;
+        const bool whole = u.first == 0 && s_part[31 - __clz(all)].last == u.tiles;
+        const int side = u.start <= block_start ? 0 : 1;
         if (!whole) crossing[side] = head;
-        if (col < cols) {
+        if (mt < MT) {
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (unsigned r = mine; r; r &= r - 1) {
-                const int i = __ffs(r) - 1;
-                add(sum, *reinterpret_cast<const float4*>(part_at(i) + e), s_weight[i][col]);
-            }
+#pragma unroll
+            for (int i = 0; i < kParts; i++)
+                if (all >> i & 1) {
+                    const float4* part = (i & 1) ? reinterpret_cast<const float4*>(smem + (i >> 1) * kStages * Rec::kBytes) : parts + (i >> 1) * MT * 32;
+                    add(sum, part[mt * 32 + lane], s_weight[i][2 * c], s_weight[i][2 * c + 1]);
+                }
             if (whole) {
-                store(u, sum, s_sum[head][col]);
+                store(u, sum, s_sum[head][2 * c], s_sum[head][2 * c + 1]);
             } else {
                 float* dst = p.parts + (size_t)(blockIdx.x * 2 + side) * part_floats<HD>();
-                *reinterpret_cast<float4*>(dst + e) = sum;
-                if (e % HD == 0) dst[8 * HD + col] = s_max[head][col], dst[8 * HD + 8 + col] = s_sum[head][col];
+                reinterpret_cast<float4*>(dst)[mt * 32 + lane] = sum;
+                if (warp == 0 && lane < 8) dst[8 * HD + 2 * lane] = s_max[head][lane], dst[8 * HD + 2 * lane + 1] = s_sum[head][lane];
             }
         }
     }
+    if (crossing[0] < 0 && crossing[1] < 0) return;
     // ---- units of several blocks: whoever arrives last adds up their parts
     const int block_run = kWarps * run;
-    float* const weight = reinterpret_cast<float*>(smem);  // [blocks][8]
-    for (int side = 0; side < 2; side++) {
-        const int head = side ? crossing[1] : crossing[0];
-        if (head < 0) continue;
-        const Part u = s_part[head];
-        const int from = u.start / block_run, to = (u.start + u.tiles - 1) / block_run;
-        __threadfence();  // this block's part is visible before its arrival is counted
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            s_last = atomicAdd(p.counters + from, 1) == to - from;
-            if (s_last) p.counters[from] = 0;
-        }
-        __syncthreads();
-        if (!s_last) continue;
-        __threadfence();
-        auto part = [&](int b) { return p.parts + (size_t)(b * 2 + (u.start <= b * block_run ? 0 : 1)) * part_floats<HD>(); };
-        {  // a warp per column: weights of the blocks' parts, and their sum
-            float m = kFloor, l = 0.f;
-            for (int b = from + lane; b <= to; b += 32) m = fmaxf(m, __ldcg(part(b) + 8 * HD + warp));
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();  // the block's parts are visible before its arrivals are counted
+        int last = 0;
 #pragma unroll
-            for (int sh = 1; sh <= 16; sh <<= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, sh));
+        for (int side = 0; side < 2; side++)
+            if (crossing[side] >= 0) {
+                const Part u = s_part[crossing[side]];
+                const int from = u.start / block_run, to = (u.start + u.tiles - 1) / block_run;
+                if (atomicAdd(p.counters + from, 1) == to - from) {
+                    last |= 1 << side;
+                    p.counters[from] = 0;
+                }
+            }
+        s_last = last;
+        __threadfence();
+    }
+    __syncthreads();
+    float2* const weight = reinterpret_cast<float2*>(smem);  // [blocks][4]: of columns 2c and 2c + 1
+    for (int side = 0; side < 2; side++) {
+        if (!(s_last >> side & 1)) continue;
+        const Part u = s_part[side ? crossing[1] : crossing[0]];
+        const int from = u.start / block_run, to = (u.start + u.tiles - 1) / block_run;
+        auto part = [&](int b) { return p.parts + (size_t)(b * 2 + (u.start <= b * block_run ? 0 : 1)) * part_floats<HD>(); };
+        if (warp < 8) {  // a warp per column: weights of the blocks' parts, and their sum
+            float m = kFloor, l = 0.f;
+            for (int b = from + lane; b <= to; b += 32) m = fmaxf(m, __ldcg(part(b) + 8 * HD + 2 * warp));
+            const float top = [&] {
+                float t = m;
+#pragma unroll
+                for (int sh = 1; sh <= 16; sh <<= 1) t = fmaxf(t, __shfl_xor_sync(kFull, t, sh));
+                return t;
+            }();
             for (int b = from + lane; b <= to; b += 32) {
-                const float f = fast_exp2(__ldcg(part(b) + 8 * HD + warp) - m);
-                l += __ldcg(part(b) + 8 * HD + 8 + warp) * f;
-                weight[(b - from) * 8 + warp] = f;
+                const float2 ml = __ldcg(reinterpret_cast<const float2*>(part(b) + 8 * HD + 2 * warp));
+                const float f = fast_exp2(ml.x - top);
+                l += ml.y * f;
+                reinterpret_cast<float*>(weight)[(b - from) * 8 + warp] = f;
             }
 #pragma unroll
             for (int sh = 1; sh <= 16; sh <<= 1) l += __shfl_xor_sync(kFull, l, sh);
             if (lane == 0) s_sum[0][warp] = l;
         }
         __syncthreads();
-        if (col < min(8, (p.q_lens ? p.q_lens[u.seq] : 1) * group - u.block * 8)) {
+        if (mt < MT) {
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-            for (int b = from; b <= to; b++) add(sum, __ldcg(reinterpret_cast<const float4*>(part(b) + e)), weight[(b - from) * 8 + col]);
-            store(u, sum, s_sum[0][col]);
+            for (int b = from; b <= to; b++) {
+                const float2 f = weight[(b - from) * 4 + c];
+                add(sum, __ldcg(reinterpret_cast<const float4*>(part(b)) + mt * 32 + lane), f.x, f.y);
+            }
+            store(u, sum, s_sum[0][2 * c], s_sum[0][2 * c + 1]);
         }
         __syncthreads();  // the weights and the sums are written again
     }
@@ -502,6 +539,10 @@ int32_t launch(b2_ctx* ctx, Q4AttnParams p) {
         B2_CUDA(cudaMalloc((void**)&ctx->q4_parts, bytes));
         B2_CUDA(cudaMemsetAsync(ctx->q4_parts, 0, bytes, ctx->stream));
     }
+    p.group = p.hq / p.hkv;
+    p.max_ctx = (int)std::min<int64_t>((int64_t)p.max_blocks * p.page_tiles * 16, 0x7ffffff0);
+    p.per_entry = (p.num_seqs + kEntries - 1) / kEntries;
+    p.entries = (p.num_seqs + p.per_entry - 1) / p.per_entry;
     p.parts = ctx->q4_parts;
     p.counters = reinterpret_cast<int*>(ctx->q4_parts + (size_t)grid * 2 * part_floats<128>());
     B2_SMEM_ONCE(ctx, kv_q4_attn_kernel<HD>, smem_bytes<HD>());
