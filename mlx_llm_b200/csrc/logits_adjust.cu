@@ -5,10 +5,12 @@
 // with a bias: v + b;  not allowed: -inf.  The choice is made among these; written out they are rounded to the logits' type.
 //
 // Bound by the bytes of the logits for many rows and by the latency of its phases for few.  A cluster of eight blocks takes a row, each
-// block one eighth of the vocabulary.  A block reads the row's whole history and biases (from L2, but for the first block) and keeps what
-// falls into its eighth: a bit per token that a rule names, and, ranked by these bits, a counter and a bias for each named token.  Shared
-// memory does not grow with the vocabulary that way, so that several blocks fit an SM and one's phases hide behind another's loads; the
-// first logits and mask words are on their way before the first phase.  Counters are integers, so the order of the atomics changes nothing.
+// block one eighth of the vocabulary.  A block reads the row's whole history and biases (from L2, but for the first block) and marks what
+// falls into its eighth: a bit per token that a rule names.  The pass over the logits leaves these out; they are listed, counted by their
+// rank among the bits, and dealt out to the threads one by one, so that a history's favourites, which lie close together in a vocabulary,
+// hold no warp up.  Shared memory does not grow with the vocabulary that way, and several blocks fit an SM, one's phases behind another's
+// loads.  The first logits, mask words and tokens of the history are on their way before the first phase.  Counters are integers, so the
+// order of the atomics changes nothing.
 #include <algorithm>
 
 #include "elt.cuh"
@@ -17,11 +19,9 @@
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kBlocks = 8, kThreads = 512;
-constexpr int kMaxSlice = 24576;        // tokens of a block at a time
+constexpr int kMaxSlice = 40960;        // tokens of a block at a time
 constexpr int kWords = kMaxSlice / 32;
-constexpr int kNamed = 4096;            // named tokens that are kept at a time
-constexpr int kAhead = 4;               // 16-byte pieces of logits that a thread asks for at the start
+constexpr int kNamed = 2048;            // named tokens that are listed at a time
 constexpr uint32_t kSeen = 0x80000000u;
 
 __device__ __forceinline__ uint32_t at_block(uint32_t addr, uint32_t block) {
@@ -29,7 +29,30 @@ __device__ __forceinline__ uint32_t at_block(uint32_t addr, uint32_t block) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(block));
     return r;
 }
-__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
+// Word j of a 16-byte piece of V logits with -inf in the place of those whose bit in `which` is set.
+template <int V>
+__device__ __forceinline__ uint32_t hide(uint32_t u, uint32_t which, int j) {
+    if constexpr (V == 4) {
+        return which >> j & 1 ? 0xff800000u : u;
+    } else {
+        const uint32_t m = which >> (2 * j) & 3, mask = ((m | m << 15) & 0x00010001u) * 0xffffu;
+        return (u & ~mask) | (0xff80ff80u & mask);
+    }
+}
+template <int V>
+__device__ __forceinline__ float largest(const uint32_t (&u)[4]) {  // NaNs do not count
+    if constexpr (V == 4) {
+        return fmaxf(fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1])), fmaxf(__uint_as_float(u[2]), __uint_as_float(u[3])));
+    } else {
+        auto max2 = [](uint32_t a, uint32_t b) {
+            uint32_t d;
+            asm("max.bf16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
+            return d;
+        };
+        const uint32_t m = max2(max2(u[0], u[1]), max2(u[2], u[3]));
+        return fmaxf(bflo(m), bfhi(m));
+    }
+}
 
 struct AdjustParams {
     b2_logit_rules r;
@@ -40,16 +63,19 @@ struct AdjustParams {
     int vocab, slice;  // tokens of a block in one round: a multiple of 32
 };
 
-template <typename T>
-__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, 2) logits_adjust_kernel(const AdjustParams p) {
+// kAhead: 16-byte pieces of logits that a thread asks for together, and tokens of the history
+template <typename T, int kBlocks, int kThreads, int kAhead, int kPerSm>
+__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, kPerSm) logits_adjust_kernel(const AdjustParams p) {
     constexpr int V = 16 / sizeof(T);
     __shared__ uint32_t named[kWords];       // a bit per token of the slice
     __shared__ uint32_t rank_of[kWords];     // named tokens before a word's
-    __shared__ uint32_t counts[kNamed];      // by rank: kSeen, and how often in the answer
-    __shared__ float biases[kNamed];
+    __shared__ uint16_t ids[kNamed];         // by rank: the token,
+    __shared__ uint32_t counts[kNamed];      // kSeen and how often it is in the answer,
+    __shared__ float biases[kNamed];         // its bias
     __shared__ uint32_t s_scan[kThreads / 32];
     __shared__ float sv[kThreads / 32], cv[kBlocks];
     __shared__ int si[kThreads / 32], ci[kBlocks];
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");  // (waited for before another block's shared memory is written)
     pdl_wait();
     const int block = blockIdx.x % kBlocks, row = blockIdx.x / kBlocks, tid = threadIdx.x, lane = tid & 31;
     const b2_logit_rules& r = p.r;
@@ -73,30 +99,61 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, 2) l
         const int whole = vec ? n / V * V : 0;
         uint4 ahead[kAhead];
         uint32_t allow[kAhead];
+        auto ask = [&](int from) {
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int at = (tid + k * kThreads) * V;
-            allow[k] = ~0u;
-            if (at < whole) {
-                ahead[k] = *reinterpret_cast<const uint4*>(in + first + at);
-                if (mask) allow[k] = mask[(first + at) >> 5];  // (first is a multiple of 32)
+            for (int k = 0; k < kAhead; k++) {
+                const int at = (from + tid + k * kThreads) * V;
+                if (at < whole) ahead[k] = *reinterpret_cast<const uint4*>(in + first + at);
             }
-        }
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int at = (from + tid + k * kThreads) * V;
+                allow[k] = mask && at < whole ? mask[(first + at) >> 5] : ~0u;  // (first is a multiple of 32)
+            }
+        };
+        ask(0);
+        // calls f(place of the token in the slice, index) for what this thread has of a list of ids
+        int head[kAhead];  // the first of the history
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) head[k] = h0 + tid + k * kThreads < h1 ? r.history_dev[h0 + tid + k * kThreads] : -1;
+        auto in_slice = [&](int id, int i, auto f) {
+            const uint32_t t = (uint32_t)(id - first);
+            if (id >= first && t < (uint32_t)n) f(t, i);
+        };
+        auto each_seen = [&](auto f) {
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) in_slice(head[k], h0 + tid + k * kThreads, f);
+            for (int i = h0 + tid + kAhead * kThreads; i < h1; i += 4 * kThreads) {
+                int id[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) id[k] = i + k * kThreads < h1 ? r.history_dev[i + k * kThreads] : -1;
+#pragma unroll
+                for (int k = 0; k < 4; k++) in_slice(id[k], i + k * kThreads, f);
+            }
+        };
+        auto each_bias = [&](auto f) {
+            for (int i = b0 + tid; i < b1; i += kThreads) in_slice(r.bias_id_dev[i], i, f);
+        };
         uint32_t total = 0;  // named tokens
         if (h1 > h0 || b1 > b0) {
             for (int i = tid; i < p.slice / 32; i += kThreads) named[i] = 0;
             __syncthreads();
-            auto mark = [&](int id) {
-                const uint32_t t = (uint32_t)(id - first);
-                if (id >= first && t < (uint32_t)n) atomicOr(&named[t >> 5], 1u << (t & 31));
+            auto mark = [&](uint32_t t, int) {  // (a look first: atomics on one word wait for one another, and favourites come in crowds)
+                if (!(named[t >> 5] >> (t & 31) & 1)) atomicOr(&named[t >> 5], 1u << (t & 31));
             };
-            for (int i = h0 + tid; i < h1; i += kThreads) mark(r.history_dev[i]);
-            for (int i = b0 + tid; i < b1; i += kThreads) mark(r.bias_id_dev[i]);
+            each_seen(mark);
+            each_bias(mark);
             __syncthreads();
-            static_assert(kWords <= 2 * kThreads, "two words a thread");
-            const int w = 2 * tid;
-            const uint32_t n0 = w < p.slice / 32 ? __popc(named[w]) : 0, n1 = w + 1 < p.slice / 32 ? __popc(named[w + 1]) : 0;
-            uint32_t incl = n0 + n1;
+            // rank of every word's first bit: a thread has kMine words
+            constexpr int kMine = (kWords + kThreads - 1) / kThreads;
+            const int w = kMine * tid;
+            uint32_t bits[kMine], mine = 0;
+#pragma unroll
+            for (int j = 0; j < kMine; j++) {
+                bits[j] = w + j < p.slice / 32 ? __popc(named[w + j]) : 0;
+                mine += bits[j];
+            }
+            uint32_t incl = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t v = __shfl_up_sync(kFull, incl, o);
@@ -104,121 +161,114 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, 2) l
             }
             if (lane == 31) s_scan[tid >> 5] = incl;
             __syncthreads();
-            uint32_t before = incl - n0 - n1;
+            uint32_t at = incl - mine;
 #pragma unroll
             for (int i = 0; i < kThreads / 32; i++) {
-                if (i < tid >> 5) before += s_scan[i];
+                if (i < tid >> 5) at += s_scan[i];
                 total += s_scan[i];
             }
-            if (w < p.slice / 32) rank_of[w] = before;
-            if (w + 1 < p.slice / 32) rank_of[w + 1] = before + n0;
-        }
-        auto rank = [&](uint32_t t) { return rank_of[t >> 5] + __popc(named[t >> 5] & ((1u << (t & 31)) - 1)); };
-        for (uint32_t from = 0; from == 0 || from < total; from += kNamed) {  // (one round, unless rules name more than kNamed of the slice)
-            const uint32_t kept = min((uint32_t)kNamed, total - from);
-            if (from > 0) __syncthreads();  // the counters of the round before have been read, and this round's tokens written as they are
-            if (kept) {
-                for (uint32_t i = tid; i < kept; i += kThreads) counts[i] = 0, biases[i] = 0.f;
-                __syncthreads();
-                for (int i = h0 + tid; i < h1; i += kThreads) {
-                    const int id = r.history_dev[i];
-                    const uint32_t t = (uint32_t)(id - first);
-                    if (id < first || t >= (uint32_t)n) continue;
-                    const uint32_t at = rank(t) - from;
-                    if (at >= kept) continue;
-                    if (i >= answer)
-                        atomicAdd(&counts[at], 1u);
-                    else
-                        atomicOr(&counts[at], kSeen);
-                }
-                for (int i = b0 + tid; i < b1; i += kThreads) {
-                    const int id = r.bias_id_dev[i];
-                    const uint32_t t = (uint32_t)(id - first);
-                    if (id < first || t >= (uint32_t)n || (i > b0 && r.bias_id_dev[i - 1] == id)) continue;
-                    const uint32_t at = rank(t) - from;
-                    if (at < kept) biases[at] = r.bias_value_dev[i];
-                }
-                __syncthreads();
+#pragma unroll
+            for (int j = 0; j < kMine; j++) {
+                if (w + j < p.slice / 32) rank_of[w + j] = at;
+                at += bits[j];
             }
-            auto ruled = [&](float v, uint32_t at) {
+        }
+        // The others, as they are or -inf: and of a piece only its largest value, a few instructions for eight logits;
+        // which of its tokens that is is looked up at the end.
+        auto allowed = [&](int i) { return !mask || (mask[i >> 5] >> (i & 31) & 1); };
+        float top = -INFINITY;
+        int place = 0;  // its piece, which `keep` holds, or its token behind the pieces
+        uint32_t keep[4] = {};
+        auto piece = [&](const uint4& raw, int at, uint32_t ok) {
+            uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+            constexpr uint32_t kAll = (1u << V) - 1;
+            const uint32_t flags = total ? named[at >> 5] >> (at & 31) & kAll : 0u;
+            ok = ok >> (at & 31) & kAll;
+            if (out) {
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = hide<V>(u[j], ~(ok | flags), j);
+                if ((const void*)out != (const void*)in || ok != kAll) *reinterpret_cast<uint4*>(out + first + at) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+            const uint32_t bad = flags | (ok ^ kAll);
+            if (bad) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) u[j] = hide<V>(u[j], bad, j);
+            }
+            const float x = largest<V>(u);
+            if (x > top) {  // a thread's places ascend, so its first maximum is kept
+                top = x, place = at;
+#pragma unroll
+                for (int j = 0; j < 4; j++) keep[j] = u[j];
+            }
+        };
+        for (int from = 0; from * V < whole; from += kAhead * kThreads) {
+            if (from > 0) ask(from);
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int at = (from + tid + k * kThreads) * V;
+                if (at < whole) piece(ahead[k], at, allow[k]);
+            }
+        }
+        for (int t = whole + tid; t < n; t += kThreads) {
+            if (total && (named[t >> 5] >> (t & 31) & 1)) continue;
+            const float v = allowed(first + t) ? Elt<T>::ld(in + first + t) : -INFINITY;
+            if (v > top) top = v, place = t;
+            if (out) Elt<T>::st(out + first + t, v);
+        }
+        if (top > -INFINITY) {
+            int found = first + place;
+            if (place < whole) {
+#pragma unroll
+                for (int j = V - 1; j >= 0; j--) {
+                    const uint32_t u = keep[j * 4 / V];
+                    const float v = V == 4 ? __uint_as_float(u) : j & 1 ? bfhi(u) : bflo(u);
+                    if (v == top) found = first + place + j;
+                }
+            }
+            take(top, found);
+        }
+        // the named ones, kNamed at a time
+        for (uint32_t from = 0; from < total; from += kNamed) {
+            const uint32_t kept = min((uint32_t)kNamed, total - from);
+            for (uint32_t i = tid; i < kept; i += kThreads) counts[i] = 0, biases[i] = 0.f;
+            __syncthreads();
+            auto rank = [&](uint32_t t) { return rank_of[t >> 5] + __popc(named[t >> 5] & ((1u << (t & 31)) - 1)) - from; };
+            each_seen([&](uint32_t t, int i) {
+                const uint32_t at = rank(t);
+                if (at >= kept) return;
+                ids[at] = (uint16_t)t;  // (whoever writes it writes the same)
+                if (i >= answer)
+                    atomicAdd(&counts[at], 1u);
+                else
+                    atomicOr(&counts[at], kSeen);
+            });
+            each_bias([&](uint32_t t, int i) {
+                const uint32_t at = rank(t);
+                if (at >= kept) return;
+                ids[at] = (uint16_t)t;
+                if (i == b0 || r.bias_id_dev[i - 1] != r.bias_id_dev[i]) biases[at] = r.bias_value_dev[i];
+            });
+            __syncthreads();
+            for (uint32_t at = tid; at < kept; at += kThreads) {
+                const int i = first + ids[at];
+                float v = Elt<T>::ld(in + i);
                 const uint32_t c = counts[at];
                 if (c) v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
                 if (c & ~kSeen) v = __fsub_rn(__fsub_rn(v, __fmul_rn((float)(c & ~kSeen), freq)), pres);
-                return __fadd_rn(v, biases[at]);
-            };
-            auto allowed = [&](int i) { return !mask || (mask[i >> 5] >> (i & 31) & 1); };
-            if (from > 0) {  // only the tokens of these ranks
-                for (int w = tid; w < (n + 31) / 32; w += kThreads)
-                    for (uint32_t bits = named[w]; bits; bits &= bits - 1) {
-                        const uint32_t t = w * 32 + __ffs(bits) - 1, at = rank(t) - from;
-                        if (at >= kept) continue;
-                        const float v = allowed(first + t) ? ruled(Elt<T>::ld(in + first + t), at) : -INFINITY;
-                        take(v > -INFINITY ? v : -INFINITY, v > -INFINITY ? first + t : 0x7fffffff);
-                        if (out) Elt<T>::st(out + first + t, v);
-                    }
-                continue;
+                v = __fadd_rn(v, biases[at]);
+                if (!allowed(i)) v = -INFINITY;
+                if (v > -INFINITY) take(v, i);
+                if (out) Elt<T>::st(out + i, v);
             }
-            // value of token first + t; a named one of a later round stays as it is
-            auto value = [&](float v, uint32_t t, bool is_named, bool ok) {
-                bool later = false;
-                if (is_named) {
-                    const uint32_t at = rank(t);
-                    later = at >= kept;
-                    if (!later) v = ruled(v, at);
-                }
-                if (later) return v;
-                if (!ok) v = -INFINITY;
-                if (v > best) best = v, bi = first + t;  // a thread's indices ascend here, so its first maximum is kept
-                return v;
-            };
-            auto piece = [&](const uint4& raw, int at, uint32_t ok) {
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-                float v[V];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if constexpr (V == 8)
-                        v[2 * j] = bflo(w[j]), v[2 * j + 1] = bfhi(w[j]);
-                    else
-                        v[j] = __uint_as_float(w[j]);
-                }
-                constexpr uint32_t kAll = (1u << V) - 1;
-                const uint32_t flags = total ? named[at >> 5] >> (at & 31) & kAll : 0u;
-                ok = ok >> (at & 31) & kAll;
-                if (flags == 0 && ok == kAll) {
-#pragma unroll
-                    for (int j = 0; j < V; j++)
-                        if (v[j] > best) best = v[j], bi = first + at + j;
-                    if (out && (const void*)out != (const void*)in) *reinterpret_cast<uint4*>(out + first + at) = raw;
-                    return;
-                }
-#pragma unroll
-                for (int j = 0; j < V; j++) v[j] = value(v[j], at + j, flags >> j & 1, ok >> j & 1);
-                if (out) {
-                    if constexpr (V == 8)
-                        Elt<T>::st8(out + first + at, v);
-                    else
-                        Elt<T>::st4(out + first + at, v);
-                }
-            };
-#pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                const int at = (tid + k * kThreads) * V;
-                if (at < whole) piece(ahead[k], at, allow[k]);
-            }
-            for (int at = (tid + kAhead * kThreads) * V; at < whole; at += kThreads * V)
-                piece(*reinterpret_cast<const uint4*>(in + first + at), at, mask ? mask[(first + at) >> 5] : ~0u);
-            for (int t = whole + tid; t < n; t += kThreads) {
-                const float v = value(Elt<T>::ld(in + first + t), t, total && (named[t >> 5] >> (t & 31) & 1), allowed(first + t));
-                if (out) Elt<T>::st(out + first + t, v);
-            }
+            __syncthreads();  // lists and marks have been read
         }
-        if (total) __syncthreads();  // what names tokens has been read
     }
-    if (!p.argmax) return;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) take(__shfl_xor_sync(kFull, best, o), __shfl_xor_sync(kFull, bi, o));
-    if ((tid & 31) == 0) sv[tid >> 5] = best, si[tid >> 5] = bi;
-    cluster_sync();  // (and all blocks of the cluster run)
+    if (lane == 0) sv[tid >> 5] = best, si[tid >> 5] = bi;
+    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+    __syncthreads();
     if (tid < 32) {
         best = tid < kThreads / 32 ? sv[tid] : -INFINITY;
         bi = tid < kThreads / 32 ? si[tid] : 0x7fffffff;
@@ -229,8 +279,10 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, 2) l
             asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(at_block(smem_u32(ci + block), 0)), "r"(bi) : "memory");
         }
     }
-    cluster_sync();
-    if (block == 0 && tid == 0) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    if (block != 0) return;  // (the first block's shared memory is the one that is written)
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (tid == 0 && p.argmax) {
         best = -INFINITY, bi = 0x7fffffff;
 #pragma unroll
         for (int j = 0; j < kBlocks; j++) take(cv[j], ci[j]);
@@ -249,9 +301,13 @@ int32_t b2_logits_adjust_launch(b2_ctx* ctx, const b2_logit_rules& rules, const 
     p.argmax = argmax;
     p.ld = ld;
     p.vocab = vocab;
-    p.slice = std::min(kMaxSlice, ((vocab + kBlocks - 1) / kBlocks + 31) / 32 * 32);
-    auto kernel = f32 ? logits_adjust_kernel<float> : logits_adjust_kernel<uint16_t>;
-    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kernel, dim3(rows * kBlocks), dim3(kThreads), 0, ctx->stream, p));
+    // Few rows: as many threads and loads as a row can use.  Many: fewer blocks, each of which reads the history, so that all rows' phases overlap.
+    const bool few = rows * 8 <= ctx->sm_count;
+    const int blocks = few ? 8 : 4;
+    p.slice = std::min(kMaxSlice, ((vocab + blocks - 1) / blocks + 31) / 32 * 32);
+    auto kernel = f32 ? few ? logits_adjust_kernel<float, 8, 512, 4, 1> : logits_adjust_kernel<float, 4, 512, 2, 3>
+                      : few ? logits_adjust_kernel<uint16_t, 8, 512, 4, 1> : logits_adjust_kernel<uint16_t, 4, 512, 2, 3>;
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kernel, dim3(rows * blocks), dim3(512), 0, ctx->stream, p));
     B2_LAUNCHED(ctx);
     B2_CUDA(cudaGetLastError());
     return B2_OK;

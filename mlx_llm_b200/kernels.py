@@ -4,7 +4,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import check, load, ptr
+from ._lib import DevBuf, check, load, ptr
 
 
 def paged_attn_decode(ctx, q, k_pool, v_pool, block_tables, ctx_lens, num_seqs, hq, hkv, head_dim, page_size, scale,
@@ -29,6 +29,39 @@ def paged_attn_prefill(ctx, q, k_pool, v_pool, block_tables, max_blocks, cu_seql
                                        int(cl.size), int(hq), int(hkv), int(head_dim), int(page_size), C.c_float(scale), ptr(out)))
 
 
+_TYPES = {"p": C.c_void_p, "i": C.c_int32, "l": C.c_int64, "f": C.c_float}
+
+
+class _Entry:
+    """An entry point with declared argument types: numbers and addresses go as they are, which saves a call of many arguments a few microseconds."""
+
+    def __init__(self, name, types):
+        self.name, self.types, self.fn = name, [_TYPES[t] for t in types], None
+
+    def __call__(self, *args):
+        if self.fn is None:
+            self.fn = getattr(load(), self.name)
+            self.fn.argtypes = self.types
+        rc = self.fn(*args)
+        if rc:
+            check(rc)
+
+
+def _at(a):
+    """Address of a device buffer (DevBuf, or a number), a host array, or nothing."""
+    if a is None or type(a) is int:
+        return a
+    if type(a) is DevBuf:
+        return a.ptr
+    return a.ctypes.data if isinstance(a, np.ndarray) else int(a)
+
+
+_append_q4 = _Entry("b2_rope_kv_append_q4", "ppiiiippppppfipippp")
+_decode_q4 = _Entry("b2_paged_attn_decode_q4", "pppipipiiiiifp")
+_prefill_q4 = _Entry("b2_paged_attn_prefill_q4", "pppipippiiiiifp")
+_adjust = _Entry("b2_logits_adjust", "ppiiilppp")
+
+
 def kv_q4_pool_bytes(n_pages, hkv, head_dim, page_size):
     lib = load()
     lib.b2_kv_q4_pool_bytes.restype = C.c_int64
@@ -37,21 +70,19 @@ def kv_q4_pool_bytes(n_pages, hkv, head_dim, page_size):
 
 def rope_kv_append_q4(ctx, qkv, T, hq, hkv, head_dim, positions, slot_mapping, cos, sin, q_norm, k_norm, eps, page_size, kv_pool, n_pages, q_out,
                       k_out=None, v_out=None):
-    check(load().b2_rope_kv_append_q4(ctx.h, ptr(qkv), int(T), int(hq), int(hkv), int(head_dim), ptr(positions), ptr(slot_mapping), ptr(cos), ptr(sin),
-                                      ptr(q_norm), ptr(k_norm), C.c_float(eps), int(page_size), ptr(kv_pool), int(n_pages), ptr(q_out), ptr(k_out),
-                                      ptr(v_out)))
+    _append_q4(ctx.h, _at(qkv), T, hq, hkv, head_dim, _at(positions), _at(slot_mapping), _at(cos), _at(sin), _at(q_norm), _at(k_norm), eps, page_size,
+               _at(kv_pool), n_pages, _at(q_out), _at(k_out), _at(v_out))
 
 
 def paged_attn_decode_q4(ctx, q, kv_pool, n_pages, block_tables, ctx_lens, num_seqs, hq, hkv, head_dim, page_size, scale, out, max_blocks):
-    check(load().b2_paged_attn_decode_q4(ctx.h, ptr(q), ptr(kv_pool), int(n_pages), ptr(block_tables), int(max_blocks), ptr(ctx_lens), int(num_seqs),
-                                         int(hq), int(hkv), int(head_dim), int(page_size), C.c_float(scale), ptr(out)))
+    _decode_q4(ctx.h, _at(q), _at(kv_pool), n_pages, _at(block_tables), max_blocks, _at(ctx_lens), num_seqs, hq, hkv, head_dim, page_size, scale, _at(out))
 
 
 def paged_attn_prefill_q4(ctx, q, kv_pool, n_pages, block_tables, max_blocks, cu_seqlens, ctx_lens, hq, hkv, head_dim, page_size, scale, out):
     cu = np.ascontiguousarray(cu_seqlens, np.int32)
     cl = np.ascontiguousarray(ctx_lens, np.int32)
-    check(load().b2_paged_attn_prefill_q4(ctx.h, ptr(q), ptr(kv_pool), int(n_pages), ptr(block_tables), int(max_blocks), ptr(cu), ptr(cl), int(cl.size),
-                                          int(hq), int(hkv), int(head_dim), int(page_size), C.c_float(scale), ptr(out)))
+    _prefill_q4(ctx.h, _at(q), _at(kv_pool), n_pages, _at(block_tables), max_blocks, cu.ctypes.data, cl.ctypes.data, cl.size, hq, hkv, head_dim, page_size,
+                scale, _at(out))
 
 
 def quantize(ctx, w, out_dim, in_dim, bits, packed, scales, biases, group=64):
@@ -125,12 +156,15 @@ class LogitRules(C.Structure):
 def logit_rules(mask_words=0, **arrays):
     """Rules for logits_adjust: history, history_off, n_prompt, repetition, presence, frequency, bias_id, bias_value, bias_off, mask, mask_row as device
     buffers (None: not used), and the words of a mask's row."""
-    return LogitRules(mask_words=int(mask_words), **{n: ptr(a) for n, a in arrays.items()})
+    rules = LogitRules()
+    rules.mask_words = mask_words
+    for name, a in arrays.items():
+        setattr(rules, name, _at(a))
+    return rules
 
 
 def logits_adjust(ctx, logits, rows, vocab, rules, f32=False, ld=None, out=None, argmax=None):
-    check(load().b2_logits_adjust(ctx.h, ptr(logits), int(f32), int(rows), int(vocab), C.c_int64(vocab if ld is None else ld), C.byref(rules), ptr(out),
-                                  ptr(argmax)))
+    _adjust(ctx.h, _at(logits), f32, rows, vocab, vocab if ld is None else ld, C.addressof(rules), _at(out), _at(argmax))
 
 
 def rope_inv_freq(head_dim, theta, kind=0, factor=1.0, low=1.0, high=4.0, orig=8192.0):
