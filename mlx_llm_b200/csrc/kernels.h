@@ -245,10 +245,9 @@ struct Q4Seq {
     int32_t bt_row, q_row, q_len, ctx;  // block-table row, first query row, query tokens (the last ones of the context), tokens in the cache
 };
 struct Q4Pass {  // sequences whose keys and values are widened to bf16 together
-    int seqs, work, max_ctx;
-    int64_t tiles;        // 16-token tiles of all of them
-    int max_tiles;        // of the longest
-    size_t list, cu;      // list: [seqs] block-table row, context, first tile; cu: rows, contexts and work items as the prefill kernels take them
+    int seqs, work, longest;  // work items, and the tiles of 128 keys that the longest sees
+    int64_t tiles;            // of all sequences
+    size_t list;              // in the plan: [seqs] block-table row, context, first tile, query row, query tokens; [work] sequence, first query token
 };
 struct Q4Plan {
     std::vector<int32_t> host;
@@ -257,7 +256,6 @@ struct Q4Plan {
 };
 struct Q4PrefillParams {
     const uint16_t* q;
-    int q_rows;                   // rows of the q allocation
     const uint8_t* pool;
     int64_t n_pages;
     const int32_t* block_tables;

@@ -35,6 +35,8 @@ __device__ __forceinline__ Scales scales_of(uint32_t s2, uint32_t b2) {
 // one token's, for both halves of a word, and two tokens', one for each half
 __device__ __forceinline__ Scales scales_twice(uint32_t sb) { return scales_of(prmt(sb, 0u, 0x1010u), prmt(sb, 0u, 0x3232u)); }
 __device__ __forceinline__ Scales scales_pair(uint32_t sb0, uint32_t sb1) { return scales_of(prmt(sb0, sb1, 0x5410u), prmt(sb0, sb1, 0x7632u)); }
+// whether a scale or a bias is infinite or NaN
+__device__ __forceinline__ bool poisoned(uint32_t sb) { return (sb & 0x7f80u) == 0x7f80u || (sb & 0x7f800000u) == 0x7f800000u; }
 // nibble i of the low half word beside nibble i of the high one
 __device__ __forceinline__ void values(uint32_t w, const Scales& s, uint32_t (&out)[4]) { scaled_q4_paired(w, s.lo, s.hi, s.bias, out); }
 

@@ -119,10 +119,22 @@ __device__ __forceinline__ void scores(const uint8_t* rec, int lane, const uint3
 #pragma unroll
     for (int j = 0; j < 4; j++) s[j] = (s[j] + s2[j]) * to_log2;
 }
-// O^T[dim, column] += V^T P^T of a record; rows g and g + 8 of tile mt are dims 2 mt and 2 mt + 1 of this lane's block.  `left`: tokens of
-// the record that belong to the context; what lies behind them may be anything, and 0 * NaN is NaN
+// Where columns see different tokens: a value that is NaN must reach those that see it and no others, but the others multiply it too, with
+// zero.  So it makes the token's scores NaN instead, which are masked by choice.
 template <int HD>
-__device__ __forceinline__ void add_values(const uint8_t* rec, int lane, const float (&p)[4], int left, float (&o)[HD / 16][4]) {
+__device__ __forceinline__ void hidden_values(const uint8_t* rec, int lane, float (&s)[4]) {
+    using Rec = q4::Record<HD>;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < Rec::kGroups; i++)
+            if (q4::poisoned(reinterpret_cast<const uint32_t*>(rec + Rec::kVsb)[i * 16 + (lane >> 2) + 8 * h])) s[2 * h] = s[2 * h + 1] = __int_as_float(0x7fc00000);
+}
+// O^T[dim, column] += V^T P^T of a record; rows g and g + 8 of tile mt are dims 2 mt and 2 mt + 1 of this lane's block.  `left`: tokens of
+// the record that belong to the context; what lies behind them may be anything, and 0 * NaN is NaN.  `some`: not every column sees every
+// token, so that values that are NaN have gone into the scores (hidden_values)
+template <int HD>
+__device__ __forceinline__ void add_values(const uint8_t* rec, int lane, const float (&p)[4], int left, bool some, float (&o)[HD / 16][4]) {
     using Rec = q4::Record<HD>;
     constexpr int W = HD / 32;
     const int g = lane >> 2, c = lane & 3;
@@ -133,6 +145,12 @@ __device__ __forceinline__ void add_values(const uint8_t* rec, int lane, const f
         if (2 * c + 1 >= left) sb0.y = 0;
         if (2 * c + 8 >= left) sb1.x = 0;
         if (2 * c + 9 >= left) sb1.y = 0;
+    }
+    if (some) {
+        if (q4::poisoned(sb0.x)) sb0.x = 0;
+        if (q4::poisoned(sb0.y)) sb0.y = 0;
+        if (q4::poisoned(sb1.x)) sb1.x = 0;
+        if (q4::poisoned(sb1.y)) sb1.y = 0;
     }
     uint32_t pb[2], pl[2];
     const uint32_t h01 = pack_bf2(p[0], p[1]), h23 = pack_bf2(p[2], p[3]);
@@ -350,6 +368,11 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
                 else
                     s1[0] = s1[1] = s1[2] = s1[3] = -INFINITY;
                 const int tok0 = t * 16;
+                const bool some = tok0 + 32 > sure && p.q_lens;
+                if (some) {
+                    if (one) hidden_values<HD>(rec0, lane, s0);
+                    if (two) hidden_values<HD>(rec1, lane, s1);
+                }
                 if (tok0 + 32 > sure) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
@@ -376,8 +399,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
                 for (int j = 0; j < 4; j++) s0[j] = fast_exp2(s0[j] - (j & 1 ? m1 : m0)), s1[j] = fast_exp2(s1[j] - (j & 1 ? m1 : m0));
                 l0 += (s0[0] + s0[2]) + (s1[0] + s1[2]);
                 l1 += (s0[1] + s0[3]) + (s1[1] + s1[3]);
-                if (one) add_values<HD>(rec0, lane, s0, use.len.ctx - tok0, o);
-                if (two) add_values<HD>(rec1, lane, s1, use.len.ctx - tok0 - 16, o);
+                if (one) add_values<HD>(rec0, lane, s0, use.len.ctx - tok0, some, o);
+                if (two) add_values<HD>(rec1, lane, s1, use.len.ctx - tok0 - 16, some, o);
             }
             pos += t1 - t0;
 #pragma unroll
@@ -583,6 +606,7 @@ extern "C" int32_t b2_paged_attn_decode_q4(b2_ctx* ctx, const uint16_t* q_dev, c
     B2_REQUIRE(num_seqs >= 0 && max_blocks > 0, B2_ERR_MSG, "b2_paged_attn_decode_q4: bad sizes");
     B2_REQUIRE((double)num_seqs * max_blocks * (page_size / 16) * hkv * ((hq / hkv + 7) / 8) < 1073741824.0, B2_ERR_UNSUPPORTED,
                "b2_paged_attn_decode_q4: the block tables reach more than 2^30 records; make fewer sequences a call");
+    B2_REQUIRE(scale > 0.f && scale < INFINITY, B2_ERR_MSG, "b2_paged_attn_decode_q4: the scale must be positive");
     B2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & 15) == 0, B2_ERR_UNSUPPORTED, "b2_paged_attn_decode_q4: q and out must be 16-byte aligned");
     B2_CUDA(cudaSetDevice(ctx->device));
     Q4AttnParams p{};

@@ -1,18 +1,33 @@
 // Attention over a 4-bit paged cache for any number of query tokens per sequence: prompts, portions of prompts, drafts.
 //
 // Few columns (query tokens x q heads of a group) go through kv_q4_attn.cu, which reads the 4 bits once per 8 columns.  With many, the
-// products decide, not the bytes: the keys and values of a sequence are widened once to bf16 in a workspace, [16-token tile][kv head]
-// [16][head size], and the prefill kernels of the 16-bit cache multiply from there, so that a code is converted once and not once per
-// query tile and head.  The workspace takes whole sequences, up to kPassBytes at a time (a longer sequence alone).
+// products decide, not the bytes, and a code is converted once for all that multiply with it: kv_q4_widen_kernel turns the records of a
+// sequence into bf16 tiles of 128 keys in a workspace, already in the shape that the tensor cores read from shared memory, and
+// kv_q4_prefill_kernel (tcgen05) multiplies from there.  The workspace takes whole sequences, up to kPassBytes at a time (a longer
+// sequence alone).
 #include <algorithm>
 
 #include "kernels.h"
 #include "kv_q4.cuh"
+#include "tc5.cuh"
 
 namespace {
 
+using namespace tc5;
+
 constexpr size_t kPassBytes = 1ull << 30;
 constexpr int kFewColumns = 32;
+constexpr int KT = 128;  // keys of a tile
+
+// A tile of K or V: [HD / 64 halves][128 keys][64 dims] bf16, rows of 128 bytes whose 16-byte pieces are swapped as the 128-byte swizzle
+// wants (piece ^ row % 8).  K is read from it as a K-major operand, V as an MN-major one.
+template <int HD>
+constexpr int tile_bytes() {
+    return KT * HD * 2;
+}
+__device__ __forceinline__ uint32_t tile_at(int row, int dim) {  // of 8 dims
+    return (uint32_t)(dim >> 6) * (KT * 128) + (uint32_t)row * 128u + ((((uint32_t)dim >> 3) & 7u) ^ ((uint32_t)row & 7u)) * 16u;
+}
 
 struct WidenParams {
     const uint8_t* pool;
@@ -22,23 +37,22 @@ struct WidenParams {
     const int32_t *rows, *ctx, *first;  // [seqs] block-table row, context, first tile
     int seqs;
     int64_t tiles;
-    int max_tiles;
-    uint16_t *k, *v;       // [tiles][hkv][16][HD]
-    int32_t* table;        // [seqs][max_tiles] tile numbers: the workspace's block table
+    uint8_t* wide;  // [tiles][hkv][K, V][tile]
 };
 
 // One warp per record.  Bound by its writes, four times what it reads; they stay in L2 for the attention behind it where they fit.
-// Tokens behind the context, and pages outside of the pool, become zeros.
+// Tokens behind the context, and pages outside of the pool, become zeros.  A value that is NaN must reach the rows that see it and no others,
+// but a row that does not still multiplies it, with zero: it goes into the token's keys, whose scores are masked by choice and not by
+// multiplication, and the value becomes zero.
 template <int HD>
 __global__ void __launch_bounds__(256) kv_q4_widen_kernel(const WidenParams p) {
     using Rec = q4::Record<HD>;
     constexpr int W = HD / 32;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     pdl_wait();
-    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (item >= p.tiles * p.hkv) return;
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int tile = (int)(item / p.hkv), kvh = (int)(item - (int64_t)tile * p.hkv);
+    // a block has a tile of one head, a warp one of its eight records
+    const int tile = blockIdx.x / p.hkv, kvh = blockIdx.x - tile * p.hkv;
+    const int sub = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     int lo = 0, hi = p.seqs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -47,32 +61,31 @@ __global__ void __launch_bounds__(256) kv_q4_widen_kernel(const WidenParams p) {
         else
             hi = mid - 1;
     }
-    const int t = tile - p.first[lo], left = p.ctx[lo] - t * 16;  // tokens of this tile that belong to the context
+    const int t = (tile - p.first[lo]) * 8 + sub, left = p.ctx[lo] - t * 16;  // tokens of this record that belong to the context
     const int index = t / p.page_tiles;
-    const int page = p.block_tables[(size_t)p.rows[lo] * p.max_blocks + index];
+    int page = -1;
+    if (left > 0) page = p.block_tables[(size_t)p.rows[lo] * p.max_blocks + index];
     const bool there = page >= 0 && page < p.n_pages;
-    if (kvh == 0 && lane == 0) p.table[(size_t)lo * p.max_tiles + t] = tile;
-    const uint8_t* rec = p.pool + (((size_t)(there ? page : 0) * p.hkv + kvh) * p.page_tiles + t - index * p.page_tiles) * Rec::kBytes;
-    auto wide = [](uint32_t v) { return mul_bf2(v, 0x5f805f80u); };  // times 2^64
-    auto store = [](uint16_t* dst, const uint32_t (&v)[W * 2]) {     // W * 4 values
-#pragma unroll
-        for (int i = 0; i < W / 2; i++) reinterpret_cast<uint4*>(dst)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    };
-    const size_t base = (size_t)item * 16 * HD;
+    const uint8_t* rec = p.pool + (((size_t)(there ? page : 0) * p.hkv + kvh) * p.page_tiles + (there ? t - index * p.page_tiles : 0)) * Rec::kBytes;
+    uint8_t* const k = p.wide + (size_t)blockIdx.x * 2 * tile_bytes<HD>();
+    uint8_t* const v = k + tile_bytes<HD>();
+    auto wide = [](uint32_t x) { return mul_bf2(x, 0x5f805f80u); };  // times 2^64
 #pragma unroll
     for (int half = 0; half < 2; half++) {
         {  // K: token g + 8 half, dims c HD/4 ...
             const int tok = g + 8 * half;
-            const q4::Scales q = q4::scales_twice(reinterpret_cast<const uint32_t*>(rec + Rec::kKsb)[(c * (HD / 4) / 64) * 16 + tok]);
+            const bool ok = there && tok < left;
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < Rec::kGroups; i++) bad |= q4::poisoned(reinterpret_cast<const uint32_t*>(rec + Rec::kVsb)[i * 16 + tok]);
+            const q4::Scales q = q4::scales_twice(bad ? 0x7fc07fc0u : reinterpret_cast<const uint32_t*>(rec + Rec::kKsb)[(c * (HD / 4) / 64) * 16 + tok]);
             const uint32_t* src = reinterpret_cast<const uint32_t*>(rec) + (half * 32 + lane) * W;
-            uint16_t* dst = p.k + base + (size_t)tok * HD + c * (HD / 4);
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                uint32_t v[4];
-                q4::values(src[w], q, v);  // (0,4) (1,5) (2,6) (3,7)
-                const bool ok = there && tok < left;
-                const uint4 r = make_uint4(wide(prmt(v[0], v[1], 0x5410u)), wide(prmt(v[2], v[3], 0x5410u)), wide(prmt(v[0], v[1], 0x7632u)), wide(prmt(v[2], v[3], 0x7632u)));
-                reinterpret_cast<uint4*>(dst)[w] = ok ? r : make_uint4(0, 0, 0, 0);
+                uint32_t x[4];
+                q4::values(src[w], q, x);  // (0,4) (1,5) (2,6) (3,7)
+                const uint4 r = make_uint4(wide(prmt(x[0], x[1], 0x5410u)), wide(prmt(x[2], x[3], 0x5410u)), wide(prmt(x[0], x[1], 0x7632u)), wide(prmt(x[2], x[3], 0x7632u)));
+                *reinterpret_cast<uint4*>(k + tile_at(sub * 16 + tok, c * (HD / 4) + 8 * w)) = ok ? r : make_uint4(0, 0, 0, 0);
             }
         }
         {  // V: tokens 8 half + 2c and the next, dims g HD/8 ...
@@ -80,71 +93,481 @@ __global__ void __launch_bounds__(256) kv_q4_widen_kernel(const WidenParams p) {
             const uint2 sb = *reinterpret_cast<const uint2*>(rec + Rec::kVsb + ((g * (HD / 8) / 64) * 16 + tok) * 4);
             const q4::Scales q = q4::scales_pair(sb.x, sb.y);
             const uint32_t* src = reinterpret_cast<const uint32_t*>(rec + Rec::kV) + (half * 32 + lane) * W;
-            uint32_t a[2 * W], b[2 * W];
-            const bool ok0 = there && tok < left, ok1 = there && tok + 1 < left;
+            const bool ok0 = there && tok < left && !q4::poisoned(sb.x), ok1 = there && tok + 1 < left && !q4::poisoned(sb.y);
 #pragma unroll
-            for (int w = 0; w < W; w++) {
-                uint32_t v[4];
-                q4::values(src[w], q, v);  // dim i of both tokens
-                a[2 * w] = ok0 ? wide(prmt(v[0], v[1], 0x5410u)) : 0u, a[2 * w + 1] = ok0 ? wide(prmt(v[2], v[3], 0x5410u)) : 0u;
-                b[2 * w] = ok1 ? wide(prmt(v[0], v[1], 0x7632u)) : 0u, b[2 * w + 1] = ok1 ? wide(prmt(v[2], v[3], 0x7632u)) : 0u;
+            for (int w = 0; w < W; w += 2) {
+                uint32_t x[4], y[4];
+                q4::values(src[w], q, x);  // dim i of both tokens
+                q4::values(src[w + 1], q, y);
+                const uint4 a = make_uint4(wide(prmt(x[0], x[1], 0x5410u)), wide(prmt(x[2], x[3], 0x5410u)), wide(prmt(y[0], y[1], 0x5410u)), wide(prmt(y[2], y[3], 0x5410u)));
+                const uint4 b = make_uint4(wide(prmt(x[0], x[1], 0x7632u)), wide(prmt(x[2], x[3], 0x7632u)), wide(prmt(y[0], y[1], 0x7632u)), wide(prmt(y[2], y[3], 0x7632u)));
+                *reinterpret_cast<uint4*>(v + tile_at(sub * 16 + tok, g * (HD / 8) + 4 * w)) = ok0 ? a : make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(v + tile_at(sub * 16 + tok + 1, g * (HD / 8) + 4 * w)) = ok1 ? b : make_uint4(0, 0, 0, 0);
             }
-            uint16_t* dst = p.v + base + (size_t)tok * HD + g * (HD / 8);
-            store(dst, a);
-            store(dst + HD, b);
         }
     }
 }
 
+// ---- the products ------------------------------------------------------------------------------------------------------
+// CTA = (two blocks of query rows, kv head[, split of the keys]).  A row is a (query token, q head of the group) pair, the heads of a token
+// next to one another, so that a group shares every tile of K and V, and the two blocks of 128 rows share them again.
+//   warps 0-3, 4-7  softmax of block A, B: thread = row = TMEM lane.  Reads its 128 scores once; exp2 against a running reference that is
+//                   raised only when a tile exceeds it by more than 2^8 (O is touched only then); P goes as bf16 over the scores' columns.
+//   warp 8          copies tiles, whole (32 or 16 KB each), into a ring of five
+//   warp 9          one thread issues S = Q K^T and O += P V with P from tensor memory, for A and B in turn: while one block's softmax runs,
+//                   the tensor cores have the other's products.  S(j + 1) of a block goes over P(j), which the in-order pipe has read by then;
+//                   and when S(j) is there, P V of j - 1 has completed, so O may be rescaled.
+// Bound by the tensor cores: 4 x 128 x 128 x HD multiply-adds per pair of blocks and tile.  P carries 8 bits (one rounding of each weight,
+// relative 2^-9; their sum is taken before the rounding, whose errors have no sign of their own): a second product for the rest of P
+// would cost half as much again.
+constexpr int kRows = 128, kSlots = 5, kThreads = 320;
+constexpr float kRaise = 8.f, kFloor = -1e30f;
+template <int HD>
+struct Smem {
+    static constexpr int kQ = 0, kRing = 2 * tile_bytes<HD>(), kBar = kRing + kSlots * tile_bytes<HD>(), kBytes = kBar + 256;
+};
+constexpr uint32_t kIdesc128 = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+template <int HD>
+constexpr uint32_t idesc_pv() {  // N = HD, B MN-major
+    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+struct ProductParams {
+    const uint16_t* q;
+    const uint8_t* wide;
+    const int32_t *q_row, *q_len, *ctx, *first;  // [seqs]
+    const int32_t *work_seq, *work_q;            // [items] sequence, first query token
+    int hq, hkv, group, per_block;               // query tokens of a block of rows
+    float scale_log2;
+    uint16_t* out;
+    int splits;
+    float* part_o;   // [item][kv head][split][256 rows][HD], unnormalised
+    float* part_ml;  // [item][kv head][split][256 rows][2]: reference (log2 domain), sum
+    int* err;
+};
+struct Item {
+    int seq, q0, queries, ctx, before, tiles, first_tile, n_tiles;
+};
+__device__ __forceinline__ Item item_of(const ProductParams& p, int item, int split) {
+    Item w;
+    w.seq = p.work_seq[item];
+    w.q0 = p.work_q[item];
+    w.queries = min(2 * p.per_block, p.q_len[w.seq] - w.q0);
+    w.ctx = p.ctx[w.seq];
+    w.before = w.ctx - p.q_len[w.seq];
+    w.tiles = (w.before + w.q0 + w.queries - 1) / KT + 1;  // up to the last key that its last query sees
+    const int per = (w.tiles + p.splits - 1) / p.splits;
+    w.first_tile = split * per;
+    w.n_tiles = min(per, w.tiles - w.first_tile);
+    return w;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t two(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
+__device__ __forceinline__ uint64_t twice(float x) { return two(__float_as_uint(x), __float_as_uint(x)); }
+__device__ __forceinline__ float low(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float high(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const ProductParams p) {
+    using S = Smem<HD>;
+    constexpr int TILE = tile_bytes<HD>(), HALF = KT * 128;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    pdl_wait();
+    const uint32_t base = smem_u32(smem);
+    if (base & 1023u) {  // the swizzled tiles need this alignment; every thread sees the same value
+        if (threadIdx.x == 0) atomicExch(p.err, 7);
+        return;
+    }
+    const int kvh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const Item w = item_of(p, blockIdx.y, blockIdx.z);
+    if (w.n_tiles <= 0) return;  // (the merge leaves such splits out)
+    const uint32_t bar = base + S::kBar;
+    const uint32_t q_full = bar;
+    auto full = [&](int s) { return bar + 8u * (1 + s); };
+    auto empty = [&](int s) { return bar + 8u * (6 + s); };
+    auto s_ready = [&](int x) { return bar + 8u * (11 + x); };
+    auto p_ready = [&](int x) { return bar + 8u * (13 + x); };
+    const uint32_t o_ready = bar + 8u * 15, slot_addr = bar + 8u * 16;
+    if (tid == 0) {
+        mbar_init(q_full, 8);
+        for (int s = 0; s < kSlots; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+        for (int x = 0; x < 2; x++) mbar_init(s_ready(x), 1), mbar_init(p_ready(x), 4);
+        mbar_init(o_ready, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(slot_addr), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot_addr - base));
+    const int n = w.n_tiles;
+    bool alive = true;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            const uint8_t* src = p.wide + ((size_t)(p.first[w.seq] + w.first_tile) * p.hkv + kvh) * 2 * TILE;
+            const size_t step = (size_t)p.hkv * 2 * TILE;
+            int slot = 0, asked = 0;
+            uint32_t parity = 0;  // of the slot's present use
+            for (int i = 0; i < 2 * n; i++) {  // K0 V0 K1 V1 ...
+                if (!mbar_wait(empty(slot), parity ^ 1u)) {
+                    alive = false;
+                    break;
+                }
+                mbar_expect_tx(full(slot), TILE);
+                bulk_load(base + S::kRing + slot * TILE, src + (i >> 1) * step + (i & 1) * TILE, TILE, full(slot));
+                asked++;
+                if (++slot == kSlots) slot = 0, parity ^= 1u;
+            }
+            if (!alive) {  // nothing may be on its way when the block ends
+                atomicExch(p.err, 2);
+                for (int i = max(0, asked - kSlots); i < asked; i++) mbar_wait(full(i % kSlots), (uint32_t)(i / kSlots) & 1u);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if (lane == 0) {
+            auto issue_s = [&](int x, int slot) {  // S of block x
+#pragma unroll
+                for (int k = 0; k < HD / 16; k++) {
+                    const uint32_t off = (uint32_t)(k >> 2) * HALF + (uint32_t)(k & 3) * 32u;
+                    tc_mma(tmem + x * 128u, desc_kmajor(base + S::kQ + x * TILE + off), desc_kmajor(base + S::kRing + slot * TILE + off), kIdesc128, k > 0 ? 1u : 0u);
+                }
+                tc_commit(s_ready(x));
+            };
+            auto issue_o = [&](int x, int slot, bool add) {  // O of block x
+#pragma unroll
+                for (int k = 0; k < KT / 16; k++)
+                    tc_mma_ts(tmem + 256u + x * 128u, tmem + x * 128u + k * 8u, desc_mnmajor(base + S::kRing + slot * TILE + k * 2048u, HALF), idesc_pv<HD>(),
+                              add || k > 0 ? 1u : 0u);
+            };
+            int slot = 0;
+            uint32_t parity = 0;
+            auto advance = [&] {
+                if (++slot == kSlots) slot = 0, parity ^= 1u;
+            };
+            alive = mbar_wait(q_full, 0) && mbar_wait(full(0), 0);
+            if (alive) {
+                tc_fence_after();
+                issue_s(0, 0);
+                issue_s(1, 0);
+                tc_commit(empty(0));
+                advance();
+            }
+            for (int j = 0; j < n && alive; j++) {
+                const int v = slot;
+                alive = mbar_wait(full(v), parity) && mbar_wait(p_ready(0), (uint32_t)j & 1u);
+                if (!alive) break;
+                tc_fence_after();
+                issue_o(0, v, j > 0);
+                advance();
+                const int k = slot;
+                if (j + 1 < n) {
+                    alive = mbar_wait(full(k), parity);
+                    if (!alive) break;
+                    tc_fence_after();
+                    issue_s(0, k);
+                }
+                alive = mbar_wait(p_ready(1), (uint32_t)j & 1u);
+                if (!alive) break;
+                tc_fence_after();
+                issue_o(1, v, j > 0);
+                tc_commit(empty(v));
+                if (j + 1 < n) {
+                    issue_s(1, k);
+                    tc_commit(empty(k));
+                    advance();
+                }
+            }
+            tc_commit(o_ready);  // (also after a wait that ran out: what is under way ends before the block does)
+            if (!alive) {
+                atomicExch(p.err, 3);
+                mbar_wait(o_ready, 0);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int x = warp >> 2, r = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int query = x * p.per_block + r / p.group, head = kvh * p.group + r % p.group;  // query: of the item
+        const bool row_ok = r < p.per_block * p.group && query < w.queries;
+        const size_t row = (size_t)(p.q_row[w.seq] + w.q0 + (row_ok ? query : 0)) * p.hq + head % p.hq;
+        {  // this thread's row of Q
+            const uint4* src = reinterpret_cast<const uint4*>(p.q + row * HD);
+            uint8_t* dst = smem + S::kQ + x * TILE;
+            uint4 v[HD / 8];
+#pragma unroll
+            for (int i = 0; i < HD / 8; i++) v[i] = row_ok ? src[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < HD / 8; i++) *reinterpret_cast<uint4*>(dst + tile_at(r, 8 * i)) = v[i];
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        // last key that the row sees; rows without a query see all (nothing comes of them)
+        const int sees = row_ok ? w.before + w.q0 + query : 0x3fffffff;
+        const uint32_t ts = tmem + lanes + x * 128u, to = tmem + lanes + 256u + x * 128u;
+        float m = kFloor, l = 0.f;
+        for (int j = 0; j < n; j++) {
+            if (!__all_sync(0xffffffffu, mbar_wait(s_ready(x), (uint32_t)j & 1u))) {
+                alive = false;
+                break;
+            }
+            tc_fence_after();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; c++) tc_ld32_nowait(ts + c * 32u, s[c]);
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+            const int key0 = (w.first_tile + j) * KT;
+            if (key0 + KT - 1 > sees) {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (key0 + c * 32 + i > sees) s[c][i] = 0xff800000u;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;  // (the scale is positive)
+            float alpha = 1.f;
+            if (j == 0) {
+                m = fmaxf(top, kFloor);
+            } else if (top > m + kRaise) {
+                alpha = fast_exp2(m - top);
+                m = top;
+            }
+            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                l *= alpha;
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; c++) {
+                    uint32_t v[32];
+                    tc_ld32(to + c * 32u, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                    tc_st32(to + c * 32u, v);
+                }
+            }
+            const uint64_t sc = twice(p.scale_log2), neg = twice(-m);
+            uint64_t sum[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t h[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const uint64_t e = fma2(two(s[c][2 * i], s[c][2 * i + 1]), sc, neg);
+                    const float a = fast_exp2(low(e)), b = fast_exp2(high(e));
+                    sum[i & 1] = add2(sum[i & 1], two(__float_as_uint(a), __float_as_uint(b)));
+                    h[i] = pack_bf2(a, b);
+                }
+                tc_st16_nowait(ts + c * 16u, h);
+            }
+            const uint64_t both = add2(sum[0], sum[1]);
+            l += low(both) + high(both);
+            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready(x));
+        }
+        if (alive && !__all_sync(0xffffffffu, mbar_wait(o_ready, 0))) alive = false;
+        if (alive) {
+            tc_fence_after();
+            const bool part = p.splits > 1;
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            const size_t at = (((size_t)blockIdx.y * p.hkv + kvh) * p.splits + blockIdx.z) * (2 * kRows) + x * kRows + r;
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; c++) {
+                uint32_t v[32];
+                tc_ld32(to + c * 32u, v);
+                if (!row_ok) continue;
+                if (part) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        reinterpret_cast<uint4*>(p.part_o + at * HD + c * 32)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                } else {
+                    uint32_t h[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) h[i] = pack_bf2(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        reinterpret_cast<uint4*>(p.out + row * HD + c * 32)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+                }
+            }
+            if (part && row_ok) p.part_ml[2 * at] = m, p.part_ml[2 * at + 1] = l;
+        } else if (lane == 0) {
+            atomicExch(p.err, 4);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Sum of the splits of an item, in their order: a warp per row, HD / 32 dims a lane.
+template <int HD>
+__global__ void __launch_bounds__(256) kv_q4_prefill_merge_kernel(const ProductParams p) {
+    constexpr int D = HD / 32;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    pdl_wait();
+    const int kvh = blockIdx.x, item = blockIdx.y, lane = threadIdx.x & 31;
+    const int r = blockIdx.z * 8 + (threadIdx.x >> 5);  // row of the item
+    const Item w = item_of(p, item, 0);
+    const int in_block = r & (kRows - 1), query = (r / kRows) * p.per_block + in_block / p.group;
+    if (in_block >= p.per_block * p.group || query >= w.queries) return;
+    const int per = (w.tiles + p.splits - 1) / p.splits, used = (w.tiles + per - 1) / per;  // splits that had tiles
+    const size_t at = (((size_t)item * p.hkv + kvh) * p.splits) * (2 * kRows) + r;
+    float m = kFloor;
+    for (int z = 0; z < used; z++) m = fmaxf(m, p.part_ml[2 * (at + (size_t)z * 2 * kRows)]);
+    float l = 0.f, o[D] = {};
+    for (int z = 0; z < used; z++) {
+        const size_t s = at + (size_t)z * 2 * kRows;
+        const float f = fast_exp2(p.part_ml[2 * s] - m);
+        l += f * p.part_ml[2 * s + 1];
+#pragma unroll
+        for (int i = 0; i < D; i += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(p.part_o + s * HD + lane * D + i);
+            o[i] += f * v.x, o[i + 1] += f * v.y;
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint16_t* dst = p.out + ((size_t)(p.q_row[w.seq] + w.q0 + query) * p.hq + (size_t)kvh * p.group + in_block % p.group) * HD + lane * D;
+#pragma unroll
+    for (int i = 0; i < D; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf2(o[i] * inv, o[i + 1] * inv);
+}
+
+int rows_per_block(int group) { return kRows / group; }
+
 }  // namespace
 
 int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int hkv, int head_dim, Q4Plan& plan) {
+    (void)ctx;
     plan = Q4Plan{};
-    const int group = hq / hkv, q_tile = b2_prefill_q_tile(ctx, head_dim);
+    const int group = hq / hkv;
     std::vector<Q4Seq> few, many;
     for (const Q4Seq& s : seqs)
-        if (s.q_len > 0) ((long)s.q_len * group <= kFewColumns ? few : many).push_back(s);
+        if (s.q_len > 0) ((long)s.q_len * group <= kFewColumns || group > kRows ? few : many).push_back(s);
     plan.few = (int)few.size();
     for (const Q4Seq& s : few) plan.host.push_back(s.bt_row);
     for (const Q4Seq& s : few) plan.host.push_back(s.q_row);
     for (const Q4Seq& s : few) plan.host.push_back(s.q_len);
     for (const Q4Seq& s : few) plan.host.push_back(s.ctx);
-    const size_t tile_bytes = (size_t)hkv * 16 * head_dim * 4;
+    const size_t bytes = (size_t)hkv * 2 * KT * head_dim * 2;  // of a tile of keys, all heads
+    const int step = 2 * rows_per_block(std::min(group, kRows));  // query tokens of an item
     for (size_t from = 0; from < many.size();) {
         Q4Pass pass{};
         size_t to = from;
         for (; to < many.size(); to++) {
-            const int64_t tiles = (many[to].ctx + 15) / 16;
-            if (to > from && (pass.tiles + tiles) * tile_bytes > kPassBytes) break;
+            const int64_t tiles = ((int64_t)many[to].ctx + KT - 1) / KT;
+            if (to > from && (size_t)(pass.tiles + tiles) * bytes > kPassBytes) break;
             pass.tiles += tiles;
-            pass.max_tiles = std::max(pass.max_tiles, (int)tiles);
-            pass.max_ctx = std::max(pass.max_ctx, many[to].ctx);
         }
         const int n = pass.seqs = (int)(to - from);
         pass.list = plan.host.size();
+        auto list = [&](auto number) {
+            for (size_t i = from; i < to; i++) plan.host.push_back(number(many[i]));
+        };
+        list([](const Q4Seq& s) { return s.bt_row; });
+        list([](const Q4Seq& s) { return s.ctx; });
         int32_t tile = 0;
-        for (size_t i = from; i < to; i++) plan.host.push_back(many[i].bt_row);
-        for (size_t i = from; i < to; i++) plan.host.push_back(many[i].ctx);
-        for (size_t i = from; i < to; i++) {
-            plan.host.push_back(tile);
-            tile += (many[i].ctx + 15) / 16;
+        list([&](const Q4Seq& s) {
+            const int32_t first = tile;
+            tile += (s.ctx + KT - 1) / KT;
+            return first;
+        });
+        list([](const Q4Seq& s) { return s.q_row; });
+        list([](const Q4Seq& s) { return s.q_len; });
+        // the longest items first, so that the last ones to start are short
+        struct Work {
+            int32_t seq, q, tiles;
+        };
+        std::vector<Work> work;
+        for (int i = 0; i < n; i++) {
+            const Q4Seq& s = many[from + i];
+            for (int q = 0; q < s.q_len; q += step) work.push_back({i, q, (s.ctx - s.q_len + std::min(q + step, s.q_len) - 1) / KT + 1});
         }
-        // The prefill kernels take the rows of sequence b from cu[b] and cu[b + 1].  Theirs need not lie behind one another here, so
-        // sequence i is number 2i, and the odd numbers have no work: rows [2n], then contexts [2n], workspace table rows [2n].
-        pass.cu = plan.host.size();
-        for (size_t i = from; i < to; i++) plan.host.insert(plan.host.end(), {many[i].q_row, many[i].q_row + many[i].q_len});
-        for (size_t i = from; i < to; i++) plan.host.insert(plan.host.end(), {many[i].ctx, 0});
-        for (int i = 0; i < n; i++) plan.host.insert(plan.host.end(), {i, 0});
-        for (int i = 0; i < n; i++)
-            for (int r = 0; r < many[from + i].q_len; r += q_tile) pass.work++;
-        for (int i = 0; i < n; i++)
-            for (int r = 0; r < many[from + i].q_len; r += q_tile) plan.host.push_back(2 * i);
-        for (int i = 0; i < n; i++)
-            for (int r = 0; r < many[from + i].q_len; r += q_tile) plan.host.push_back(r);
-        plan.host.push_back(pass.work);
+        std::stable_sort(work.begin(), work.end(), [](const Work& a, const Work& b) { return a.tiles > b.tiles; });
+        pass.work = (int)work.size();
+        pass.longest = work[0].tiles;
+        for (const Work& x : work) plan.host.push_back(x.seq);
+        for (const Work& x : work) plan.host.push_back(x.q);
         plan.passes.push_back(pass);
         from = to;
     }
+    return B2_OK;
+}
+
+template <int HD>
+static int32_t launch_pass(b2_ctx* ctx, const Q4PrefillParams& p, const Q4Pass& pass, const int32_t* plan_dev) {
+    WidenParams w{};
+    w.pool = p.pool;
+    w.n_pages = p.n_pages;
+    w.block_tables = p.block_tables;
+    w.max_blocks = p.max_blocks;
+    w.hkv = p.hkv;
+    w.page_tiles = p.page_tiles;
+    w.rows = plan_dev + pass.list;
+    w.ctx = w.rows + pass.seqs;
+    w.first = w.ctx + pass.seqs;
+    w.seqs = pass.seqs;
+    w.tiles = pass.tiles;
+    w.wide = ctx->q4_wide;
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_widen_kernel<HD>, dim3((unsigned)(pass.tiles * p.hkv)), dim3(256), 0, ctx->stream, w));
+    B2_LAUNCHED(ctx);
+    ProductParams a{};
+    a.q = p.q;
+    a.wide = ctx->q4_wide;
+    a.ctx = w.ctx;
+    a.first = w.first;
+    a.q_row = w.first + pass.seqs;
+    a.q_len = a.q_row + pass.seqs;
+    a.work_seq = a.q_len + pass.seqs;
+    a.work_q = a.work_seq + pass.work;
+    a.hq = p.hq;
+    a.hkv = p.hkv;
+    a.group = p.hq / p.hkv;
+    a.per_block = rows_per_block(a.group);
+    a.scale_log2 = p.scale_log2;
+    a.out = p.out;
+    a.err = ctx->dev_err;
+    // A CTA fills an SM.  Where the items leave half of the SMs idle, the keys are split as well, four tiles a split at least.
+    const int ctas = pass.work * p.hkv;
+    a.splits = ctas * 2 <= ctx->sm_count ? std::max(1, std::min({ctx->sm_count / ctas, pass.longest / 4, 16})) : 1;
+    if (a.splits > 1) {
+        const size_t slots = (size_t)ctas * a.splits * 2 * kRows, bytes = slots * (HD + 2) * sizeof(float);
+        if (bytes > ctx->pf_part_bytes) {
+            B2_CUDA(cudaStreamSynchronize(ctx->stream));
+            if (ctx->pf_part) B2_CUDA(cudaFree(ctx->pf_part));
+            ctx->pf_part = nullptr;
+            ctx->pf_part_bytes = 0;
+            B2_CUDA(cudaMalloc((void**)&ctx->pf_part, bytes + (bytes >> 2)));
+            ctx->pf_part_bytes = bytes + (bytes >> 2);
+        }
+        a.part_o = ctx->pf_part;
+        a.part_ml = ctx->pf_part + slots * HD;
+    }
+    B2_SMEM_ONCE(ctx, kv_q4_prefill_kernel<HD>, Smem<HD>::kBytes);
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_kernel<HD>, dim3(p.hkv, pass.work, a.splits), dim3(kThreads), (size_t)Smem<HD>::kBytes, ctx->stream, a));
+    B2_LAUNCHED(ctx);
+    if (a.splits > 1) {
+        B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_merge_kernel<HD>, dim3(p.hkv, pass.work, 2 * kRows / 8), dim3(256), 0, ctx->stream, a));
+        B2_LAUNCHED(ctx);
+    }
+    B2_CUDA(cudaGetLastError());
     return B2_OK;
 }
 
@@ -169,8 +592,10 @@ int32_t b2_kv_q4_prefill_launch(b2_ctx* ctx, const Q4PrefillParams& p, int head_
         B2_CHECK(b2_kv_q4_attn_launch(ctx, a, head_dim));
     }
     size_t need = 0;
-    for (const Q4Pass& pass : plan.passes)
-        need = std::max(need, (size_t)pass.tiles * p.hkv * 16 * head_dim * 4 + (size_t)pass.seqs * pass.max_tiles * 4);
+    for (const Q4Pass& pass : plan.passes) {
+        B2_REQUIRE(pass.tiles * p.hkv < (1ll << 31) && pass.work <= 65535, B2_ERR_UNSUPPORTED, "attention over a 4-bit cache: too many query tokens or too long a context for one call");
+        need = std::max(need, (size_t)pass.tiles * p.hkv * 2 * KT * head_dim * 2);
+    }
     if (need > ctx->q4_wide_bytes) {
         B2_CUDA(cudaStreamSynchronize(ctx->stream));
         if (ctx->q4_wide) B2_CUDA(cudaFree(ctx->q4_wide));
@@ -179,50 +604,7 @@ int32_t b2_kv_q4_prefill_launch(b2_ctx* ctx, const Q4PrefillParams& p, int head_
         B2_CUDA(cudaMalloc((void**)&ctx->q4_wide, need + (need >> 2)));
         ctx->q4_wide_bytes = need + (need >> 2);
     }
-    for (const Q4Pass& pass : plan.passes) {
-        const size_t elems = (size_t)pass.tiles * p.hkv * 16 * head_dim;
-        WidenParams w{};
-        w.pool = p.pool;
-        w.n_pages = p.n_pages;
-        w.block_tables = p.block_tables;
-        w.max_blocks = p.max_blocks;
-        w.hkv = p.hkv;
-        w.page_tiles = p.page_tiles;
-        w.rows = plan_dev + pass.list;
-        w.ctx = w.rows + pass.seqs;
-        w.first = w.ctx + pass.seqs;
-        w.seqs = pass.seqs;
-        w.tiles = pass.tiles;
-        w.max_tiles = pass.max_tiles;
-        w.k = reinterpret_cast<uint16_t*>(ctx->q4_wide);
-        w.v = w.k + elems;
-        w.table = reinterpret_cast<int32_t*>(w.v + elems);
-        const dim3 grid((unsigned)((pass.tiles * p.hkv + 7) / 8));
-        B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, head_dim == 128 ? kv_q4_widen_kernel<128> : kv_q4_widen_kernel<64>, grid, dim3(256), 0, ctx->stream, w));
-        B2_LAUNCHED(ctx);
-        PrefillAttnParams a{};
-        a.q = p.q;
-        a.k_pool = w.k;
-        a.v_pool = w.v;
-        a.block_tables = w.table;
-        a.max_blocks = pass.max_tiles;
-        a.cu_seqlens = plan_dev + pass.cu;
-        a.context_lens = a.cu_seqlens + 2 * pass.seqs;
-        a.seq_slot = a.context_lens + 2 * pass.seqs;
-        a.pf_seq = a.seq_slot + 2 * pass.seqs;
-        a.pf_qstart = a.pf_seq + pass.work;
-        a.n_work = a.pf_qstart + pass.work;
-        a.hq = p.hq;
-        a.hkv = p.hkv;
-        a.page_tiles = 1;
-        a.scale_log2 = p.scale_log2;
-        a.out = p.out;
-        a.q_tile = b2_prefill_q_tile(ctx, head_dim);
-        a.q_rows = p.q_rows;
-        a.pool_rows = pass.tiles * p.hkv * 16;
-        a.max_ctx = pass.max_ctx;
-        B2_CHECK(b2_prefill_attn_launch(ctx, a, head_dim, pass.work));
-    }
+    for (const Q4Pass& pass : plan.passes) B2_CHECK(head_dim == 128 ? launch_pass<128>(ctx, p, pass, plan_dev) : launch_pass<64>(ctx, p, pass, plan_dev));
     return B2_OK;
 }
 
@@ -232,6 +614,7 @@ extern "C" int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, 
     B2_REQUIRE(ctx && q_dev && kv_pool_dev && block_tables_dev && cu_seqlens_host && ctx_lens_host && out_dev, B2_ERR_MSG, "b2_paged_attn_prefill_q4: null argument");
     B2_CHECK(b2_kv_q4_check("b2_paged_attn_prefill_q4", kv_pool_dev, n_pages, hq, hkv, head_dim, page_size));
     B2_REQUIRE(num_seqs >= 0 && max_blocks > 0, B2_ERR_MSG, "b2_paged_attn_prefill_q4: bad sizes");
+    B2_REQUIRE(scale > 0.f && scale < INFINITY, B2_ERR_MSG, "b2_paged_attn_prefill_q4: the scale must be positive");
     B2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & 15) == 0, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: q and out must be 16-byte aligned");
     if (num_seqs == 0) return B2_OK;
     std::vector<Q4Seq> seqs;
@@ -255,7 +638,6 @@ extern "C" int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, 
     B2_CUDA(cudaMemcpyAsync(dev, plan.host.data(), plan.host.size() * 4, cudaMemcpyHostToDevice, ctx->stream));
     Q4PrefillParams p{};
     p.q = q_dev;
-    p.q_rows = cu_seqlens_host[num_seqs];
     p.pool = kv_pool_dev;
     p.n_pages = n_pages;
     p.block_tables = block_tables_dev;

@@ -38,12 +38,12 @@ def append(K, ctx=CTX, qkv=AT, T=1, hq=4, hkv=2, hd=128, pos=AT, slots=AT, page=
     K.rope_kv_append_q4(ctx, qkv, T, hq, hkv, hd, pos, slots, AT, AT, None, None, 1e-6, page, pool, pages, q_out, k_out)
 
 
-def decode(K, q=AT, pool=AT, pages=4, tables=AT, n=1, hq=4, hkv=2, hd=128, page=16, out=AT, blocks=4):
-    K.paged_attn_decode_q4(CTX, q, pool, pages, tables, AT, n, hq, hkv, hd, page, 0.1, out, blocks)
+def decode(K, q=AT, pool=AT, pages=4, tables=AT, n=1, hq=4, hkv=2, hd=128, page=16, out=AT, blocks=4, scale=0.1):
+    K.paged_attn_decode_q4(CTX, q, pool, pages, tables, AT, n, hq, hkv, hd, page, scale, out, blocks)
 
 
-def prefill(K, q=AT, pool=AT, pages=4, blocks=4, cu=(0, 1), ctx=(1,), hq=4, hkv=2, hd=128, page=16, out=AT):
-    K.paged_attn_prefill_q4(CTX, q, pool, pages, AT, blocks, cu, ctx, hq, hkv, hd, page, 0.1, out)
+def prefill(K, q=AT, pool=AT, pages=4, blocks=4, cu=(0, 1), ctx=(1,), hq=4, hkv=2, hd=128, page=16, out=AT, scale=0.1):
+    K.paged_attn_prefill_q4(CTX, q, pool, pages, AT, blocks, cu, ctx, hq, hkv, hd, page, scale, out)
 
 
 @pytest.mark.parametrize("call", [append, decode, prefill])
@@ -60,6 +60,7 @@ def test_pool_and_heads(kernels, call, bad, code):
     (append, dict(q_out=AT + 2), -5), (append, dict(k_out=AT + 2), -5), (append, dict(T=1 << 29), -5),
     (decode, dict(q=None), -7), (decode, dict(tables=None), -7), (decode, dict(n=-1), -7), (decode, dict(blocks=0), -7), (decode, dict(q=AT + 2), -5),
     (decode, dict(out=AT + 4), -5), (decode, dict(n=1 << 20, blocks=1 << 12), -5),
+    (decode, dict(scale=0.0), -7), (decode, dict(scale=float("nan")), -7), (prefill, dict(scale=-1.0), -7), (prefill, dict(scale=float("inf")), -7),
     (prefill, dict(q=None), -7), (prefill, dict(cu=(0, 2)), -7), (prefill, dict(cu=(3, 1), ctx=(9,)), -7), (prefill, dict(cu=(-1, 1), ctx=(9,)), -7),
     (prefill, dict(ctx=(65,)), -7), (prefill, dict(out=AT + 8), -5),
 ])
