@@ -171,8 +171,7 @@ int32_t b2_paged_attn_decode_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_
                                 int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size, float scale,
                                 uint16_t* out_dev);
 /* b2_paged_attn_prefill over such a pool: any number of query tokens per sequence, causal as there.  A query that does not see a
- * token is not touched by it, whatever it holds.  Sequences with many query
- * tokens are widened to bf16 in a workspace of the context (up to 1 GiB, or what the longest sequence needs). */
+ * token is not touched by it, whatever it holds. */
 int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_t* kv_pool_dev, int32_t n_pages,
                                  const int32_t* block_tables_dev, int32_t max_blocks, const int32_t* cu_seqlens_host,
                                  const int32_t* ctx_lens_host, int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim,

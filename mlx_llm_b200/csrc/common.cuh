@@ -65,8 +65,6 @@ struct b2_ctx {
     size_t attn_counters_cap = 0;
     int* tile_counters = nullptr;  // per row-tile arrival counters of the split-K streaming kernel (self-resetting)
     float* q4_parts = nullptr;     // attention over a 4-bit cache: parts of units that blocks share, and the blocks' arrival counters
-    uint8_t* q4_wide = nullptr;    // ... with many query tokens: its keys and values in bf16
-    size_t q4_wide_bytes = 0;
     bool use_tc = true;
     bool pdl_consumers = true;     // norm / SwiGLU / RoPE / attention / split-K sums launched with programmatic stream serialisation
     int pdl_min_tokens = 1;        // ... by the engine on iterations of at least this many tokens (B2_PDL_MIN_TOKENS at context creation)

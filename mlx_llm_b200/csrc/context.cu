@@ -76,7 +76,6 @@ int32_t b2_ctx_free(b2_ctx* ctx) {
     if (ctx->tile_counters) cudaFree(ctx->tile_counters);
     if (ctx->attn_counters) cudaFree(ctx->attn_counters);
     if (ctx->q4_parts) cudaFree(ctx->q4_parts);
-    if (ctx->q4_wide) cudaFree(ctx->q4_wide);
     for (auto e : ctx->prof_ev) cudaEventDestroy(e);
     cudaEventDestroy(ctx->ev0);
     cudaEventDestroy(ctx->ev1);

@@ -244,15 +244,12 @@ int32_t b2_kv_q4_attn_launch(b2_ctx* ctx, const Q4AttnParams& p, int head_dim);
 struct Q4Seq {
     int32_t bt_row, q_row, q_len, ctx;  // block-table row, first query row, query tokens (the last ones of the context), tokens in the cache
 };
-struct Q4Pass {  // sequences whose keys and values are widened to bf16 together
-    int seqs, work, longest;  // work items, and the tiles of 128 keys that the longest sees
-    int64_t tiles;            // of all sequences
-    size_t list;              // in the plan: [seqs] block-table row, context, first tile, query row, query tokens; [work] sequence, first query token
-};
 struct Q4Plan {
     std::vector<int32_t> host;
-    int few = 0;          // sequences that kv_q4_attn.cu takes: [few] of each of Q4Seq's numbers, from host[0] on
-    std::vector<Q4Pass> passes;
+    int few = 0;   // sequences that kv_q4_attn.cu takes: [few] of each of Q4Seq's numbers, from host[0] on
+    int many = 0;  // the others: [many] of each, from host[list] on, then [work] items' sequences and first query tokens
+    int work = 0, longest = 0;  // work items, and the tiles of 128 keys that the longest sees
+    size_t list = 0;
 };
 struct Q4PrefillParams {
     const uint16_t* q;

@@ -1,10 +1,8 @@
 // Attention over a 4-bit paged cache for any number of query tokens per sequence: prompts, portions of prompts, drafts.
 //
 // Few columns (query tokens x q heads of a group) go through kv_q4_attn.cu, which reads the 4 bits once per 8 columns.  With many, the
-// products decide, not the bytes, and a code is converted once for all that multiply with it: kv_q4_widen_kernel turns the records of a
-// sequence into bf16 tiles of 128 keys in a workspace, already in the shape that the tensor cores read from shared memory, and
-// kv_q4_prefill_kernel (tcgen05) multiplies from there.  The workspace takes whole sequences, up to kPassBytes at a time (a longer
-// sequence alone).
+// products decide, not the bytes: kv_q4_prefill_kernel (tcgen05) converts the codes of a tile of 128 keys into the bf16 operands that the
+// tensor cores read from shared memory, once for 256 rows of queries.
 #include <algorithm>
 
 #include "kernels.h"
@@ -15,7 +13,6 @@ namespace {
 
 using namespace tc5;
 
-constexpr size_t kPassBytes = 1ull << 30;
 constexpr int kFewColumns = 32;
 constexpr int KT = 128;  // keys of a tile
 
@@ -29,98 +26,24 @@ __device__ __forceinline__ uint32_t tile_at(int row, int dim) {  // of 8 dims
     return (uint32_t)(dim >> 6) * (KT * 128) + (uint32_t)row * 128u + ((((uint32_t)dim >> 3) & 7u) ^ ((uint32_t)row & 7u)) * 16u;
 }
 
-struct WidenParams {
-    const uint8_t* pool;
-    int64_t n_pages;
-    const int32_t* block_tables;
-    int max_blocks, hkv, page_tiles;
-    const int32_t *rows, *ctx, *first;  // [seqs] block-table row, context, first tile
-    int seqs;
-    int64_t tiles;
-    uint8_t* wide;  // [tiles][hkv][K, V][tile]
-};
-
-// One warp per record.  Bound by its writes, four times what it reads; they stay in L2 for the attention behind it where they fit.
-// Tokens behind the context, and pages outside of the pool, become zeros.  A value that is NaN must reach the rows that see it and no others,
-// but a row that does not still multiplies it, with zero: it goes into the token's keys, whose scores are masked by choice and not by
-// multiplication, and the value becomes zero.
-template <int HD>
-__global__ void __launch_bounds__(256) kv_q4_widen_kernel(const WidenParams p) {
-    using Rec = q4::Record<HD>;
-    constexpr int W = HD / 32;
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    pdl_wait();
-    // a block has a tile of one head, a warp one of its eight records
-    const int tile = blockIdx.x / p.hkv, kvh = blockIdx.x - tile * p.hkv;
-    const int sub = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    int lo = 0, hi = p.seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.first[mid] <= tile)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    const int t = (tile - p.first[lo]) * 8 + sub, left = p.ctx[lo] - t * 16;  // tokens of this record that belong to the context
-    const int index = t / p.page_tiles;
-    int page = -1;
-    if (left > 0) page = p.block_tables[(size_t)p.rows[lo] * p.max_blocks + index];
-    const bool there = page >= 0 && page < p.n_pages;
-    const uint8_t* rec = p.pool + (((size_t)(there ? page : 0) * p.hkv + kvh) * p.page_tiles + (there ? t - index * p.page_tiles : 0)) * Rec::kBytes;
-    uint8_t* const k = p.wide + (size_t)blockIdx.x * 2 * tile_bytes<HD>();
-    uint8_t* const v = k + tile_bytes<HD>();
-    auto wide = [](uint32_t x) { return mul_bf2(x, 0x5f805f80u); };  // times 2^64
-#pragma unroll
-    for (int half = 0; half < 2; half++) {
-        {  // K: token g + 8 half, dims c HD/4 ...
-            const int tok = g + 8 * half;
-            const bool ok = there && tok < left;
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < Rec::kGroups; i++) bad |= q4::poisoned(reinterpret_cast<const uint32_t*>(rec + Rec::kVsb)[i * 16 + tok]);
-            const q4::Scales q = q4::scales_twice(bad ? 0x7fc07fc0u : reinterpret_cast<const uint32_t*>(rec + Rec::kKsb)[(c * (HD / 4) / 64) * 16 + tok]);
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(rec) + (half * 32 + lane) * W;
-#pragma unroll
-            for (int w = 0; w < W; w++) {
-                uint32_t x[4];
-                q4::values(src[w], q, x);  // (0,4) (1,5) (2,6) (3,7)
-                const uint4 r = make_uint4(wide(prmt(x[0], x[1], 0x5410u)), wide(prmt(x[2], x[3], 0x5410u)), wide(prmt(x[0], x[1], 0x7632u)), wide(prmt(x[2], x[3], 0x7632u)));
-                *reinterpret_cast<uint4*>(k + tile_at(sub * 16 + tok, c * (HD / 4) + 8 * w)) = ok ? r : make_uint4(0, 0, 0, 0);
-            }
-        }
-        {  // V: tokens 8 half + 2c and the next, dims g HD/8 ...
-            const int tok = 8 * half + 2 * c;
-            const uint2 sb = *reinterpret_cast<const uint2*>(rec + Rec::kVsb + ((g * (HD / 8) / 64) * 16 + tok) * 4);
-            const q4::Scales q = q4::scales_pair(sb.x, sb.y);
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(rec + Rec::kV) + (half * 32 + lane) * W;
-            const bool ok0 = there && tok < left && !q4::poisoned(sb.x), ok1 = there && tok + 1 < left && !q4::poisoned(sb.y);
-#pragma unroll
-            for (int w = 0; w < W; w += 2) {
-                uint32_t x[4], y[4];
-                q4::values(src[w], q, x);  // dim i of both tokens
-                q4::values(src[w + 1], q, y);
-                const uint4 a = make_uint4(wide(prmt(x[0], x[1], 0x5410u)), wide(prmt(x[2], x[3], 0x5410u)), wide(prmt(y[0], y[1], 0x5410u)), wide(prmt(y[2], y[3], 0x5410u)));
-                const uint4 b = make_uint4(wide(prmt(x[0], x[1], 0x7632u)), wide(prmt(x[2], x[3], 0x7632u)), wide(prmt(y[0], y[1], 0x7632u)), wide(prmt(y[2], y[3], 0x7632u)));
-                *reinterpret_cast<uint4*>(v + tile_at(sub * 16 + tok, g * (HD / 8) + 4 * w)) = ok0 ? a : make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(v + tile_at(sub * 16 + tok + 1, g * (HD / 8) + 4 * w)) = ok1 ? b : make_uint4(0, 0, 0, 0);
-            }
-        }
-    }
-}
-
-// ---- the products ------------------------------------------------------------------------------------------------------
 // CTA = (two blocks of query rows, kv head[, split of the keys]).  A row is a (query token, q head of the group) pair, the heads of a token
 // next to one another, so that a group shares every tile of K and V, and the two blocks of 128 rows share them again.
-//   warps 0-3, 4-7  softmax of block A, B: thread = row = TMEM lane.  Reads its 128 scores once; exp2 against a running reference that is
-//                   raised only when a tile exceeds it by more than 2^8 (O is touched only then); P goes as bf16 over the scores' columns.
-//   warp 8          copies tiles, whole (32 or 16 KB each), into a ring of five
-//   warp 9          one thread issues S = Q K^T and O += P V with P from tensor memory, for A and B in turn: while one block's softmax runs,
+//   warps 0-3, 4-7  softmax of block A, B: thread = row = TMEM lane.  exp2 against a running reference that is raised only when a tile exceeds
+//                   it by more than 2^8 (O is touched only then); P goes as bf16 over the scores' columns.
+//   warps 8-11      codes to operands: a warp has two of the eight records of a tile, reads the next tile's while it converts this one's, and
+//                   fills a ring of five tiles K0 V0 K1 V1 ...  K keeps the order that nibbles come out in, 0 4 1 5 2 6 3 7 of eight dims, and Q is
+//                   put in the same; both carry the conversion's 2^-64 (kv_q4.cuh), which the softmax scale and the division take back.
+//   warp 12         one thread issues S = Q K^T and O += P V with P from tensor memory, for A and B in turn: while one block's softmax runs,
 //                   the tensor cores have the other's products.  S(j + 1) of a block goes over P(j), which the in-order pipe has read by then;
 //                   and when S(j) is there, P V of j - 1 has completed, so O may be rescaled.
-// Bound by the tensor cores: 4 x 128 x 128 x HD multiply-adds per pair of blocks and tile.  P carries 8 bits (one rounding of each weight,
-// relative 2^-9; their sum is taken before the rounding, whose errors have no sign of their own): a second product for the rest of P
-// would cost half as much again.
-constexpr int kRows = 128, kSlots = 5, kThreads = 320;
+// Bound by a block's chain of product, softmax, product (two thirds of it are the tensor cores').  Converting in here costs each CTA what an
+// own kernel would do once per 128 keys, in warps that the chain leaves idle: 512 tokens behind 11800 that read bf16 tiles, made by such a
+// kernel, from L2 took 210 us, with the tensor cores waiting for copies a seventh of the time.
+// A value that is NaN must reach the rows that see it and no others, but a row that does not still multiplies it, with zero: it goes into the
+// token's keys, whose scores are masked by choice and not by multiplication, and the value becomes zero.
+// P carries 8 bits (one rounding of each weight, relative 2^-9; their sum is taken before the rounding, whose errors have no sign of their
+// own): a second product for the rest of P would cost half as much again.
+constexpr int kRows = 128, kSlots = 5, kConvert = 8, kIssuer = 12, kThreads = 416;
 constexpr float kRaise = 8.f, kFloor = -1e30f;
 template <int HD>
 struct Smem {
@@ -134,14 +57,17 @@ constexpr uint32_t idesc_pv() {  // N = HD, B MN-major
 
 struct ProductParams {
     const uint16_t* q;
-    const uint8_t* wide;
-    const int32_t *q_row, *q_len, *ctx, *first;  // [seqs]
-    const int32_t *work_seq, *work_q;            // [items] sequence, first query token
-    int hq, hkv, group, per_block;               // query tokens of a block of rows
-    float scale_log2;
+    const uint8_t* pool;
+    int64_t n_pages;
+    const int32_t* block_tables;
+    int max_blocks, page_tiles;
+    const int32_t *bt_row, *q_row, *q_len, *ctx;  // [seqs]
+    const int32_t *work_seq, *work_q;             // [items] sequence, first query token
+    int hq, hkv, group, per_block;                // query tokens of a block of rows
+    float scale_log2;                             // times 2^64
     uint16_t* out;
     int splits;
-    float* part_o;   // [item][kv head][split][256 rows][HD], unnormalised
+    float* part_o;   // [item][kv head][split][256 rows][HD], unnormalised, times 2^-64
     float* part_ml;  // [item][kv head][split][256 rows][2]: reference (log2 domain), sum
     int* err;
 };
@@ -174,7 +100,112 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint64_t two(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
 __device__ __forceinline__ uint64_t twice(float x) { return two(__float_as_uint(x), __float_as_uint(x)); }
 __device__ __forceinline__ float low(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float high(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+
+// What a lane has of a record's keys, or values: the words of tokens g and g + 8 (or of the pairs c and c + 4), and their scales.
+template <int HD>
+struct Words {
+    uint32_t w[2][HD / 32], sb[2][2];
+};
+// The two records of a converting warp in tile t, and how many tokens of each belong to the context.
+template <int HD>
+struct Source {
+    const uint8_t* rec[2];
+    int left[2];
+    __device__ __forceinline__ void find(const ProductParams& p, const Item& w, int kvh, int t, int warp) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = t * 8 + warp * 2 + i;
+            left[i] = w.ctx - r * 16;
+            rec[i] = p.pool;
+            if (left[i] <= 0) continue;
+            const int index = r / p.page_tiles, page = p.block_tables[(size_t)p.bt_row[w.seq] * p.max_blocks + index];
+            if (page < 0 || page >= p.n_pages)
+                left[i] = 0;  // nothing there: zeros
+            else
+                rec[i] += (((size_t)page * p.hkv + kvh) * p.page_tiles + r - index * p.page_tiles) * q4::Record<HD>::kBytes;
+        }
+    }
+    __device__ __forceinline__ void read(Words<HD> (&x)[2], bool values, int lane) const {
+        using Rec = q4::Record<HD>;
+        const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (left[i] <= 0) {
+                x[i] = Words<HD>{};
+                continue;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint8_t* at = rec[i] + (values ? Rec::kV : 0) + h * 4 * HD;
+                if constexpr (HD == 128) {
+                    const uint4 v = reinterpret_cast<const uint4*>(at)[lane];
+                    x[i].w[h][0] = v.x, x[i].w[h][1] = v.y, x[i].w[h][2] = v.z, x[i].w[h][3] = v.w;
+                } else {
+                    const uint2 v = reinterpret_cast<const uint2*>(at)[lane];
+                    x[i].w[h][0] = v.x, x[i].w[h][1] = v.y;
+                }
+                if (values) {  // tokens 8 h + 2 c and the next
+                    const uint2 sb = *reinterpret_cast<const uint2*>(rec[i] + Rec::kVsb + ((g * (HD / 8) / 64) * 16 + 8 * h + 2 * c) * 4);
+                    x[i].sb[h][0] = 8 * h + 2 * c < left[i] ? sb.x : 0u;  // behind the context: zeros
+                    x[i].sb[h][1] = 8 * h + 2 * c + 1 < left[i] ? sb.y : 0u;
+                } else {       // token 8 h + g
+                    const int t = 8 * h + g;
+                    x[i].sb[h][0] = reinterpret_cast<const uint32_t*>(rec[i] + Rec::kKsb)[(c * (HD / 4) / 64) * 16 + t];
+                    x[i].sb[h][1] = 0;
+#pragma unroll
+                    for (int k = 0; k < Rec::kGroups; k++)
+                        if (q4::poisoned(reinterpret_cast<const uint32_t*>(rec[i] + Rec::kVsb)[k * 16 + t])) x[i].sb[h][0] = 0x7fc07fc0u;
+                    if (t >= left[i]) x[i].sb[h][0] = 0;
+                }
+            }
+        }
+    }
+};
+template <int HD>
+__device__ __forceinline__ void put_keys(uint8_t* tile, int row0, const Words<HD> (&x)[2], int lane) {
+    const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const q4::Scales q = q4::scales_twice(x[i].sb[h][0]);
+#pragma unroll
+            for (int w = 0; w < HD / 32; w++) {
+                uint32_t v[4];
+                q4::values(x[i].w[h][w], q, v);
+                *reinterpret_cast<uint4*>(tile + tile_at(row0 + 16 * i + 8 * h + g, c * (HD / 4) + 8 * w)) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+        }
+}
+template <int HD>
+__device__ __forceinline__ void put_values(uint8_t* tile, int row0, const Words<HD> (&x)[2], int lane) {
+    const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t sb0 = q4::poisoned(x[i].sb[h][0]) ? 0u : x[i].sb[h][0], sb1 = q4::poisoned(x[i].sb[h][1]) ? 0u : x[i].sb[h][1];
+            const q4::Scales q = q4::scales_pair(sb0, sb1);
+            const int row = row0 + 16 * i + 8 * h + 2 * c;
+#pragma unroll
+            for (int w = 0; w < HD / 32; w += 2) {
+                uint32_t a[4], b[4];
+                q4::values(x[i].w[h][w], q, a);  // dim k of both tokens
+                q4::values(x[i].w[h][w + 1], q, b);
+                const int d = g * (HD / 8) + 4 * w;
+                *reinterpret_cast<uint4*>(tile + tile_at(row, d)) =
+                    make_uint4(prmt(a[0], a[1], 0x5410u), prmt(a[2], a[3], 0x5410u), prmt(b[0], b[1], 0x5410u), prmt(b[2], b[3], 0x5410u));
+                *reinterpret_cast<uint4*>(tile + tile_at(row + 1, d)) =
+                    make_uint4(prmt(a[0], a[1], 0x7632u), prmt(a[2], a[3], 0x7632u), prmt(b[0], b[1], 0x7632u), prmt(b[2], b[3], 0x7632u));
+            }
+        }
+}
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const ProductParams p) {
@@ -200,12 +231,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
     const uint32_t o_ready = bar + 8u * 15, slot_addr = bar + 8u * 16;
     if (tid == 0) {
         mbar_init(q_full, 8);
-        for (int s = 0; s < kSlots; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+        for (int s = 0; s < kSlots; s++) mbar_init(full(s), 4), mbar_init(empty(s), 1);
         for (int x = 0; x < 2; x++) mbar_init(s_ready(x), 1), mbar_init(p_ready(x), 4);
         mbar_init(o_ready, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == kIssuer) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(slot_addr), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
@@ -216,47 +247,57 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
     const int n = w.n_tiles;
     bool alive = true;
 
-    if (warp == 8) {
-        if (lane == 0) {
-            const uint8_t* src = p.wide + ((size_t)(p.first[w.seq] + w.first_tile) * p.hkv + kvh) * 2 * TILE;
-            const size_t step = (size_t)p.hkv * 2 * TILE;
-            int slot = 0, asked = 0;
-            uint32_t parity = 0;  // of the slot's present use
-            for (int i = 0; i < 2 * n; i++) {  // K0 V0 K1 V1 ...
-                if (!mbar_wait(empty(slot), parity ^ 1u)) {
-                    alive = false;
-                    break;
-                }
-                mbar_expect_tx(full(slot), TILE);
-                bulk_load(base + S::kRing + slot * TILE, src + (i >> 1) * step + (i & 1) * TILE, TILE, full(slot));
-                asked++;
-                if (++slot == kSlots) slot = 0, parity ^= 1u;
-            }
-            if (!alive) {  // nothing may be on its way when the block ends
-                atomicExch(p.err, 2);
-                for (int i = max(0, asked - kSlots); i < asked; i++) mbar_wait(full(i % kSlots), (uint32_t)(i / kSlots) & 1u);
-            }
+    if (warp >= kConvert && warp < kIssuer) {
+        const int row0 = (warp - kConvert) * 32;
+        Source<HD> from;
+        Words<HD> keys[2], vals[2];
+        from.find(p, w, kvh, w.first_tile, warp - kConvert);
+        from.read(keys, false, lane);
+        from.read(vals, true, lane);
+        int slot = 0;
+        uint32_t parity = 0;  // of the slot's present use
+        auto fill = [&](auto put) {
+            alive = __all_sync(0xffffffffu, mbar_wait(empty(slot), parity ^ 1u));
+            if (!alive) return;
+            put(smem + S::kRing + slot * TILE);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full(slot));
+            if (++slot == kSlots) slot = 0, parity ^= 1u;
+        };
+        for (int j = 0; j < n && alive; j++) {
+            if (j + 1 < n) from.find(p, w, kvh, w.first_tile + j + 1, warp - kConvert);
+            fill([&](uint8_t* tile) { put_keys<HD>(tile, row0, keys, lane); });
+            if (!alive) break;
+            if (j + 1 < n) from.read(keys, false, lane);
+            fill([&](uint8_t* tile) { put_values<HD>(tile, row0, vals, lane); });
+            if (j + 1 < n) from.read(vals, true, lane);
         }
-        __syncwarp();
-    } else if (warp == 9) {
+        if (!alive && lane == 0) atomicExch(p.err, 2);
+    } else if (warp == kIssuer) {
         if (lane == 0) {
+            // This thread's instructions per step set how soon the next products are queued, so descriptors are made once: the address is
+            // the low word's (no carry leaves it), and all offsets but the ring's slot are constants.
+            const uint64_t dq = desc_kmajor(base + S::kQ), dk = desc_kmajor(base + S::kRing), dv = desc_mnmajor(base + S::kRing, HALF);
+            const uint32_t q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, v_lo = (uint32_t)dv, k_hi = (uint32_t)(dk >> 32), v_hi = (uint32_t)(dv >> 32);
             auto issue_s = [&](int x, int slot) {  // S of block x
+                const uint32_t at = k_lo + slot * (TILE >> 4);
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++) {
-                    const uint32_t off = (uint32_t)(k >> 2) * HALF + (uint32_t)(k & 3) * 32u;
-                    tc_mma(tmem + x * 128u, desc_kmajor(base + S::kQ + x * TILE + off), desc_kmajor(base + S::kRing + slot * TILE + off), kIdesc128, k > 0 ? 1u : 0u);
+                    const uint32_t off = ((k >> 2) * HALF + (k & 3) * 32) >> 4;
+                    tc_mma(tmem + x * 128u, two(q_lo + x * (TILE >> 4) + off, k_hi), two(at + off, k_hi), kIdesc128, k > 0 ? 1u : 0u);
                 }
                 tc_commit(s_ready(x));
             };
-            auto issue_o = [&](int x, int slot, bool add) {  // O of block x
+            auto issue_o = [&](int x, int slot, uint32_t add) {  // O of block x
+                const uint32_t at = v_lo + slot * (TILE >> 4);
 #pragma unroll
                 for (int k = 0; k < KT / 16; k++)
-                    tc_mma_ts(tmem + 256u + x * 128u, tmem + x * 128u + k * 8u, desc_mnmajor(base + S::kRing + slot * TILE + k * 2048u, HALF), idesc_pv<HD>(),
-                              add || k > 0 ? 1u : 0u);
+                    tc_mma_ts(tmem + 256u + x * 128u, tmem + x * 128u + k * 8u, two(at + k * (2048 >> 4), v_hi), idesc_pv<HD>(), k > 0 ? 1u : add);
             };
             int slot = 0;
             uint32_t parity = 0;
-            auto advance = [&] {
+            auto advance = [&] {  // along the ring: K0 V0 K1 V1 ...
                 if (++slot == kSlots) slot = 0, parity ^= 1u;
             };
             alive = mbar_wait(q_full, 0) && mbar_wait(full(0), 0);
@@ -312,7 +353,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
 #pragma unroll
             for (int i = 0; i < HD / 8; i++) v[i] = row_ok ? src[i] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < HD / 8; i++) *reinterpret_cast<uint4*>(dst + tile_at(r, 8 * i)) = v[i];
+            for (int i = 0; i < HD / 8; i++)
+                *reinterpret_cast<uint4*>(dst + tile_at(r, 8 * i)) =
+                    make_uint4(prmt(v[i].x, v[i].z, 0x5410u), prmt(v[i].x, v[i].z, 0x7632u), prmt(v[i].y, v[i].w, 0x5410u), prmt(v[i].y, v[i].w, 0x7632u));
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
@@ -327,28 +370,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
                 break;
             }
             tc_fence_after();
-            uint32_t s[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; c++) tc_ld32_nowait(ts + c * 32u, s[c]);
-            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+            // The upper 64 scores are read for the maximum and, once the lower ones have become P, again: a thread has 128 registers.
             const int key0 = (w.first_tile + j) * KT;
-            if (key0 + KT - 1 > sees) {
+            const bool masked = key0 + KT - 1 > sees;
+            uint32_t s[2][32];
+            auto read = [&](int half) {
 #pragma unroll
-                for (int c = 0; c < 4; c++)
+                for (int c = 0; c < 2; c++) tc_ld32_nowait(ts + half * 64u + c * 32u, s[c]);
+                asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+                if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (key0 + c * 32 + i > sees) s[c][i] = 0xff800000u;
-            }
+                    for (int i = 0; i < 64; i++)
+                        if (key0 + half * 64 + i > sees) s[i >> 5][i & 31] = 0xff800000u;
+                }
+            };
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 32; i++)
+            for (int half = 1; half >= 0; half--) {
+                read(half);
 #pragma unroll
-                for (int c = 0; c < 4; c++) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;  // (the scale is positive)
+                for (int i = 0; i < 32; i += 4)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        mx[c] = max3(mx[c], __uint_as_float(s[c >> 1][i + 2 * (c & 1)]), __uint_as_float(s[c >> 1][i + 2 * (c & 1) + 1]));
+            }
+            const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;  // (the scale is positive)
             float alpha = 1.f;
             if (j == 0) {
-                m = fmaxf(top, kFloor);
-            } else if (top > m + kRaise) {
+                m = top < kFloor ? kFloor : top;
+            } else if (!(top <= m + kRaise)) {  // (a NaN too, which makes all of the row NaN)
                 alpha = fast_exp2(m - top);
                 m = top;
             }
@@ -366,16 +416,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
             const uint64_t sc = twice(p.scale_log2), neg = twice(-m);
             uint64_t sum[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t h[16];
+            for (int half = 0; half < 2; half++) {
+                if (half == 1) read(1);
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const uint64_t e = fma2(two(s[c][2 * i], s[c][2 * i + 1]), sc, neg);
-                    const float a = fast_exp2(low(e)), b = fast_exp2(high(e));
-                    sum[i & 1] = add2(sum[i & 1], two(__float_as_uint(a), __float_as_uint(b)));
-                    h[i] = pack_bf2(a, b);
+                for (int c = 0; c < 2; c++) {
+                    uint32_t h[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const uint64_t e = fma2(two(s[c][2 * i], s[c][2 * i + 1]), sc, neg);
+                        const float a = fast_exp2(low(e)), b = fast_exp2(high(e));
+                        sum[i & 1] = add2(sum[i & 1], two(__float_as_uint(a), __float_as_uint(b)));
+                        h[i] = pack_bf2(a, b);
+                    }
+                    tc_st16_nowait(ts + (half * 2 + c) * 16u, h);
                 }
-                tc_st16_nowait(ts + c * 16u, h);
             }
             const uint64_t both = add2(sum[0], sum[1]);
             l += low(both) + high(both);
@@ -388,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
         if (alive) {
             tc_fence_after();
             const bool part = p.splits > 1;
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            const float inv = l == 0.f ? 0.f : q4::kUnscale / l;
             const size_t at = (((size_t)blockIdx.y * p.hkv + kvh) * p.splits + blockIdx.z) * (2 * kRows) + x * kRows + r;
 #pragma unroll 1
             for (int c = 0; c < HD / 32; c++) {
@@ -415,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == kIssuer) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // Sum of the splits of an item, in their order: a warp per row, HD / 32 dims a lane.
@@ -444,18 +498,18 @@ __global__ void __launch_bounds__(256) kv_q4_prefill_merge_kernel(const ProductP
             o[i] += f * v.x, o[i + 1] += f * v.y;
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = l == 0.f ? 0.f : q4::kUnscale / l;
     uint16_t* dst = p.out + ((size_t)(p.q_row[w.seq] + w.q0 + query) * p.hq + (size_t)kvh * p.group + in_block % p.group) * HD + lane * D;
 #pragma unroll
     for (int i = 0; i < D; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf2(o[i] * inv, o[i + 1] * inv);
 }
 
-int rows_per_block(int group) { return kRows / group; }
-
 }  // namespace
 
 int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int hkv, int head_dim, Q4Plan& plan) {
     (void)ctx;
+    (void)hkv;
+    (void)head_dim;
     plan = Q4Plan{};
     const int group = hq / hkv;
     std::vector<Q4Seq> few, many;
@@ -466,87 +520,55 @@ int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int h
     for (const Q4Seq& s : few) plan.host.push_back(s.q_row);
     for (const Q4Seq& s : few) plan.host.push_back(s.q_len);
     for (const Q4Seq& s : few) plan.host.push_back(s.ctx);
-    const size_t bytes = (size_t)hkv * 2 * KT * head_dim * 2;  // of a tile of keys, all heads
-    const int step = 2 * rows_per_block(std::min(group, kRows));  // query tokens of an item
-    for (size_t from = 0; from < many.size();) {
-        Q4Pass pass{};
-        size_t to = from;
-        for (; to < many.size(); to++) {
-            const int64_t tiles = ((int64_t)many[to].ctx + KT - 1) / KT;
-            if (to > from && (size_t)(pass.tiles + tiles) * bytes > kPassBytes) break;
-            pass.tiles += tiles;
-        }
-        const int n = pass.seqs = (int)(to - from);
-        pass.list = plan.host.size();
-        auto list = [&](auto number) {
-            for (size_t i = from; i < to; i++) plan.host.push_back(number(many[i]));
-        };
-        list([](const Q4Seq& s) { return s.bt_row; });
-        list([](const Q4Seq& s) { return s.ctx; });
-        int32_t tile = 0;
-        list([&](const Q4Seq& s) {
-            const int32_t first = tile;
-            tile += (s.ctx + KT - 1) / KT;
-            return first;
-        });
-        list([](const Q4Seq& s) { return s.q_row; });
-        list([](const Q4Seq& s) { return s.q_len; });
-        // the longest items first, so that the last ones to start are short
-        struct Work {
-            int32_t seq, q, tiles;
-        };
-        std::vector<Work> work;
-        for (int i = 0; i < n; i++) {
-            const Q4Seq& s = many[from + i];
-            for (int q = 0; q < s.q_len; q += step) work.push_back({i, q, (s.ctx - s.q_len + std::min(q + step, s.q_len) - 1) / KT + 1});
-        }
-        std::stable_sort(work.begin(), work.end(), [](const Work& a, const Work& b) { return a.tiles > b.tiles; });
-        pass.work = (int)work.size();
-        pass.longest = work[0].tiles;
-        for (const Work& x : work) plan.host.push_back(x.seq);
-        for (const Work& x : work) plan.host.push_back(x.q);
-        plan.passes.push_back(pass);
-        from = to;
-    }
+    plan.many = (int)many.size();
+    if (many.empty()) return B2_OK;
+    plan.list = plan.host.size();
+    for (const Q4Seq& s : many) plan.host.push_back(s.bt_row);
+    for (const Q4Seq& s : many) plan.host.push_back(s.q_row);
+    for (const Q4Seq& s : many) plan.host.push_back(s.q_len);
+    for (const Q4Seq& s : many) plan.host.push_back(s.ctx);
+    // the longest items first, so that the last ones to start are short
+    struct Work {
+        int32_t seq, q, tiles;
+    };
+    std::vector<Work> work;
+    const int step = 2 * (kRows / group);  // query tokens of an item
+    for (int i = 0; i < plan.many; i++)
+        for (int q = 0; q < many[i].q_len; q += step)
+            work.push_back({i, q, (many[i].ctx - many[i].q_len + std::min(q + step, many[i].q_len) - 1) / KT + 1});
+    std::stable_sort(work.begin(), work.end(), [](const Work& a, const Work& b) { return a.tiles > b.tiles; });
+    plan.work = (int)work.size();
+    plan.longest = work[0].tiles;
+    for (const Work& x : work) plan.host.push_back(x.seq);
+    for (const Work& x : work) plan.host.push_back(x.q);
     return B2_OK;
 }
 
 template <int HD>
-static int32_t launch_pass(b2_ctx* ctx, const Q4PrefillParams& p, const Q4Pass& pass, const int32_t* plan_dev) {
-    WidenParams w{};
-    w.pool = p.pool;
-    w.n_pages = p.n_pages;
-    w.block_tables = p.block_tables;
-    w.max_blocks = p.max_blocks;
-    w.hkv = p.hkv;
-    w.page_tiles = p.page_tiles;
-    w.rows = plan_dev + pass.list;
-    w.ctx = w.rows + pass.seqs;
-    w.first = w.ctx + pass.seqs;
-    w.seqs = pass.seqs;
-    w.tiles = pass.tiles;
-    w.wide = ctx->q4_wide;
-    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_widen_kernel<HD>, dim3((unsigned)(pass.tiles * p.hkv)), dim3(256), 0, ctx->stream, w));
-    B2_LAUNCHED(ctx);
+static int32_t launch_many(b2_ctx* ctx, const Q4PrefillParams& p, const Q4Plan& plan, const int32_t* plan_dev) {
     ProductParams a{};
     a.q = p.q;
-    a.wide = ctx->q4_wide;
-    a.ctx = w.ctx;
-    a.first = w.first;
-    a.q_row = w.first + pass.seqs;
-    a.q_len = a.q_row + pass.seqs;
-    a.work_seq = a.q_len + pass.seqs;
-    a.work_q = a.work_seq + pass.work;
+    a.pool = p.pool;
+    a.n_pages = p.n_pages;
+    a.block_tables = p.block_tables;
+    a.max_blocks = p.max_blocks;
+    a.page_tiles = p.page_tiles;
+    a.bt_row = plan_dev + plan.list;
+    a.q_row = a.bt_row + plan.many;
+    a.q_len = a.q_row + plan.many;
+    a.ctx = a.q_len + plan.many;
+    a.work_seq = a.ctx + plan.many;
+    a.work_q = a.work_seq + plan.work;
     a.hq = p.hq;
     a.hkv = p.hkv;
     a.group = p.hq / p.hkv;
-    a.per_block = rows_per_block(a.group);
-    a.scale_log2 = p.scale_log2;
+    a.per_block = kRows / a.group;
+    a.scale_log2 = p.scale_log2 * q4::kUnscale;
     a.out = p.out;
     a.err = ctx->dev_err;
     // A CTA fills an SM.  Where the items leave half of the SMs idle, the keys are split as well, four tiles a split at least.
-    const int ctas = pass.work * p.hkv;
-    a.splits = ctas * 2 <= ctx->sm_count ? std::max(1, std::min({ctx->sm_count / ctas, pass.longest / 4, 16})) : 1;
+    const int ctas = plan.work * p.hkv;
+    a.splits = ctas * 2 <= ctx->sm_count ? std::max(1, std::min({ctx->sm_count / ctas, plan.longest / 4, 16})) : 1;
     if (a.splits > 1) {
         const size_t slots = (size_t)ctas * a.splits * 2 * kRows, bytes = slots * (HD + 2) * sizeof(float);
         if (bytes > ctx->pf_part_bytes) {
@@ -561,10 +583,10 @@ static int32_t launch_pass(b2_ctx* ctx, const Q4PrefillParams& p, const Q4Pass& 
         a.part_ml = ctx->pf_part + slots * HD;
     }
     B2_SMEM_ONCE(ctx, kv_q4_prefill_kernel<HD>, Smem<HD>::kBytes);
-    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_kernel<HD>, dim3(p.hkv, pass.work, a.splits), dim3(kThreads), (size_t)Smem<HD>::kBytes, ctx->stream, a));
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_kernel<HD>, dim3(p.hkv, plan.work, a.splits), dim3(kThreads), (size_t)Smem<HD>::kBytes, ctx->stream, a));
     B2_LAUNCHED(ctx);
     if (a.splits > 1) {
-        B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_merge_kernel<HD>, dim3(p.hkv, pass.work, 2 * kRows / 8), dim3(256), 0, ctx->stream, a));
+        B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_merge_kernel<HD>, dim3(p.hkv, plan.work, 2 * kRows / 8), dim3(256), 0, ctx->stream, a));
         B2_LAUNCHED(ctx);
     }
     B2_CUDA(cudaGetLastError());
@@ -591,21 +613,9 @@ int32_t b2_kv_q4_prefill_launch(b2_ctx* ctx, const Q4PrefillParams& p, int head_
         a.out = p.out;
         B2_CHECK(b2_kv_q4_attn_launch(ctx, a, head_dim));
     }
-    size_t need = 0;
-    for (const Q4Pass& pass : plan.passes) {
-        B2_REQUIRE(pass.tiles * p.hkv < (1ll << 31) && pass.work <= 65535, B2_ERR_UNSUPPORTED, "attention over a 4-bit cache: too many query tokens or too long a context for one call");
-        need = std::max(need, (size_t)pass.tiles * p.hkv * 2 * KT * head_dim * 2);
-    }
-    if (need > ctx->q4_wide_bytes) {
-        B2_CUDA(cudaStreamSynchronize(ctx->stream));
-        if (ctx->q4_wide) B2_CUDA(cudaFree(ctx->q4_wide));
-        ctx->q4_wide = nullptr;
-        ctx->q4_wide_bytes = 0;
-        B2_CUDA(cudaMalloc((void**)&ctx->q4_wide, need + (need >> 2)));
-        ctx->q4_wide_bytes = need + (need >> 2);
-    }
-    for (const Q4Pass& pass : plan.passes) B2_CHECK(head_dim == 128 ? launch_pass<128>(ctx, p, pass, plan_dev) : launch_pass<64>(ctx, p, pass, plan_dev));
-    return B2_OK;
+    if (plan.many == 0) return B2_OK;
+    B2_REQUIRE(plan.work <= 65535, B2_ERR_UNSUPPORTED, "attention over a 4-bit cache: too many query tokens for one call");
+    return head_dim == 128 ? launch_many<128>(ctx, p, plan, plan_dev) : launch_many<64>(ctx, p, plan, plan_dev);
 }
 
 extern "C" int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_t* kv_pool_dev, int32_t n_pages, const int32_t* block_tables_dev,
