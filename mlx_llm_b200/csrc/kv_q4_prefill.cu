@@ -107,14 +107,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if on
 }
 __device__ __forceinline__ float high(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
 
-// What a lane has of a record's keys, or values: the words of tokens g and g + 8 (or of the pairs c and c + 4), and their scales.
+// What a lane has of two records' keys, or values: the words of tokens g and g + 8 (or of the pairs c and c + 4), their scales, and for keys
+// the scales of the same tokens' values.  Nothing is decided by them before they are used, so that they may still be on their way.
 template <int HD>
 struct Words {
-    uint32_t w[2][HD / 32], sb[2][2];
+    static constexpr int kGroups = HD / 64;
+    uint32_t w[2][2][HD / 32], sb[2][2][2], other[2][2][kGroups];
+    int left[2];  // tokens of the records that belong to the context
 };
-// The two records of a converting warp in tile t, and how many tokens of each belong to the context.
 template <int HD>
-struct Source {
+struct Source {  // the two records of a converting warp in a tile
     const uint8_t* rec[2];
     int left[2];
     __device__ __forceinline__ void find(const ProductParams& p, const Item& w, int kvh, int t, int warp) {
@@ -131,73 +133,78 @@ struct Source {
                 rec[i] += (((size_t)page * p.hkv + kvh) * p.page_tiles + r - index * p.page_tiles) * q4::Record<HD>::kBytes;
         }
     }
-    __device__ __forceinline__ void read(Words<HD> (&x)[2], bool values, int lane) const {
+    __device__ __forceinline__ void read(Words<HD>& x, bool values, int lane) const {
         using Rec = q4::Record<HD>;
         const int g = lane >> 2, c = lane & 3;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            if (left[i] <= 0) {
-                x[i] = Words<HD>{};
-                continue;
-            }
+            x.left[i] = left[i];
+            if (left[i] <= 0) continue;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint8_t* at = rec[i] + (values ? Rec::kV : 0) + h * 4 * HD;
                 if constexpr (HD == 128) {
                     const uint4 v = reinterpret_cast<const uint4*>(at)[lane];
-                    x[i].w[h][0] = v.x, x[i].w[h][1] = v.y, x[i].w[h][2] = v.z, x[i].w[h][3] = v.w;
+                    x.w[i][h][0] = v.x, x.w[i][h][1] = v.y, x.w[i][h][2] = v.z, x.w[i][h][3] = v.w;
                 } else {
                     const uint2 v = reinterpret_cast<const uint2*>(at)[lane];
-                    x[i].w[h][0] = v.x, x[i].w[h][1] = v.y;
+                    x.w[i][h][0] = v.x, x.w[i][h][1] = v.y;
                 }
                 if (values) {  // tokens 8 h + 2 c and the next
                     const uint2 sb = *reinterpret_cast<const uint2*>(rec[i] + Rec::kVsb + ((g * (HD / 8) / 64) * 16 + 8 * h + 2 * c) * 4);
-                    x[i].sb[h][0] = 8 * h + 2 * c < left[i] ? sb.x : 0u;  // behind the context: zeros
-                    x[i].sb[h][1] = 8 * h + 2 * c + 1 < left[i] ? sb.y : 0u;
-                } else {       // token 8 h + g
-                    const int t = 8 * h + g;
-                    x[i].sb[h][0] = reinterpret_cast<const uint32_t*>(rec[i] + Rec::kKsb)[(c * (HD / 4) / 64) * 16 + t];
-                    x[i].sb[h][1] = 0;
+                    x.sb[i][h][0] = sb.x, x.sb[i][h][1] = sb.y;
+                } else {  // token 8 h + g
+                    x.sb[i][h][0] = reinterpret_cast<const uint32_t*>(rec[i] + Rec::kKsb)[(c * (HD / 4) / 64) * 16 + 8 * h + g];
 #pragma unroll
-                    for (int k = 0; k < Rec::kGroups; k++)
-                        if (q4::poisoned(reinterpret_cast<const uint32_t*>(rec[i] + Rec::kVsb)[k * 16 + t])) x[i].sb[h][0] = 0x7fc07fc0u;
-                    if (t >= left[i]) x[i].sb[h][0] = 0;
+                    for (int k = 0; k < Rec::kGroups; k++) x.other[i][h][k] = reinterpret_cast<const uint32_t*>(rec[i] + Rec::kVsb)[k * 16 + 8 * h + g];
                 }
             }
         }
     }
 };
 template <int HD>
-__device__ __forceinline__ void put_keys(uint8_t* tile, int row0, const Words<HD> (&x)[2], int lane) {
+__device__ __forceinline__ void put_keys(uint8_t* tile, int row0, const Words<HD>& x, int lane) {
     const int g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const q4::Scales q = q4::scales_twice(x[i].sb[h][0]);
+            uint32_t sb = x.sb[i][h][0];
 #pragma unroll
-            for (int w = 0; w < HD / 32; w++) {
+            for (int k = 0; k < Words<HD>::kGroups; k++)
+                if (q4::poisoned(x.other[i][h][k])) sb = 0x7fc07fc0u;
+            const bool real = 8 * h + g < x.left[i];
+            const q4::Scales q = q4::scales_twice(real ? sb : 0u);
+#pragma unroll
+            for (int k = 0; k < HD / 32; k++) {
+                // (at head size 128 lanes c and c + 2 have pieces that the swizzle puts into the same banks: the latter take another one first)
+                const int w = HD == 128 ? k ^ (c & 2) : k;
+                const uint32_t word = HD == 128 && (c & 2) ? x.w[i][h][k ^ (HD / 64)] : x.w[i][h][k];
                 uint32_t v[4];
-                q4::values(x[i].w[h][w], q, v);
+                q4::values(real ? word : 0u, q, v);
                 *reinterpret_cast<uint4*>(tile + tile_at(row0 + 16 * i + 8 * h + g, c * (HD / 4) + 8 * w)) = make_uint4(v[0], v[1], v[2], v[3]);
             }
         }
 }
 template <int HD>
-__device__ __forceinline__ void put_values(uint8_t* tile, int row0, const Words<HD> (&x)[2], int lane) {
+__device__ __forceinline__ void put_values(uint8_t* tile, int row0, const Words<HD>& x, int lane) {
     const int g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const uint32_t sb0 = q4::poisoned(x[i].sb[h][0]) ? 0u : x[i].sb[h][0], sb1 = q4::poisoned(x[i].sb[h][1]) ? 0u : x[i].sb[h][1];
+            const int t = 8 * h + 2 * c;
+            const uint32_t sb0 = t >= x.left[i] || q4::poisoned(x.sb[i][h][0]) ? 0u : x.sb[i][h][0];
+            const uint32_t sb1 = t + 1 >= x.left[i] || q4::poisoned(x.sb[i][h][1]) ? 0u : x.sb[i][h][1];
             const q4::Scales q = q4::scales_pair(sb0, sb1);
-            const int row = row0 + 16 * i + 8 * h + 2 * c;
+            const int row = row0 + 16 * i + t;
 #pragma unroll
-            for (int w = 0; w < HD / 32; w += 2) {
+            for (int k = 0; k < HD / 32; k += 2) {
+                const bool other = HD == 128 && (g & 1);  // (as above, lanes g and g + 1)
+                const int w = other ? k ^ 2 : k;
                 uint32_t a[4], b[4];
-                q4::values(x[i].w[h][w], q, a);  // dim k of both tokens
-                q4::values(x[i].w[h][w + 1], q, b);
+                q4::values(other ? x.w[i][h][(k ^ 2) % (HD / 32)] : x.w[i][h][k], q, a);  // dim i of both tokens
+                q4::values(other ? x.w[i][h][(k ^ 2) % (HD / 32) + 1] : x.w[i][h][k + 1], q, b);
                 const int d = g * (HD / 8) + 4 * w;
                 *reinterpret_cast<uint4*>(tile + tile_at(row, d)) =
                     make_uint4(prmt(a[0], a[1], 0x5410u), prmt(a[2], a[3], 0x5410u), prmt(b[0], b[1], 0x5410u), prmt(b[2], b[3], 0x5410u));
@@ -250,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
     if (warp >= kConvert && warp < kIssuer) {
         const int row0 = (warp - kConvert) * 32;
         Source<HD> from;
-        Words<HD> keys[2], vals[2];
+        Words<HD> keys, vals;
         from.find(p, w, kvh, w.first_tile, warp - kConvert);
         from.read(keys, false, lane);
         from.read(vals, true, lane);
