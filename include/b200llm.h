@@ -149,8 +149,9 @@ int32_t b2_paged_attn_prefill(b2_ctx* ctx, const uint16_t* q_dev, const uint16_t
  *            half, each the dims g * head_dim / 8 + 4d .. + 3 from the lowest nibble on
  *   K, then V scales and biases: u32 [head_dim / 64][16 tokens], scale in the low half, bias in the high one (both bf16)
  * b2_kv_q4_pool_bytes gives the pool's size; a pool needs no initial contents.  Any hq / hkv that is whole, head_dim 64 or 128,
- * page_size a multiple of 16, a positive softmax scale, pool and bf16 arrays 16-byte aligned.  A block table may name pages in any order; a page number outside of
- * 0 .. n_pages - 1 reads nothing (decode and short queries leave its tokens out, long ones see zeros there). */
+ * page_size a multiple of 16, a positive softmax scale, pool and bf16 arrays 16-byte aligned.  A block table may name pages in
+ * any order; of a page number outside of 0 .. n_pages - 1 nothing is read: decode leaves its tokens out, prefill leaves them out
+ * or takes them for zeros. */
 int64_t b2_kv_q4_pool_bytes(int64_t n_pages, int32_t hkv, int32_t head_dim, int32_t page_size); /* 0 for sizes that are refused */
 /* b2_rope_kv_append into such a pool: [per-head q/k RMSNorm ->] NeoX RoPE -> quantization -> append.  The rotation and its
  * roundings are the same.  Per 64 values: e = the one farthest from zero (the largest in a tie), n = round(15 |e| / (max - min)),
@@ -171,7 +172,8 @@ int32_t b2_paged_attn_decode_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_
                                 int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size, float scale,
                                 uint16_t* out_dev);
 /* b2_paged_attn_prefill over such a pool: any number of query tokens per sequence, causal as there.  A query that does not see a
- * token is not touched by it, whatever it holds. */
+ * token is not touched by it, whatever it holds.  Which of two kernels a sequence goes through, and with it how P is rounded
+ * (16 or 8 bits), depends on all the lengths of the call. */
 int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_t* kv_pool_dev, int32_t n_pages,
                                  const int32_t* block_tables_dev, int32_t max_blocks, const int32_t* cu_seqlens_host,
                                  const int32_t* ctx_lens_host, int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim,

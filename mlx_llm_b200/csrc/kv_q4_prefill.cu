@@ -1,9 +1,10 @@
 // Attention over a 4-bit paged cache for any number of query tokens per sequence: prompts, portions of prompts, drafts.
 //
-// Few columns (query tokens x q heads of a group) go through kv_q4_attn.cu, which reads the 4 bits once per 8 columns.  With many, the
-// products decide, not the bytes: kv_q4_prefill_kernel (tcgen05) converts the codes of a tile of 128 keys into the bf16 operands that the
-// tensor cores read from shared memory, once for 256 rows of queries.
+// Few columns (query tokens x q heads of a group) go through kv_q4_attn.cu, which reads and converts the 4 bits once per 8 columns.  With
+// many, the products decide, not the bytes: kv_q4_prefill_kernel (tcgen05) converts the codes of a tile of 128 keys into the bf16 operands
+// that the tensor cores read from shared memory, once for 256 rows of queries.
 #include <algorithm>
+#include <cmath>
 
 #include "kernels.h"
 #include "kv_q4.cuh"
@@ -13,7 +14,11 @@ namespace {
 
 using namespace tc5;
 
-constexpr int kFewColumns = 32;
+// Which of the two, for all sequences of a call, by what they cost in records x blocks of 8 columns.  Both kernels at work on 64 sequences
+// behind 2000 tokens, 4 q heads a kv head: 8 new tokens (~36 columns) 160 and 186 us, 16 new 300 and 189 us; so a tile of 128 keys counts
+// like 41.  The second kernel has ~6 us more of start and end (64 tokens behind 100: 14 and 21 us), and two kernels, one after the other,
+// cost the shorter one's latency (8 sequences of 4 to 12 new tokens behind 1500: 31 us with either kernel, 49 with both).
+constexpr double kTileCost = 41, kStartCost = 8e3, kBothCost = 2e4;
 constexpr int KT = 128;  // keys of a tile
 
 // A tile of K or V: [HD / 64 halves][128 keys][64 dims] bf16, rows of 128 bytes whose 16-byte pieces are swapped as the 128-byte swizzle
@@ -38,7 +43,7 @@ __device__ __forceinline__ uint32_t tile_at(int row, int dim) {  // of 8 dims
 //                   and when S(j) is there, P V of j - 1 has completed, so O may be rescaled.
 // Bound by a block's chain of product, softmax, product (two thirds of it are the tensor cores').  Converting in here costs each CTA what an
 // own kernel would do once per 128 keys, in warps that the chain leaves idle: 512 tokens behind 11800 that read bf16 tiles, made by such a
-// kernel, from L2 took 210 us, with the tensor cores waiting for copies a seventh of the time.
+// kernel, from L2 took 210 us instead of 236, but 64 tokens behind 12000 took 60 instead of 45, and eight sequences of 16 behind 1500 took 47 instead of 33.
 // A value that is NaN must reach the rows that see it and no others, but a row that does not still multiplies it, with zero: it goes into the
 // token's keys, whose scores are masked by choice and not by multiplication, and the value becomes zero.
 // P carries 8 bits (one rounding of each weight, relative 2^-9; their sum is taken before the rounding, whose errors have no sign of their
@@ -514,14 +519,23 @@ __global__ void __launch_bounds__(256) kv_q4_prefill_merge_kernel(const ProductP
 }  // namespace
 
 int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int hkv, int head_dim, Q4Plan& plan) {
-    (void)ctx;
-    (void)hkv;
     (void)head_dim;
     plan = Q4Plan{};
-    const int group = hq / hkv;
+    const int group = hq / hkv, step = 2 * (kRows / group);  // query tokens of an item
+    auto few_cost = [&](const Q4Seq& s) { return (double)((s.ctx + 15) / 16) * hkv * (((int64_t)s.q_len * group + 7) / 8); };
+    auto many_cost = [&](const Q4Seq& s) {
+        return group > kRows ? INFINITY : kTileCost * ((s.ctx + KT - 1) / KT) * hkv * ((s.q_len + step - 1) / step);
+    };
+    double all_few = 0, all_many = kStartCost, each = kStartCost + kBothCost;
+    for (const Q4Seq& s : seqs)
+        if (s.q_len > 0) all_few += few_cost(s), all_many += many_cost(s), each += std::min(few_cost(s), many_cost(s));
+    const bool by_few = all_few <= std::min(all_many, each), by_many = all_many <= each;
     std::vector<Q4Seq> few, many;
     for (const Q4Seq& s : seqs)
-        if (s.q_len > 0) ((long)s.q_len * group <= kFewColumns || group > kRows ? few : many).push_back(s);
+        if (s.q_len > 0) (by_few || (!by_many && few_cost(s) <= many_cost(s)) ? few : many).push_back(s);
+    double line = 0;
+    for (const Q4Seq& s : few) line += few_cost(s);
+    B2_REQUIRE(line < 1073741824.0, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: more than 2^30 records in one call; make fewer sequences a call");
     plan.few = (int)few.size();
     for (const Q4Seq& s : few) plan.host.push_back(s.bt_row);
     for (const Q4Seq& s : few) plan.host.push_back(s.q_row);
@@ -539,7 +553,6 @@ int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int h
         int32_t seq, q, tiles;
     };
     std::vector<Work> work;
-    const int step = 2 * (kRows / group);  // query tokens of an item
     for (int i = 0; i < plan.many; i++)
         for (int q = 0; q < many[i].q_len; q += step)
             work.push_back({i, q, (many[i].ctx - many[i].q_len + std::min(q + step, many[i].q_len) - 1) / KT + 1});
@@ -635,16 +648,13 @@ extern "C" int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, 
     B2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & 15) == 0, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: q and out must be 16-byte aligned");
     if (num_seqs == 0) return B2_OK;
     std::vector<Q4Seq> seqs;
-    double records = 0;
     for (int i = 0; i < num_seqs; i++) {
         const int n = cu_seqlens_host[i + 1] - cu_seqlens_host[i], ctx_len = ctx_lens_host[i];
         B2_REQUIRE(cu_seqlens_host[i] >= 0 && n >= 0 && ctx_len >= n, B2_ERR_MSG, "b2_paged_attn_prefill_q4: ctx_lens must include the new tokens, and cu_seqlens ascend");
         B2_REQUIRE(((int64_t)ctx_len + page_size - 1) / page_size <= max_blocks, B2_ERR_MSG,
                    "b2_paged_attn_prefill_q4: a context needs more blocks than a block-table row holds");
         seqs.push_back(Q4Seq{i, cu_seqlens_host[i], n, ctx_len});
-        records += (ctx_len + 15) / 16 * (double)hkv * (kFewColumns / 8 + 1);
     }
-    B2_REQUIRE(records < 1073741824.0, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: more than 2^30 records in one call; make fewer sequences a call");
     B2_CUDA(cudaSetDevice(ctx->device));
     Q4Plan plan;
     B2_CHECK(b2_kv_q4_plan(ctx, seqs, hq, hkv, head_dim, plan));

@@ -5,7 +5,7 @@ largest sum |q||k| scale.  A weight exp(score) is then off by that, relatively, 
 2^-22 and P, as a bf16 head and remainder, by 2^-17; weights and their sum enter the result.  The sums over n tokens in f32 add at most n 2^-24,
 parts of a run and of blocks included.  So |error| <= (2 (264 2^-24 S + 2^-22 + 2^-17 + n 2^-24)) max|v|, and then the result is rounded to bf16:
 2^-8 of it.
-With many query tokens P is one bf16 number: every weight is off by at most 2^-8 of itself (half a step) and their sum, taken before, is not, so
+With many query tokens P may be one bf16 number: every weight is off by at most 2^-8 of itself (half a step) and their sum, taken before, is not, so
 |error| grows by at most 2^-8 sum(w |v|) / sum(w) <= 2^-8 max|v|."""
 import numpy as np
 import pytest
@@ -362,6 +362,61 @@ def test_prefill(env, seqs, hq, hkv, hd, page):
             check_rows(got[cu[i]:cu[i + 1]], q[cu[i]:cu[i + 1]], cache, i, hd ** -0.5, many=n * hq // hkv > 32)
 
 
+# Long enough that the tensor cores' kernel is the cheaper one for some sequence, or all: keys split over blocks or not, rows of a block that
+# no query fills, groups that do not divide a block of rows, and single tokens next to prompts.
+@pytest.mark.parametrize("seqs, hq, hkv, hd, page", [
+    ([(200, 300), (129, 700), (1, 40), (0, 9), (64, 64)], 32, 8, 128, 16),
+    ([(512, 1000), (1, 9000), (1, 9000), (2, 8999)], 32, 8, 128, 16),  # both kernels
+    ([(100, 6000)], 8, 1, 128, 16),   # 12 splits
+    ([(300, 5001)], 4, 2, 64, 64),    # splits, the last of them shorter
+    ([(300, 2000)], 6, 2, 128, 48),
+    ([(130, 900)], 40, 8, 64, 32),
+    ([(9, 2000)], 128, 1, 128, 16),   # one query a block of rows
+    ([(5, 50)], 130, 1, 128, 16),     # a group that no block of rows holds
+    ([(700, 500)], 8, 8, 128, 16),
+    ([(1000, 0)], 16, 4, 128, 16),
+    ([(1025, 0), (63, 1), (257, 0)], 14, 2, 64, 16),
+])
+def test_prefill_of_many(env, seqs, hq, hkv, hd, page):
+    ctx, K = env
+    lengths = [a + b for a, b in seqs]
+    cache = Cache(env, hq + len(seqs), lengths, hkv, hd, page)
+    cu = np.concatenate([[0], np.cumsum([a for a, _ in seqs])]).astype(np.int32)
+    q = queries(hq, int(cu[-1]), hq, hd)
+    out = ctx.buf(np.full((cu[-1] + 2, hq, hd), 0x7FC1, np.uint16))
+    K.paged_attn_prefill_q4(ctx, ctx.buf(as_bf16(q)), cache.pool, cache.pages, cache.dev_tables, cache.max_blocks, cu, lengths, hq, hkv, hd, page, hd ** -0.5, out)
+    ctx.sync()
+    got = out.download()
+    assert (got[cu[-1]:] == 0x7FC1).all()
+    for i, (n, _) in enumerate(seqs):
+        if n:
+            check_rows(got[cu[i]:cu[i + 1]], q[cu[i]:cu[i + 1]], cache, i, hd ** -0.5, many=True)
+
+
+@pytest.mark.parametrize("new", [2, 300])
+def test_prefill_reads_nothing_outside_the_pool(env, new):
+    """Page numbers outside the pool in one sequence's row: the other sequences' rows are as they were, and finite."""
+    ctx, K = env
+    hq, hkv, hd, page, seqs = 32, 8, 128, 16, [(new, 500), (new, 400), (new, 300)]
+    lengths = [a + b for a, b in seqs]
+    cache = Cache(env, 3, lengths, hkv, hd, page)
+    cu = np.arange(4) * new
+    q = queries(3, 3 * new, hq, hd)
+    got = []
+    for bad in (False, True):
+        tables = cache.tables.copy()
+        if bad:
+            tables[1, :6] = [-1, cache.pages, 2 ** 31 - 1, -2 ** 31, 10 ** 6, -5]
+        out = ctx.empty(q.shape, np.uint16)
+        K.paged_attn_prefill_q4(ctx, ctx.buf(as_bf16(q)), cache.pool, cache.pages, ctx.buf(tables), cache.max_blocks, cu, lengths, hq, hkv, hd, page, hd ** -0.5, out)
+        ctx.sync()
+        got.append(out.download())
+    for i in (0, 2):
+        assert np.array_equal(got[0][cu[i]:cu[i + 1]], got[1][cu[i]:cu[i + 1]])
+        check_rows(got[1][cu[i]:cu[i + 1]], q[cu[i]:cu[i + 1]], cache, i, hd ** -0.5, many=True)
+    assert np.isfinite(H.bf16_to_f32_np(got[1])).all()
+
+
 def test_one_query_is_decode(env):
     ctx, K = env
     lengths = [40, 333, 16, 1]
@@ -438,11 +493,11 @@ def test_prompt_then_tokens_then_choices(env, hd, hq, hkv):
 
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("what", ["key", "value"])
-@pytest.mark.parametrize("new", [3, 60])
-def test_prefill_keeps_a_bad_token_from_earlier_queries(env, hd, what, new):
+@pytest.mark.parametrize("new, cached", [(3, 37), (60, 37), (400, 700)])
+def test_prefill_keeps_a_bad_token_from_earlier_queries(env, hd, what, new, cached):
     """A token whose key or value is NaN: queries before it are as if it were not there, those that see it are NaN."""
     ctx, K = env
-    hq, hkv, page, cached = 4, 2, 16, 37
+    hq, hkv, page = 4, 2, 16
     n = cached + new
     cache = Cache(env, 91, [n], hkv, hd, page)
     q = queries(91, new, hq, hd)
