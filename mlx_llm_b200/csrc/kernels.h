@@ -247,9 +247,9 @@ struct Q4Seq {
 struct Q4Plan {
     std::vector<int32_t> host;
     int few = 0;   // sequences that kv_q4_attn.cu takes: [few] of each of Q4Seq's numbers, from host[0] on
-    int many = 0;  // the others: [many] of each, from host[list] on, then [work] items' sequences and first query tokens
-    int work = 0, longest = 0;  // work items, and the tiles of 128 keys that the longest sees
-    size_t list = 0;
+    // the others, as the segments of kv_q4_prefill.cu: [segments], [joins], [ctas + 1], from these places in host on
+    int ctas = 0, joins = 0, parts = 0;
+    size_t segments = 0, join_list = 0, first = 0;
 };
 struct Q4PrefillParams {
     const uint16_t* q;

@@ -5,6 +5,8 @@
 // that the tensor cores read from shared memory, once for 256 rows of queries.
 #include <algorithm>
 #include <cmath>
+#include <functional>
+#include <type_traits>
 
 #include "kernels.h"
 #include "kv_q4.cuh"
@@ -19,6 +21,8 @@ using namespace tc5;
 // like 41.  The second kernel has ~6 us more of start and end (64 tokens behind 100: 14 and 21 us), and two kernels, one after the other,
 // cost the shorter one's latency (8 sequences of 4 to 12 new tokens behind 1500: 31 us with either kernel, 49 with both).
 constexpr double kTileCost = 41, kStartCost = 8e3, kBothCost = 2e4;
+// In tiles (2.4 us): what a segment costs besides its tiles, what joining parts does, and the shortest run worth a CTA.
+constexpr double kSegmentCost = 2, kJoinCost = 4, kShortRun = 4;
 constexpr int KT = 128;  // keys of a tile
 
 // A tile of K or V: [HD / 64 halves][128 keys][64 dims] bf16, rows of 128 bytes whose 16-byte pieces are swapped as the 128-byte swizzle
@@ -31,8 +35,11 @@ __device__ __forceinline__ uint32_t tile_at(int row, int dim) {  // of 8 dims
     return (uint32_t)(dim >> 6) * (KT * 128) + (uint32_t)row * 128u + ((((uint32_t)dim >> 3) & 7u) ^ ((uint32_t)row & 7u)) * 16u;
 }
 
-// CTA = (two blocks of query rows, kv head[, split of the keys]).  A row is a (query token, q head of the group) pair, the heads of a token
-// next to one another, so that a group shares every tile of K and V, and the two blocks of 128 rows share them again.
+// A CTA fills an SM and goes through segments: two blocks of 128 query rows, a kv head, and tiles of their keys.  A row is a (query token,
+// q head of the group) pair, the heads of a token next to one another, so that a group shares every tile of K and V, and the two blocks share
+// them again.  The host, which knows all lengths, deals the segments out (b2_kv_q4_plan).  The warps that convert are at the next segment's
+// keys, and the other block at its products, while a block writes its rows out: three prompts of ~1049 took 65 us, with a CTA for each
+// segment 72.
 //   warps 0-3, 4-7  softmax of block A, B: thread = row = TMEM lane.  exp2 against a running reference that is raised only when a tile exceeds
 //                   it by more than 2^8 (O is touched only then); P goes as bf16 over the scores' columns.
 //   warps 8-11      codes to operands: a warp has two of the eight records of a tile, reads the next tile's while it converts this one's, and
@@ -43,7 +50,7 @@ __device__ __forceinline__ uint32_t tile_at(int row, int dim) {  // of 8 dims
 //                   and when S(j) is there, P V of j - 1 has completed, so O may be rescaled.
 // Bound by a block's chain of product, softmax, product (two thirds of it are the tensor cores').  Converting in here costs each CTA what an
 // own kernel would do once per 128 keys, in warps that the chain leaves idle: 512 tokens behind 11800 that read bf16 tiles, made by such a
-// kernel, from L2 took 210 us instead of 236, but 64 tokens behind 12000 took 60 instead of 45, and eight sequences of 16 behind 1500 took 47 instead of 33.
+// kernel, from L2 took 210 us instead of 234, but 64 tokens behind 12000 took 60 instead of 42, and eight sequences of 16 behind 1500 took 47 instead of 33.
 // A value that is NaN must reach the rows that see it and no others, but a row that does not still multiplies it, with zero: it goes into the
 // token's keys, whose scores are masked by choice and not by multiplication, and the value becomes zero.
 // P carries 8 bits (one rounding of each weight, relative 2^-9; their sum is taken before the rounding, whose errors have no sign of their
@@ -60,38 +67,31 @@ constexpr uint32_t idesc_pv() {  // N = HD, B MN-major
     return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
+// What a CTA does at a time: 256 rows of queries of a kv head over some tiles of their keys.
+struct alignas(16) Segment {
+    int32_t bt_row, q_row, queries, ctx;        // q_row: of the first query token
+    int32_t sees, kvh, first_tile, n_tiles;     // sees: the last key that the first query token sees
+    int32_t part, unused[3];                    // where the sum goes that other segments complete, or -1: these are all tiles
+};
+struct alignas(16) Join {
+    int32_t q_row, queries, kvh, first_part, parts, unused[3];
+};
 struct ProductParams {
     const uint16_t* q;
     const uint8_t* pool;
     int64_t n_pages;
     const int32_t* block_tables;
     int max_blocks, page_tiles;
-    const int32_t *bt_row, *q_row, *q_len, *ctx;  // [seqs]
-    const int32_t *work_seq, *work_q;             // [items] sequence, first query token
-    int hq, hkv, group, per_block;                // query tokens of a block of rows
-    float scale_log2;                             // times 2^64
+    const Segment* segments;
+    const int32_t* first_segment;  // [CTAs + 1]
+    const Join* joins;
+    int hq, hkv, group, per_block;  // query tokens of a block of rows
+    float scale_log2;               // times 2^64
     uint16_t* out;
-    int splits;
-    float* part_o;   // [item][kv head][split][256 rows][HD], unnormalised, times 2^-64
-    float* part_ml;  // [item][kv head][split][256 rows][2]: reference (log2 domain), sum
+    float* part_o;   // [part][256 rows][HD], unnormalised, times 2^-64
+    float* part_ml;  // [part][256 rows][2]: reference (log2 domain), sum
     int* err;
 };
-struct Item {
-    int seq, q0, queries, ctx, before, tiles, first_tile, n_tiles;
-};
-__device__ __forceinline__ Item item_of(const ProductParams& p, int item, int split) {
-    Item w;
-    w.seq = p.work_seq[item];
-    w.q0 = p.work_q[item];
-    w.queries = min(2 * p.per_block, p.q_len[w.seq] - w.q0);
-    w.ctx = p.ctx[w.seq];
-    w.before = w.ctx - p.q_len[w.seq];
-    w.tiles = (w.before + w.q0 + w.queries - 1) / KT + 1;  // up to the last key that its last query sees
-    const int per = (w.tiles + p.splits - 1) / p.splits;
-    w.first_tile = split * per;
-    w.n_tiles = min(per, w.tiles - w.first_tile);
-    return w;
-}
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
@@ -124,18 +124,18 @@ template <int HD>
 struct Source {  // the two records of a converting warp in a tile
     const uint8_t* rec[2];
     int left[2];
-    __device__ __forceinline__ void find(const ProductParams& p, const Item& w, int kvh, int t, int warp) {
+    __device__ __forceinline__ void find(const ProductParams& p, const Segment& w, int t, int warp) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int r = t * 8 + warp * 2 + i;
             left[i] = w.ctx - r * 16;
             rec[i] = p.pool;
             if (left[i] <= 0) continue;
-            const int index = r / p.page_tiles, page = p.block_tables[(size_t)p.bt_row[w.seq] * p.max_blocks + index];
+            const int index = r / p.page_tiles, page = p.block_tables[(size_t)w.bt_row * p.max_blocks + index];
             if (page < 0 || page >= p.n_pages)
                 left[i] = 0;  // nothing there: zeros
             else
-                rec[i] += (((size_t)page * p.hkv + kvh) * p.page_tiles + r - index * p.page_tiles) * q4::Record<HD>::kBytes;
+                rec[i] += (((size_t)page * p.hkv + w.kvh) * p.page_tiles + r - index * p.page_tiles) * q4::Record<HD>::kBytes;
         }
     }
     __device__ __forceinline__ void read(Words<HD>& x, bool values, int lane) const {
@@ -231,21 +231,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
         if (threadIdx.x == 0) atomicExch(p.err, 7);
         return;
     }
-    const int kvh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const Item w = item_of(p, blockIdx.y, blockIdx.z);
-    if (w.n_tiles <= 0) return;  // (the merge leaves such splits out)
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int begin = p.first_segment[blockIdx.x], end = p.first_segment[blockIdx.x + 1];
     const uint32_t bar = base + S::kBar;
-    const uint32_t q_full = bar;
-    auto full = [&](int s) { return bar + 8u * (1 + s); };
-    auto empty = [&](int s) { return bar + 8u * (6 + s); };
-    auto s_ready = [&](int x) { return bar + 8u * (11 + x); };
-    auto p_ready = [&](int x) { return bar + 8u * (13 + x); };
-    const uint32_t o_ready = bar + 8u * 15, slot_addr = bar + 8u * 16;
+    auto full = [&](int s) { return bar + 8u * s; };
+    auto empty = [&](int s) { return bar + 8u * (5 + s); };
+    auto s_ready = [&](int x) { return bar + 8u * (10 + x); };
+    auto p_ready = [&](int x) { return bar + 8u * (12 + x); };
+    auto q_full = [&](int x) { return bar + 8u * (14 + x); };   // once a segment: Q is there, and O of the last one has been read
+    auto o_ready = [&](int x) { return bar + 8u * (16 + x); };  // once a segment
+    const uint32_t gone = bar + 8u * 18, slot_addr = bar + 8u * 19;
     if (tid == 0) {
-        mbar_init(q_full, 8);
         for (int s = 0; s < kSlots; s++) mbar_init(full(s), 4), mbar_init(empty(s), 1);
-        for (int x = 0; x < 2; x++) mbar_init(s_ready(x), 1), mbar_init(p_ready(x), 4);
-        mbar_init(o_ready, 1);
+        for (int x = 0; x < 2; x++) mbar_init(s_ready(x), 1), mbar_init(p_ready(x), 4), mbar_init(q_full(x), 4), mbar_init(o_ready(x), 1);
+        mbar_init(gone, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == kIssuer) {
@@ -256,14 +255,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot_addr - base));
-    const int n = w.n_tiles;
     bool alive = true;
 
     if (warp >= kConvert && warp < kIssuer) {
         const int row0 = (warp - kConvert) * 32;
         Source<HD> from;
         Words<HD> keys, vals;
-        from.find(p, w, kvh, w.first_tile, warp - kConvert);
+        Segment w = p.segments[begin];
+        int segment = begin, j = 0;
+        auto next = [&] {  // the tile after this one; false if there is none
+            if (++j == w.n_tiles) {
+                if (++segment == end) return false;
+                w = p.segments[segment], j = 0;
+            }
+            from.find(p, w, w.first_tile + j, warp - kConvert);
+            return true;
+        };
+        from.find(p, w, w.first_tile, warp - kConvert);
         from.read(keys, false, lane);
         from.read(vals, true, lane);
         int slot = 0;
@@ -277,13 +285,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
             if (lane == 0) mbar_arrive(full(slot));
             if (++slot == kSlots) slot = 0, parity ^= 1u;
         };
-        for (int j = 0; j < n && alive; j++) {
-            if (j + 1 < n) from.find(p, w, kvh, w.first_tile + j + 1, warp - kConvert);
+        for (bool more = true; more;) {
+            more = next();
             fill([&](uint8_t* tile) { put_keys<HD>(tile, row0, keys, lane); });
             if (!alive) break;
-            if (j + 1 < n) from.read(keys, false, lane);
+            if (more) from.read(keys, false, lane);
             fill([&](uint8_t* tile) { put_values<HD>(tile, row0, vals, lane); });
-            if (j + 1 < n) from.read(vals, true, lane);
+            if (!alive) break;
+            if (more) from.read(vals, true, lane);
         }
         if (!alive && lane == 0) atomicExch(p.err, 2);
     } else if (warp == kIssuer) {
@@ -312,208 +321,265 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
             auto advance = [&] {  // along the ring: K0 V0 K1 V1 ...
                 if (++slot == kSlots) slot = 0, parity ^= 1u;
             };
-            alive = mbar_wait(q_full, 0) && mbar_wait(full(0), 0);
-            if (alive) {
-                tc_fence_after();
-                issue_s(0, 0);
-                issue_s(1, 0);
-                tc_commit(empty(0));
-                advance();
-            }
-            for (int j = 0; j < n && alive; j++) {
-                const int v = slot;
-                alive = mbar_wait(full(v), parity) && mbar_wait(p_ready(0), (uint32_t)j & 1u);
+            uint32_t phase = 0, seg_phase = 0;  // of a tile's barriers, of a segment's
+            for (int segment = begin; segment < end && alive; segment++, seg_phase ^= 1u) {
+                const int n = p.segments[segment].n_tiles, first = slot;
+                alive = mbar_wait(full(first), parity) && mbar_wait(q_full(0), seg_phase);
                 if (!alive) break;
                 tc_fence_after();
-                issue_o(0, v, j > 0);
+                issue_s(0, first);
+                alive = mbar_wait(q_full(1), seg_phase);
+                if (!alive) break;
+                tc_fence_after();
+                issue_s(1, first);
+                tc_commit(empty(first));
                 advance();
-                const int k = slot;
-                if (j + 1 < n) {
-                    alive = mbar_wait(full(k), parity);
+                for (int j = 0; j < n; j++, phase ^= 1u) {
+                    const int v = slot;
+                    alive = mbar_wait(full(v), parity) && mbar_wait(p_ready(0), phase);
                     if (!alive) break;
                     tc_fence_after();
-                    issue_s(0, k);
-                }
-                alive = mbar_wait(p_ready(1), (uint32_t)j & 1u);
-                if (!alive) break;
-                tc_fence_after();
-                issue_o(1, v, j > 0);
-                tc_commit(empty(v));
-                if (j + 1 < n) {
-                    issue_s(1, k);
-                    tc_commit(empty(k));
+                    issue_o(0, v, j > 0);
                     advance();
+                    const int k = slot;
+                    if (j + 1 < n) {
+                        alive = mbar_wait(full(k), parity);
+                        if (!alive) break;
+                        tc_fence_after();
+                        issue_s(0, k);
+                    } else {
+                        tc_commit(o_ready(0));
+                    }
+                    alive = mbar_wait(p_ready(1), phase);
+                    if (!alive) break;
+                    tc_fence_after();
+                    issue_o(1, v, j > 0);
+                    tc_commit(empty(v));
+                    if (j + 1 < n) {
+                        issue_s(1, k);
+                        tc_commit(empty(k));
+                        advance();
+                    } else {
+                        tc_commit(o_ready(1));
+                    }
                 }
             }
-            tc_commit(o_ready);  // (also after a wait that ran out: what is under way ends before the block does)
-            if (!alive) {
+            if (!alive) {  // what is under way ends before the block does
                 atomicExch(p.err, 3);
-                mbar_wait(o_ready, 0);
+                tc_commit(gone);
+                mbar_wait(gone, 0);
             }
         }
         __syncwarp();
     } else {
         const int x = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const int query = x * p.per_block + r / p.group, head = kvh * p.group + r % p.group;  // query: of the item
-        const bool row_ok = r < p.per_block * p.group && query < w.queries;
-        const size_t row = (size_t)(p.q_row[w.seq] + w.q0 + (row_ok ? query : 0)) * p.hq + head % p.hq;
-        {  // this thread's row of Q
-            const uint4* src = reinterpret_cast<const uint4*>(p.q + row * HD);
+        const uint32_t ts = tmem + lanes + x * 128u, to = tmem + lanes + 256u + x * 128u;
+        const int query = x * p.per_block + r / p.group;  // of the segment's
+        const bool in_block = r < p.per_block * p.group;
+        auto row_of = [&](const Segment& w) { return ((size_t)(w.q_row + query) * p.hq + w.kvh * p.group + r % p.group) * HD; };
+        auto copy_q = [&](const Segment& w) {  // this thread's row
+            const bool ok = in_block && query < w.queries;
+            const uint4* src = reinterpret_cast<const uint4*>(p.q + (ok ? row_of(w) : 0));
             uint8_t* dst = smem + S::kQ + x * TILE;
             uint4 v[HD / 8];
 #pragma unroll
-            for (int i = 0; i < HD / 8; i++) v[i] = row_ok ? src[i] : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < HD / 8; i++) v[i] = ok ? src[i] : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < HD / 8; i++)
                 *reinterpret_cast<uint4*>(dst + tile_at(r, 8 * i)) =
                     make_uint4(prmt(v[i].x, v[i].z, 0x5410u), prmt(v[i].x, v[i].z, 0x7632u), prmt(v[i].y, v[i].w, 0x5410u), prmt(v[i].y, v[i].w, 0x7632u));
             fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-        }
-        // last key that the row sees; rows without a query see all (nothing comes of them)
-        const int sees = row_ok ? w.before + w.q0 + query : 0x3fffffff;
-        const uint32_t ts = tmem + lanes + x * 128u, to = tmem + lanes + 256u + x * 128u;
-        float m = kFloor, l = 0.f;
-        for (int j = 0; j < n; j++) {
-            if (!__all_sync(0xffffffffu, mbar_wait(s_ready(x), (uint32_t)j & 1u))) {
-                alive = false;
-                break;
-            }
-            tc_fence_after();
-            // The upper 64 scores are read for the maximum and, once the lower ones have become P, again: a thread has 128 registers.
-            const int key0 = (w.first_tile + j) * KT;
-            const bool masked = key0 + KT - 1 > sees;
-            uint32_t s[2][32];
-            auto read = [&](int half) {
-#pragma unroll
-                for (int c = 0; c < 2; c++) tc_ld32_nowait(ts + half * 64u + c * 32u, s[c]);
-                asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-                if (masked) {
-#pragma unroll
-                    for (int i = 0; i < 64; i++)
-                        if (key0 + half * 64 + i > sees) s[i >> 5][i & 31] = 0xff800000u;
-                }
-            };
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int half = 1; half >= 0; half--) {
-                read(half);
-#pragma unroll
-                for (int i = 0; i < 32; i += 4)
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        mx[c] = max3(mx[c], __uint_as_float(s[c >> 1][i + 2 * (c & 1)]), __uint_as_float(s[c >> 1][i + 2 * (c & 1) + 1]));
-            }
-            const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;  // (the scale is positive)
-            float alpha = 1.f;
-            if (j == 0) {
-                m = top < kFloor ? kFloor : top;
-            } else if (!(top <= m + kRaise)) {  // (a NaN too, which makes all of the row NaN)
-                alpha = fast_exp2(m - top);
-                m = top;
-            }
-            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                l *= alpha;
-#pragma unroll 1
-                for (int c = 0; c < HD / 32; c++) {
-                    uint32_t v[32];
-                    tc_ld32(to + c * 32u, v);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-                    tc_st32(to + c * 32u, v);
-                }
-            }
-            const uint64_t sc = twice(p.scale_log2), neg = twice(-m);
-            uint64_t sum[2] = {0, 0};
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                if (half == 1) read(1);
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t h[16];
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const uint64_t e = fma2(two(s[c][2 * i], s[c][2 * i + 1]), sc, neg);
-                        const float a = fast_exp2(low(e)), b = fast_exp2(high(e));
-                        sum[i & 1] = add2(sum[i & 1], two(__float_as_uint(a), __float_as_uint(b)));
-                        h[i] = pack_bf2(a, b);
-                    }
-                    tc_st16_nowait(ts + (half * 2 + c) * 16u, h);
-                }
-            }
-            const uint64_t both = add2(sum[0], sum[1]);
-            l += low(both) + high(both);
-            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+        };
+        auto q_there = [&] {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready(x));
-        }
-        if (alive && !__all_sync(0xffffffffu, mbar_wait(o_ready, 0))) alive = false;
-        if (alive) {
+            if (lane == 0) mbar_arrive(q_full(x));
+        };
+        Segment w = p.segments[begin];
+        copy_q(w);
+        q_there();
+        uint32_t phase = 0, seg_phase = 0;
+        for (int segment = begin; segment < end; segment++, seg_phase ^= 1u) {
+            // last key that the row sees; rows without a query see all (nothing comes of them)
+            const bool row_ok = in_block && query < w.queries;
+            const int sees = row_ok ? w.sees + query : 0x3fffffff;
+            float m = kFloor, l = 0.f;
+            for (int j = 0; j < w.n_tiles; j++, phase ^= 1u) {
+                if (!__all_sync(0xffffffffu, mbar_wait(s_ready(x), phase))) {
+                    alive = false;
+                    break;
+                }
+                tc_fence_after();
+                // The upper 64 scores are read for the maximum and, once the lower ones have become P, again: a thread has 128 registers.
+                const int key0 = (w.first_tile + j) * KT;
+                const bool masked = key0 + KT - 1 > sees;
+                uint32_t s[2][32];
+                auto read = [&](int half) {
+#pragma unroll
+                    for (int c = 0; c < 2; c++) tc_ld32_nowait(ts + half * 64u + c * 32u, s[c]);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 64; i++)
+                            if (key0 + half * 64 + i > sees) s[i >> 5][i & 31] = 0xff800000u;
+                    }
+                };
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int half = 1; half >= 0; half--) {
+                    read(half);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+                            mx[c] = max3(mx[c], __uint_as_float(s[c >> 1][i + 2 * (c & 1)]), __uint_as_float(s[c >> 1][i + 2 * (c & 1) + 1]));
+                }
+                const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;  // (the scale is positive)
+                float alpha = 1.f;
+                if (j == 0) {
+                    m = top < kFloor ? kFloor : top;
+                } else if (!(top <= m + kRaise)) {  // (a NaN too, which makes all of the row NaN)
+                    alpha = fast_exp2(m - top);
+                    m = top;
+                }
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    l *= alpha;
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; c++) {
+                        uint32_t v[32];
+                        tc_ld32(to + c * 32u, v);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                        tc_st32(to + c * 32u, v);
+                    }
+                }
+                const uint64_t sc = twice(p.scale_log2), neg = twice(-m);
+                uint64_t sum[2] = {0, 0};
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    if (half == 1) read(1);
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t h[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const uint64_t e = fma2(two(s[c][2 * i], s[c][2 * i + 1]), sc, neg);
+                            const float a = fast_exp2(low(e)), b = fast_exp2(high(e));
+                            sum[i & 1] = add2(sum[i & 1], two(__float_as_uint(a), __float_as_uint(b)));
+                            h[i] = pack_bf2(a, b);
+                        }
+                        tc_st16_nowait(ts + (half * 2 + c) * 16u, h);
+                    }
+                }
+                const uint64_t both = add2(sum[0], sum[1]);
+                l += low(both) + high(both);
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready(x));
+            }
+            if (!alive) break;
+            const size_t row = row_of(w);
+            const int part = w.part;
+            if (segment + 1 < end) {  // (all of this segment's scores are there, so its Q is not read any more)
+                w = p.segments[segment + 1];
+                copy_q(w);
+            }
+            alive = __all_sync(0xffffffffu, mbar_wait(o_ready(x), seg_phase));
+            if (!alive) break;
             tc_fence_after();
-            const bool part = p.splits > 1;
             const float inv = l == 0.f ? 0.f : q4::kUnscale / l;
-            const size_t at = (((size_t)blockIdx.y * p.hkv + kvh) * p.splits + blockIdx.z) * (2 * kRows) + x * kRows + r;
+            const size_t at = (size_t)part * (2 * kRows) + x * kRows + r;
 #pragma unroll 1
             for (int c = 0; c < HD / 32; c++) {
-                uint32_t v[32];
-                tc_ld32(to + c * 32u, v);
+                uint32_t o[32];
+                tc_ld32(to + c * 32u, o);
                 if (!row_ok) continue;
-                if (part) {
+                if (part >= 0) {
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        reinterpret_cast<uint4*>(p.part_o + at * HD + c * 32)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        reinterpret_cast<uint4*>(p.part_o + at * HD + c * 32)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 } else {
                     uint32_t h[16];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) h[i] = pack_bf2(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
+                    for (int i = 0; i < 16; i++) h[i] = pack_bf2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        reinterpret_cast<uint4*>(p.out + row * HD + c * 32)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+                    for (int i = 0; i < 4; i++) reinterpret_cast<uint4*>(p.out + row + c * 32)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
                 }
             }
-            if (part && row_ok) p.part_ml[2 * at] = m, p.part_ml[2 * at + 1] = l;
-        } else if (lane == 0) {
-            atomicExch(p.err, 4);
+            if (part >= 0 && row_ok) p.part_ml[2 * at] = m, p.part_ml[2 * at + 1] = l;
+            if (segment + 1 < end) q_there();
         }
+        if (!alive && lane == 0) atomicExch(p.err, 4);
     }
     tc_fence_before();
     __syncthreads();
     if (warp == kIssuer) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Sum of the splits of an item, in their order: a warp per row, HD / 32 dims a lane.
+// Sum of the segments of a query's rows, in their order: a warp has four rows, HD / 32 dims a lane, and reads two segments of all four at
+// once (most rows have two; 36 MB behind 512 tokens: one row and one segment at a time took 16 us).
+constexpr int kJoinRows = 4;
 template <int HD>
 __global__ void __launch_bounds__(256) kv_q4_prefill_merge_kernel(const ProductParams p) {
-    constexpr int D = HD / 32;
+    constexpr int D = HD / 32, N = kJoinRows;
+    using Vec = std::conditional_t<HD == 128, float4, float2>;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     pdl_wait();
-    const int kvh = blockIdx.x, item = blockIdx.y, lane = threadIdx.x & 31;
-    const int r = blockIdx.z * 8 + (threadIdx.x >> 5);  // row of the item
-    const Item w = item_of(p, item, 0);
-    const int in_block = r & (kRows - 1), query = (r / kRows) * p.per_block + in_block / p.group;
-    if (in_block >= p.per_block * p.group || query >= w.queries) return;
-    const int per = (w.tiles + p.splits - 1) / p.splits, used = (w.tiles + per - 1) / per;  // splits that had tiles
-    const size_t at = (((size_t)item * p.hkv + kvh) * p.splits) * (2 * kRows) + r;
-    float m = kFloor;
-    for (int z = 0; z < used; z++) m = fmaxf(m, p.part_ml[2 * (at + (size_t)z * 2 * kRows)]);
-    float l = 0.f, o[D] = {};
-    for (int z = 0; z < used; z++) {
-        const size_t s = at + (size_t)z * 2 * kRows;
-        const float f = fast_exp2(p.part_ml[2 * s] - m);
-        l += f * p.part_ml[2 * s + 1];
+    const int lane = threadIdx.x & 31, row0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * N;
+    const Join w = p.joins[blockIdx.x];
+    const int last = p.per_block * p.group, end = (w.queries - (row0 >= kRows ? p.per_block : 0)) * p.group;  // rows of the block that there are
+    const int in_block = row0 & (kRows - 1), rows = min(min(last, end) - in_block, N);
+    if (rows <= 0) return;
+    float m[N], l[N], o[N][D];
 #pragma unroll
-        for (int i = 0; i < D; i += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(p.part_o + s * HD + lane * D + i);
-            o[i] += f * v.x, o[i + 1] += f * v.y;
-        }
+    for (int i = 0; i < N; i++) {
+        m[i] = kFloor, l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D; d++) o[i][d] = 0.f;
     }
-    const float inv = l == 0.f ? 0.f : q4::kUnscale / l;
-    uint16_t* dst = p.out + ((size_t)(p.q_row[w.seq] + w.q0 + query) * p.hq + (size_t)kvh * p.group + in_block % p.group) * HD + lane * D;
+    for (int z = 0; z < w.parts; z += 2) {
+        float2 ml[2][N];
+        union {
+            Vec v;
+            float f[D];
+        } x[2][N];
 #pragma unroll
-    for (int i = 0; i < D; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf2(o[i] * inv, o[i + 1] * inv);
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const size_t at = (size_t)(w.first_part + min(z + k, w.parts - 1)) * (2 * kRows) + row0 + min(i, rows - 1);
+                ml[k][i] = reinterpret_cast<const float2*>(p.part_ml)[at];
+                x[k][i].v = reinterpret_cast<const Vec*>(p.part_o + at * HD)[lane];
+            }
+        if (z + 1 == w.parts) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                ml[1][i] = make_float2(kFloor, 0.f);
+#pragma unroll
+                for (int d = 0; d < D; d++) x[1][i].f[d] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float top = fmaxf(m[i], ml[k][i].x), f = fast_exp2(m[i] - top), g = fast_exp2(ml[k][i].x - top);
+                m[i] = top, l[i] = l[i] * f + ml[k][i].y * g;  // (a row that is NaN has a NaN sum)
+#pragma unroll
+                for (int d = 0; d < D; d++) o[i][d] = o[i][d] * f + x[k][i].f[d] * g;
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (i >= rows) break;
+        const float inv = l[i] == 0.f ? 0.f : q4::kUnscale / l[i];
+        const int query = (row0 / kRows) * p.per_block + (in_block + i) / p.group;
+        uint16_t* dst = p.out + ((size_t)(w.q_row + query) * p.hq + (size_t)w.kvh * p.group + (in_block + i) % p.group) * HD + lane * D;
+#pragma unroll
+        for (int d = 0; d < D; d += 2) *reinterpret_cast<uint32_t*>(dst + d) = pack_bf2(o[i][d] * inv, o[i][d + 1] * inv);
+    }
 }
 
 }  // namespace
@@ -541,26 +607,80 @@ int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int h
     for (const Q4Seq& s : few) plan.host.push_back(s.q_row);
     for (const Q4Seq& s : few) plan.host.push_back(s.q_len);
     for (const Q4Seq& s : few) plan.host.push_back(s.ctx);
-    plan.many = (int)many.size();
     if (many.empty()) return B2_OK;
-    plan.list = plan.host.size();
-    for (const Q4Seq& s : many) plan.host.push_back(s.bt_row);
-    for (const Q4Seq& s : many) plan.host.push_back(s.q_row);
-    for (const Q4Seq& s : many) plan.host.push_back(s.q_len);
-    for (const Q4Seq& s : many) plan.host.push_back(s.ctx);
-    // the longest items first, so that the last ones to start are short
     struct Work {
         int32_t seq, q, tiles;
     };
     std::vector<Work> work;
-    for (int i = 0; i < plan.many; i++)
+    for (int i = 0; i < (int)many.size(); i++)
         for (int q = 0; q < many[i].q_len; q += step)
             work.push_back({i, q, (many[i].ctx - many[i].q_len + std::min(q + step, many[i].q_len) - 1) / KT + 1});
     std::stable_sort(work.begin(), work.end(), [](const Work& a, const Work& b) { return a.tiles > b.tiles; });
-    plan.work = (int)work.size();
-    plan.longest = work[0].tiles;
-    for (const Work& x : work) plan.host.push_back(x.seq);
-    for (const Work& x : work) plan.host.push_back(x.q);
+    // Two ways to give a GPU's CTAs (one fills an SM) their segments.  Whole: every (item, kv head) in one segment, the longest first, each to
+    // the CTA that has least.  Cut: all their tiles in one line, cut into runs that cost the same; what is cut is joined by another kernel.
+    const double units = (double)work.size() * hkv;
+    double tiles = 0;
+    for (const Work& x : work) tiles += (double)x.tiles * hkv;
+    std::vector<std::pair<double, int>> load;  // a heap with the least loaded CTA first
+    const int whole_ctas = (int)std::min((double)ctx->sm_count, units);
+    for (int i = 0; i < whole_ctas; i++) load.push_back({0, i});
+    std::vector<int32_t> owner;
+    double whole = 0;
+    for (const Work& x : work)
+        for (int h = 0; h < hkv; h++) {
+            std::pop_heap(load.begin(), load.end(), std::greater<>());
+            owner.push_back(load.back().second);
+            whole = std::max(whole, load.back().first += x.tiles + kSegmentCost);
+            std::push_heap(load.begin(), load.end(), std::greater<>());
+        }
+    const int cut_ctas = (int)std::max(1.0, std::min((double)ctx->sm_count, tiles / kShortRun));
+    const double run = std::ceil((tiles + kSegmentCost * (units + cut_ctas)) / cut_ctas);
+    std::vector<Segment> segments;
+    std::vector<Join> joins;
+    std::vector<int32_t> first;
+    auto segment = [&](const Work& x, int h, int from, int n, int part) {
+        const Q4Seq& s = many[x.seq];
+        return Segment{s.bt_row, s.q_row + x.q, std::min(step, s.q_len - x.q), s.ctx, s.ctx - s.q_len + x.q, h, from, n, part, {}};
+    };
+    if (whole <= run + kJoinCost) {
+        std::vector<int32_t> count(whole_ctas + 1, 0);
+        for (int o : owner) count[o + 1]++;
+        for (int i = 0; i < whole_ctas; i++) count[i + 1] += count[i];
+        first = count;
+        segments.resize(owner.size());
+        size_t i = 0;
+        for (const Work& x : work)
+            for (int h = 0; h < hkv; h++) segments[count[owner[i++]]++] = segment(x, h, 0, x.tiles, -1);
+    } else {
+        double left = run;
+        first.push_back(0);
+        for (const Work& x : work)
+            for (int h = 0; h < hkv; h++) {
+                const int start = plan.parts;
+                for (int t = 0; t < x.tiles;) {
+                    const bool last = (int)first.size() >= cut_ctas;
+                    if (!last && left < kSegmentCost + 1) first.push_back((int)segments.size()), left = run;
+                    const int n = (int)first.size() >= cut_ctas ? x.tiles - t : std::min(x.tiles - t, (int)(left - kSegmentCost));
+                    const bool all = n == x.tiles;
+                    segments.push_back(segment(x, h, t, n, all ? -1 : plan.parts));
+                    if (!all) plan.parts++;
+                    t += n, left -= n + kSegmentCost;
+                }
+                if (plan.parts > start)
+                    joins.push_back(Join{segments.back().q_row, segments.back().queries, h, start, plan.parts - start, {}});
+            }
+        first.push_back((int)segments.size());
+    }
+    plan.ctas = (int)first.size() - 1;
+    plan.joins = (int)joins.size();
+    while (plan.host.size() % 4) plan.host.push_back(0);
+    auto add = [&](const void* x, size_t n) { plan.host.insert(plan.host.end(), (const int32_t*)x, (const int32_t*)x + n); };
+    plan.segments = plan.host.size();
+    add(segments.data(), segments.size() * (sizeof(Segment) / 4));
+    plan.join_list = plan.host.size();
+    add(joins.data(), joins.size() * (sizeof(Join) / 4));
+    plan.first = plan.host.size();
+    add(first.data(), first.size());
     return B2_OK;
 }
 
@@ -573,12 +693,9 @@ static int32_t launch_many(b2_ctx* ctx, const Q4PrefillParams& p, const Q4Plan& 
     a.block_tables = p.block_tables;
     a.max_blocks = p.max_blocks;
     a.page_tiles = p.page_tiles;
-    a.bt_row = plan_dev + plan.list;
-    a.q_row = a.bt_row + plan.many;
-    a.q_len = a.q_row + plan.many;
-    a.ctx = a.q_len + plan.many;
-    a.work_seq = a.ctx + plan.many;
-    a.work_q = a.work_seq + plan.work;
+    a.segments = reinterpret_cast<const Segment*>(plan_dev + plan.segments);
+    a.joins = reinterpret_cast<const Join*>(plan_dev + plan.join_list);
+    a.first_segment = plan_dev + plan.first;
     a.hq = p.hq;
     a.hkv = p.hkv;
     a.group = p.hq / p.hkv;
@@ -586,11 +703,8 @@ static int32_t launch_many(b2_ctx* ctx, const Q4PrefillParams& p, const Q4Plan& 
     a.scale_log2 = p.scale_log2 * q4::kUnscale;
     a.out = p.out;
     a.err = ctx->dev_err;
-    // A CTA fills an SM.  Where the items leave half of the SMs idle, the keys are split as well, four tiles a split at least.
-    const int ctas = plan.work * p.hkv;
-    a.splits = ctas * 2 <= ctx->sm_count ? std::max(1, std::min({ctx->sm_count / ctas, plan.longest / 4, 16})) : 1;
-    if (a.splits > 1) {
-        const size_t slots = (size_t)ctas * a.splits * 2 * kRows, bytes = slots * (HD + 2) * sizeof(float);
+    if (plan.parts > 0) {
+        const size_t rows = (size_t)plan.parts * 2 * kRows, bytes = rows * (HD + 2) * sizeof(float);
         if (bytes > ctx->pf_part_bytes) {
             B2_CUDA(cudaStreamSynchronize(ctx->stream));
             if (ctx->pf_part) B2_CUDA(cudaFree(ctx->pf_part));
@@ -600,13 +714,13 @@ static int32_t launch_many(b2_ctx* ctx, const Q4PrefillParams& p, const Q4Plan& 
             ctx->pf_part_bytes = bytes + (bytes >> 2);
         }
         a.part_o = ctx->pf_part;
-        a.part_ml = ctx->pf_part + slots * HD;
+        a.part_ml = ctx->pf_part + rows * HD;
     }
     B2_SMEM_ONCE(ctx, kv_q4_prefill_kernel<HD>, Smem<HD>::kBytes);
-    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_kernel<HD>, dim3(p.hkv, plan.work, a.splits), dim3(kThreads), (size_t)Smem<HD>::kBytes, ctx->stream, a));
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_kernel<HD>, dim3(plan.ctas), dim3(kThreads), (size_t)Smem<HD>::kBytes, ctx->stream, a));
     B2_LAUNCHED(ctx);
-    if (a.splits > 1) {
-        B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_merge_kernel<HD>, dim3(p.hkv, plan.work, 2 * kRows / 8), dim3(256), 0, ctx->stream, a));
+    if (plan.joins > 0) {
+        B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_prefill_merge_kernel<HD>, dim3(plan.joins, 2 * kRows / (8 * kJoinRows)), dim3(256), 0, ctx->stream, a));
         B2_LAUNCHED(ctx);
     }
     B2_CUDA(cudaGetLastError());
@@ -633,8 +747,7 @@ int32_t b2_kv_q4_prefill_launch(b2_ctx* ctx, const Q4PrefillParams& p, int head_
         a.out = p.out;
         B2_CHECK(b2_kv_q4_attn_launch(ctx, a, head_dim));
     }
-    if (plan.many == 0) return B2_OK;
-    B2_REQUIRE(plan.work <= 65535, B2_ERR_UNSUPPORTED, "attention over a 4-bit cache: too many query tokens for one call");
+    if (plan.ctas == 0) return B2_OK;
     return head_dim == 128 ? launch_many<128>(ctx, p, plan, plan_dev) : launch_many<64>(ctx, p, plan, plan_dev);
 }
 
