@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     __shared__ int4 s_scan[kWarps];
     __shared__ Part s_part[kParts];
     __shared__ float s_m[kParts][8], s_l[kParts][8], s_weight[kParts][8], s_sum[kParts][8], s_max[kParts][8];
-    __shared__ int s_last;
+    __shared__ int s_last[2];
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -495,62 +495,60 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         }
     }
     if (crossing[0] < 0 && crossing[1] < 0) return;
-    // ---- units of several blocks: whoever arrives last adds up their parts
+    // ---- units of several blocks: whoever arrives last adds up their parts.  All blocks come here at the same time, so what counts is the
+    // number of trips to L2, one after the other: fence, arrival, parts.
     const int block_run = kWarps * run;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();  // the block's parts are visible before its arrivals are counted
+    if (lane == 0 && warp < 2) {
         int last = 0;
-#pragma unroll
-        for (int side = 0; side < 2; side++)
-            if (crossing[side] >= 0) {
-                const Part u = s_part[crossing[side]];
-                const int from = u.start / block_run, to = (u.start + u.tiles - 1) / block_run;
-                if (atomicAdd(p.counters + from, 1) == to - from) {
-                    last |= 1 << side;
-                    p.counters[from] = 0;
-                }
+        const int mine = crossing[warp];
+        if (mine >= 0) {
+            const Part u = s_part[mine];
+            const int from = u.start / block_run, to = (u.start + u.tiles - 1) / block_run;
+            __threadfence();  // the block's parts are visible before its arrival is counted
+            if (atomicAdd(p.counters + from, 1) == to - from) {
+                last = 1;
+                p.counters[from] = 0;
+                __threadfence();
             }
-        s_last = last;
-        __threadfence();
+        }
+        s_last[warp] = last;
     }
     __syncthreads();
-    float2* const weight = reinterpret_cast<float2*>(smem);  // [blocks][4]: of columns 2c and 2c + 1
+    if (mt >= MT) return;
+#pragma unroll 1
     for (int side = 0; side < 2; side++) {
-        if (!(s_last >> side & 1)) continue;
+        if (!s_last[side]) continue;
         const Part u = s_part[side ? crossing[1] : crossing[0]];
         const int from = u.start / block_run, to = (u.start + u.tiles - 1) / block_run;
-        auto part = [&](int b) { return p.parts + (size_t)(b * 2 + (u.start <= b * block_run ? 0 : 1)) * part_floats<HD>(); };
-        if (warp < 8) {  // a warp per column: weights of the blocks' parts, and their sum
-            float m = kFloor, l = 0.f;
-            for (int b = from + lane; b <= to; b += 32) m = fmaxf(m, __ldcg(part(b) + 8 * HD + 2 * warp));
-            const float top = [&] {
-                float t = m;
+        constexpr int N = 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float m0 = kFloor, m1 = kFloor, l0 = 0.f, l1 = 0.f;
+        for (int b0 = from; b0 <= to; b0 += N) {
+            float4 v[N], ml[N];  // ml: maximum and sum of columns 2c and 2c + 1
 #pragma unroll
-                for (int sh = 1; sh <= 16; sh <<= 1) t = fmaxf(t, __shfl_xor_sync(kFull, t, sh));
-                return t;
-            }();
-            for (int b = from + lane; b <= to; b += 32) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(part(b) + 8 * HD + 2 * warp));
-                const float f = fast_exp2(ml.x - top);
-                l += ml.y * f;
-                reinterpret_cast<float*>(weight)[(b - from) * 8 + warp] = f;
+            for (int i = 0; i < N; i++) {
+                const int b = min(b0 + i, to);
+                const float* part = p.parts + (size_t)(b * 2 + (u.start <= b * block_run ? 0 : 1)) * part_floats<HD>();
+                ml[i] = __ldcg(reinterpret_cast<const float4*>(part + 8 * HD) + c);
+                v[i] = __ldcg(reinterpret_cast<const float4*>(part) + mt * 32 + lane);
             }
+            float top0 = m0, top1 = m1;
 #pragma unroll
-            for (int sh = 1; sh <= 16; sh <<= 1) l += __shfl_xor_sync(kFull, l, sh);
-            if (lane == 0) s_sum[0][warp] = l;
-        }
-        __syncthreads();
-        if (mt < MT) {
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int b = from; b <= to; b++) {
-                const float2 f = weight[(b - from) * 4 + c];
-                add(sum, __ldcg(reinterpret_cast<const float4*>(part(b)) + mt * 32 + lane), f.x, f.y);
+            for (int i = 0; i < N; i++) top0 = fmaxf(top0, ml[i].x), top1 = fmaxf(top1, ml[i].z);
+            const float a0 = fast_exp2(m0 - top0), a1 = fast_exp2(m1 - top1);
+            m0 = top0, m1 = top1;
+            l0 *= a0, l1 *= a1;
+            sum.x *= a0, sum.y *= a1, sum.z *= a0, sum.w *= a1;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if (b0 + i > to) break;
+                const float f0 = fast_exp2(ml[i].x - m0), f1 = fast_exp2(ml[i].z - m1);
+                l0 += ml[i].y * f0, l1 += ml[i].w * f1;
+                add(sum, v[i], f0, f1);
             }
-            store(u, sum, s_sum[0][2 * c], s_sum[0][2 * c + 1]);
         }
-        __syncthreads();  // the weights and the sums are written again
+        store(u, sum, l0, l1);
     }
 }
 
