@@ -315,28 +315,29 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
             }
             cp_async_commit();
         };
+        uint32_t qf[KS][2];
+        auto load_q = [&] {  // Q as the B operand, in the order of the nibbles; columns past the last are zeros
+            const int cols = min(8, use.len.columns - use.block * 8), col = use.block * 8 + min(g, cols - 1), query = col / group;
+            const size_t row = (p.q_rows ? p.q_rows[use.seq] : use.seq) + query;
+            const uint16_t* q = p.q + (row * p.hq + (size_t)use.kvh * group + (col - query * group)) * HD + c * (HD / 4);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                uint4 u = *reinterpret_cast<const uint4*>(q + 8 * w);
+                if (g >= cols) u = make_uint4(0, 0, 0, 0);
+                qf[2 * w][0] = prmt(u.x, u.z, 0x5410u);
+                qf[2 * w][1] = prmt(u.x, u.z, 0x7632u);
+                qf[2 * w + 1][0] = prmt(u.y, u.w, 0x5410u);
+                qf[2 * w + 1][1] = prmt(u.y, u.w, 0x7632u);
+            }
+        };
+        load_q();  // before the records: they would queue up ahead of it
         ask_until(min(end, pos + kStages));
         bool first_of_run = true;
         while (pos < end) {
             const int t0 = use.tile, t1 = min(use.len.tiles, t0 + end - pos);
             const int start = pos - t0;
-            // Q as the B operand, in the order of the nibbles; columns past the last are zeros
-            uint32_t qf[KS][2];
             const int cols = min(8, use.len.columns - use.block * 8);
-            {
-                const int col = use.block * 8 + min(g, cols - 1), query = col / group;
-                const size_t row = (p.q_rows ? p.q_rows[use.seq] : use.seq) + query;
-                const uint16_t* q = p.q + (row * p.hq + (size_t)use.kvh * group + (col - query * group)) * HD + c * (HD / 4);
-#pragma unroll
-                for (int w = 0; w < W; w++) {
-                    uint4 u = *reinterpret_cast<const uint4*>(q + 8 * w);
-                    if (g >= cols) u = make_uint4(0, 0, 0, 0);
-                    qf[2 * w][0] = prmt(u.x, u.z, 0x5410u);
-                    qf[2 * w][1] = prmt(u.x, u.z, 0x7632u);
-                    qf[2 * w + 1][0] = prmt(u.y, u.w, 0x5410u);
-                    qf[2 * w + 1][1] = prmt(u.y, u.w, 0x7632u);
-                }
-            }
+            if (!first_of_run) load_q();
             // keys that columns 2c and 2c + 1 see; all columns see those before `sure`
             int lim0 = use.len.ctx, lim1 = lim0, sure = lim0;
             if (p.q_lens) {
@@ -449,15 +450,28 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         const unsigned up_to = (2u << lane) - 1, head = heads & up_to, later = heads & ~up_to;
         unit = there & (later ? (later & -later) - 1 : ~0u) & ~(head ? (1u << (31 - __clz(head))) - 1 : ~0u);
     }
-    for (int i = threadIdx.x >> 3; i < kParts; i += kThreads / 8) {  // weight of a part's column, and its unit's maximum and sum
-        const unsigned u = __shfl_sync(kFull, unit, i);
-        const int col = threadIdx.x & 7;
-        float m = kFloor, l = 0.f;
+    {  // a warp per column, a lane per part: weight of the part, and its unit's maximum and sum
+        static_assert(kWarps == 8 && kParts <= 32, "a warp has a column, a lane a part");
+        const bool is = there >> lane & 1;
+        const unsigned so_far = heads & ((2u << lane) - 1);
+        const int head = so_far ? 31 - __clz(so_far) : 0, last = unit ? 31 - __clz(unit) : 0;
+        const float own = is ? s_m[lane][warp] : kFloor;
+        float m = own;
 #pragma unroll
-        for (int j = 0; j < kParts; j++) m = fmaxf(m, u >> j & 1 ? s_m[j][col] : kFloor);
+        for (int o = 1; o < kParts; o <<= 1) {
+            const float other = __shfl_up_sync(kFull, m, o);
+            if (lane - o >= head) m = fmaxf(m, other);
+        }
+        m = __shfl_sync(kFull, m, last);
+        const float f = fast_exp2(own - m);
+        float l = is ? s_l[lane][warp] * f : 0.f;
 #pragma unroll
-        for (int j = 0; j < kParts; j++) l += u >> j & 1 ? s_l[j][col] * fast_exp2(s_m[j][col] - m) : 0.f;
-        if (there >> i & 1) s_weight[i][col] = fast_exp2(s_m[i][col] - m), s_max[i][col] = m, s_sum[i][col] = l;
+        for (int o = 1; o < kParts; o <<= 1) {
+            const float other = __shfl_up_sync(kFull, l, o);
+            if (lane - o >= head) l += other;
+        }
+        l = __shfl_sync(kFull, l, last);
+        if (is) s_weight[lane][warp] = f, s_max[lane][warp] = m, s_sum[lane][warp] = l;
     }
     __syncthreads();
     const int mt = warp;
@@ -470,28 +484,30 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     auto add = [](float4& sum, const float4& v, float f0, float f1) { sum.x += v.x * f0, sum.y += v.y * f1, sum.z += v.z * f0, sum.w += v.w * f1; };
     static_assert(MT <= kWarps, "a warp has a tile of the output");
     int crossing[2] = {-1, -1};  // parts of the units that other blocks share: this block's first and its last one
-    for (unsigned h = heads; h; h &= h - 1) {
-        const int head = __ffs(h) - 1;
-        const unsigned all = __shfl_sync(kFull, unit, head);
+    // (kept short: the tail of a kernel is fetched when all blocks come to it)
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    int head = 0;
+#pragma unroll 1
+    for (unsigned rest = there; rest; rest &= rest - 1) {
+        const int i = __ffs(rest) - 1;
+        if (heads >> i & 1) head = i, sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (mt < MT) {
+            const float4* part = (i & 1) ? reinterpret_cast<const float4*>(smem + (i >> 1) * kStages * Rec::kBytes) : parts + (i >> 1) * MT * 32;
+            add(sum, part[mt * 32 + lane], s_weight[i][2 * c], s_weight[i][2 * c + 1]);
+        }
+        const unsigned later = rest & (rest - 1);
+        if (later && !(heads >> (__ffs(later) - 1) & 1)) continue;  // the unit has more parts here
         const Part u = s_part[head];
-        const bool whole = u.first == 0 && s_part[31 - __clz(all)].last == u.tiles;
+        const bool whole = u.first == 0 && s_part[i].last == u.tiles;
         const int side = u.start <= block_start ? 0 : 1;
         if (!whole) crossing[side] = head;
-        if (mt < MT) {
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int i = 0; i < kParts; i++)
-                if (all >> i & 1) {
-                    const float4* part = (i & 1) ? reinterpret_cast<const float4*>(smem + (i >> 1) * kStages * Rec::kBytes) : parts + (i >> 1) * MT * 32;
-                    add(sum, part[mt * 32 + lane], s_weight[i][2 * c], s_weight[i][2 * c + 1]);
-                }
-            if (whole) {
-                store(u, sum, s_sum[head][2 * c], s_sum[head][2 * c + 1]);
-            } else {
-                float* dst = p.parts + (size_t)(blockIdx.x * 2 + side) * part_floats<HD>();
-                reinterpret_cast<float4*>(dst)[mt * 32 + lane] = sum;
-                if (warp == 0 && lane < 8) dst[8 * HD + 2 * lane] = s_max[head][lane], dst[8 * HD + 2 * lane + 1] = s_sum[head][lane];
-            }
+        if (mt >= MT) continue;
+        if (whole) {
+            store(u, sum, s_sum[head][2 * c], s_sum[head][2 * c + 1]);
+        } else {
+            float* dst = p.parts + (size_t)(blockIdx.x * 2 + side) * part_floats<HD>();
+            reinterpret_cast<float4*>(dst)[mt * 32 + lane] = sum;
+            if (warp == 0 && lane < 8) dst[8 * HD + 2 * lane] = s_max[head][lane], dst[8 * HD + 2 * lane + 1] = s_sum[head][lane];
         }
     }
     if (crossing[0] < 0 && crossing[1] < 0) return;
@@ -522,7 +538,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         const Part u = s_part[side ? crossing[1] : crossing[0]];
         const int from = u.start / block_run, to = (u.start + u.tiles - 1) / block_run;
         constexpr int N = 4;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        sum = make_float4(0.f, 0.f, 0.f, 0.f);
         float m0 = kFloor, m1 = kFloor, l0 = 0.f, l1 = 0.f;
         for (int b0 = from; b0 <= to; b0 += N) {
             float4 v[N], ml[N];  // ml: maximum and sum of columns 2c and 2c + 1
