@@ -231,6 +231,7 @@ struct Q4AttnParams {
     const int32_t* ctx_lens;      // [num_seqs] tokens in the cache, the queries' own included
     const int32_t* q_lens;        // [num_seqs] query tokens, the last of the context; null: one each
     int num_seqs, hq, hkv, page_tiles;
+    int64_t columns;              // the most (query tokens x q heads of a group) that a sequence has
     float scale_log2;             // softmax scale * log2(e)
     uint16_t* out;                // [rows, hq, hd] bf16
     // filled in by the launch
@@ -246,6 +247,7 @@ struct Q4Seq {
 };
 struct Q4Plan {
     std::vector<int32_t> host;
+    int64_t few_columns = 0;  // the most that a sequence of those has
     int few = 0;   // sequences that kv_q4_attn.cu takes: [few] of each of Q4Seq's numbers, from host[0] on
     // the others, as the segments of kv_q4_prefill.cu: [segments], [joins], [ctas + 1], from these places in host on
     int ctas = 0, joins = 0, parts = 0;

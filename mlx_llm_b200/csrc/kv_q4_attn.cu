@@ -13,7 +13,9 @@
 //   tensor  = mma.sync m16n8k16 with the record's 16 tokens on M and the columns on N: S^T = K Q^T, then O^T += V^T P^T.  Codes become
 //             A operands in place (9 instructions for 8 codes, kv_q4.cuh); the order of dims inside a product is free, so Q is read in
 //             the order that the nibbles come out.  P^T reaches the B layout with one movmatrix per 8 tokens; it is split into a bf16
-//             head and remainder, so that P V keeps ~16 bits.
+//             head and remainder, so that P V keeps ~16 bits.  Where no unit has more than 4 columns (single tokens of groups of 4) the other
+//             four carry the remainder: Q is there twice, P's lanes take one or the other, and one product does for two (HD / 16 fewer
+//             a record; 64 sequences of 8192 150 -> 143 us).
 //   softmax = in the log2 domain against a running reference that is raised only when a score exceeds it by more than 2^8.
 #include <algorithm>
 
@@ -133,7 +135,7 @@ __device__ __forceinline__ void hidden_values(const uint8_t* rec, int lane, floa
 // O^T[dim, column] += V^T P^T of a record; rows g and g + 8 of tile mt are dims 2 mt and 2 mt + 1 of this lane's block.  `left`: tokens of
 // the record that belong to the context; what lies behind them may be anything, and 0 * NaN is NaN.  `some`: not every column sees every
 // token, so that values that are NaN have gone into the scores (hidden_values)
-template <int HD>
+template <int HD, bool kNarrow>
 __device__ __forceinline__ void add_values(const uint8_t* rec, int lane, const float (&p)[4], int left, bool some, float (&o)[HD / 16][4]) {
     using Rec = q4::Record<HD>;
     constexpr int W = HD / 32;
@@ -155,8 +157,12 @@ __device__ __forceinline__ void add_values(const uint8_t* rec, int lane, const f
     uint32_t pb[2], pl[2];
     const uint32_t h01 = pack_bf2(p[0], p[1]), h23 = pack_bf2(p[2], p[3]);
     const uint32_t r01 = pack_bf2(p[0] - bflo(h01), p[1] - bfhi(h01)), r23 = pack_bf2(p[2] - bflo(h23), p[3] - bfhi(h23));
-    pb[0] = movmatrix_trans(h01), pb[1] = movmatrix_trans(h23);
-    pl[0] = movmatrix_trans(r01), pl[1] = movmatrix_trans(r23);
+    if constexpr (kNarrow) {
+        pb[0] = movmatrix_trans(c < 2 ? h01 : r01), pb[1] = movmatrix_trans(c < 2 ? h23 : r23);
+    } else {
+        pb[0] = movmatrix_trans(h01), pb[1] = movmatrix_trans(h23);
+        pl[0] = movmatrix_trans(r01), pl[1] = movmatrix_trans(r23);
+    }
     const q4::Scales qa = q4::scales_pair(sb0.x, sb0.y), qb = q4::scales_pair(sb1.x, sb1.y);
     uint32_t wa[W], wb[W];
     lane_words<W>(rec + Rec::kV, lane, wa);
@@ -169,12 +175,14 @@ __device__ __forceinline__ void add_values(const uint8_t* rec, int lane, const f
         const uint32_t a0[4] = {va[0], va[1], vb[0], vb[1]}, a1[4] = {va[2], va[3], vb[2], vb[3]};
         mma_bf16_16816(o[2 * w], a0, pb);
         mma_bf16_16816(o[2 * w + 1], a1, pb);
-        mma_bf16_16816(o[2 * w], a0, pl);
-        mma_bf16_16816(o[2 * w + 1], a1, pl);
+        if constexpr (!kNarrow) {
+            mma_bf16_16816(o[2 * w], a0, pl);
+            mma_bf16_16816(o[2 * w + 1], a1, pl);
+        }
     }
 }
 
-template <int HD>
+template <int HD, bool kNarrow>
 __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(const Q4AttnParams p) {
     using Rec = q4::Record<HD>;
     constexpr int W = HD / 32;  // words of a lane per token (K) or token pair (V)
@@ -317,13 +325,13 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         };
         uint32_t qf[KS][2];
         auto load_q = [&] {  // Q as the B operand, in the order of the nibbles; columns past the last are zeros
-            const int cols = min(8, use.len.columns - use.block * 8), col = use.block * 8 + min(g, cols - 1), query = col / group;
+            const int cols = min(8, use.len.columns - use.block * 8), col = use.block * 8 + min(kNarrow ? g & 3 : g, cols - 1), query = col / group;
             const size_t row = (p.q_rows ? p.q_rows[use.seq] : use.seq) + query;
             const uint16_t* q = p.q + (row * p.hq + (size_t)use.kvh * group + (col - query * group)) * HD + c * (HD / 4);
 #pragma unroll
             for (int w = 0; w < W; w++) {
                 uint4 u = *reinterpret_cast<const uint4*>(q + 8 * w);
-                if (g >= cols) u = make_uint4(0, 0, 0, 0);
+                if (!kNarrow && g >= cols) u = make_uint4(0, 0, 0, 0);
                 qf[2 * w][0] = prmt(u.x, u.z, 0x5410u);
                 qf[2 * w][1] = prmt(u.x, u.z, 0x7632u);
                 qf[2 * w + 1][0] = prmt(u.y, u.w, 0x5410u);
@@ -342,7 +350,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
             int lim0 = use.len.ctx, lim1 = lim0, sure = lim0;
             if (p.q_lens) {
                 const int hidden = use.len.ctx - p.q_lens[use.seq] + 1;
-                lim0 = hidden + (use.block * 8 + 2 * c) / group, lim1 = hidden + (use.block * 8 + 2 * c + 1) / group;
+                const int col = use.block * 8 + 2 * (kNarrow ? c & 1 : c);
+                lim0 = hidden + col / group, lim1 = hidden + (col + 1) / group;
                 sure = hidden + use.block * 8 / group;
             }
             float m0 = kFloor, m1 = kFloor, l0 = 0.f, l1 = 0.f;
@@ -400,14 +409,20 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
                 for (int j = 0; j < 4; j++) s0[j] = fast_exp2(s0[j] - (j & 1 ? m1 : m0)), s1[j] = fast_exp2(s1[j] - (j & 1 ? m1 : m0));
                 l0 += (s0[0] + s0[2]) + (s1[0] + s1[2]);
                 l1 += (s0[1] + s0[3]) + (s1[1] + s1[3]);
-                if (one) add_values<HD>(rec0, lane, s0, use.len.ctx - tok0, some, o);
-                if (two) add_values<HD>(rec1, lane, s1, use.len.ctx - tok0 - 16, some, o);
+                if (one) add_values<HD, kNarrow>(rec0, lane, s0, use.len.ctx - tok0, some, o);
+                if (two) add_values<HD, kNarrow>(rec1, lane, s1, use.len.ctx - tok0 - 16, some, o);
             }
             pos += t1 - t0;
 #pragma unroll
             for (int sh = 4; sh <= 16; sh <<= 1) {
                 l0 += __shfl_xor_sync(kFull, l0, sh);
                 l1 += __shfl_xor_sync(kFull, l1, sh);
+            }
+            if constexpr (kNarrow) {
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[mt][j] += __shfl_xor_sync(kFull, o[mt][j], 2);
             }
             if (t0 == 0 && t1 == use.len.tiles) {
 #pragma unroll
@@ -568,7 +583,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     }
 }
 
-template <int HD>
+template <int HD, bool kNarrow>
 int32_t launch(b2_ctx* ctx, Q4AttnParams p) {
     const int grid = kBlocksPerSm * ctx->sm_count;
     if (!ctx->q4_parts) {  // two parts per block, and an arrival counter each (zero between launches)
@@ -582,8 +597,9 @@ int32_t launch(b2_ctx* ctx, Q4AttnParams p) {
     p.entries = (p.num_seqs + p.per_entry - 1) / p.per_entry;
     p.parts = ctx->q4_parts;
     p.counters = reinterpret_cast<int*>(ctx->q4_parts + (size_t)grid * 2 * part_floats<128>());
-    B2_SMEM_ONCE(ctx, kv_q4_attn_kernel<HD>, smem_bytes<HD>());
-    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kv_q4_attn_kernel<HD>, dim3(grid), dim3(kWarps * 32), (size_t)smem_bytes<HD>(), ctx->stream, p));
+    const auto kernel = kv_q4_attn_kernel<HD, kNarrow>;
+    B2_SMEM_ONCE(ctx, kernel, smem_bytes<HD>());
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kernel, dim3(grid), dim3(kWarps * 32), (size_t)smem_bytes<HD>(), ctx->stream, p));
     B2_LAUNCHED(ctx);
     B2_CUDA(cudaGetLastError());
     return B2_OK;
@@ -604,7 +620,8 @@ int32_t b2_kv_q4_check(const char* who, const void* pool, int64_t n_pages, int32
 
 int32_t b2_kv_q4_attn_launch(b2_ctx* ctx, const Q4AttnParams& p, int head_dim) {
     if (p.num_seqs <= 0) return B2_OK;
-    return head_dim == 128 ? launch<128>(ctx, p) : launch<64>(ctx, p);
+    if (p.columns <= 4) return head_dim == 128 ? launch<128, true>(ctx, p) : launch<64, true>(ctx, p);
+    return head_dim == 128 ? launch<128, false>(ctx, p) : launch<64, false>(ctx, p);
 }
 
 extern "C" int64_t b2_kv_q4_pool_bytes(int64_t n_pages, int32_t hkv, int32_t head_dim, int32_t page_size) {
@@ -631,6 +648,7 @@ extern "C" int32_t b2_paged_attn_decode_q4(b2_ctx* ctx, const uint16_t* q_dev, c
     p.max_blocks = max_blocks;
     p.ctx_lens = ctx_lens_dev;
     p.num_seqs = num_seqs;
+    p.columns = hq / hkv;
     p.hq = hq;
     p.hkv = hkv;
     p.page_tiles = page_size / 16;

@@ -600,7 +600,7 @@ int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int h
     for (const Q4Seq& s : seqs)
         if (s.q_len > 0) (by_few || (!by_many && few_cost(s) <= many_cost(s)) ? few : many).push_back(s);
     double line = 0;
-    for (const Q4Seq& s : few) line += few_cost(s);
+    for (const Q4Seq& s : few) line += few_cost(s), plan.few_columns = std::max(plan.few_columns, (int64_t)s.q_len * group);
     B2_REQUIRE(line < 1073741824.0, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: more than 2^30 records in one call; make fewer sequences a call");
     plan.few = (int)few.size();
     for (const Q4Seq& s : few) plan.host.push_back(s.bt_row);
@@ -740,6 +740,7 @@ int32_t b2_kv_q4_prefill_launch(b2_ctx* ctx, const Q4PrefillParams& p, int head_
         a.q_lens = plan_dev + 2 * plan.few;
         a.ctx_lens = plan_dev + 3 * plan.few;
         a.num_seqs = plan.few;
+        a.columns = plan.few_columns;
         a.hq = p.hq;
         a.hkv = p.hkv;
         a.page_tiles = p.page_tiles;
