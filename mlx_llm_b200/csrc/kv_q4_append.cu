@@ -6,10 +6,11 @@
 // (e the maximum in a tie; halves away from zero).  Codes are taken for the scale as it is stored, so that its rounding costs nothing
 // again; all values equal: scale 0.  A NaN or an infinity makes the scale a NaN, and with it the group's values, as they would be in bf16.
 //
-// Bound by HBM (6151 tokens of 64 + 16 heads: 261 MB) once the instructions are few: HD / 16 lanes take a head, each 8 adjacent dims of
-// either half, so that reads and writes are 16 bytes, the rotation's roundings come with bf16x2 instructions (a product or a sum of two
-// bf16 numbers rounded once is what they give), a lane's codes of a group are one word, and a warp has HD 128: 4, HD 64: 8 heads.
-// Queries, keys and values are warps of their own.
+// Bound by HBM (6151 tokens of 64 + 16 heads with norms: 261 MB in 58.6 us, 4.5 TB/s) once the instructions are few: HD / 16 lanes take a
+// head, each 8 adjacent dims of either half, so that reads and writes are 16 bytes, the rotation's roundings come with bf16x2 instructions
+// (a product or a sum of two bf16 numbers rounded once is what they give), and a lane's codes of a group are one word.  The lanes go through
+// two heads of a token with one set of positions and norm weights (one head: 65.7 us, four: 60.5 us, and few tokens wait longer: 608 take
+// 6.5, 6.8 and 12.9 us).  Queries, keys and values are warps of their own, keys first, since they take longest (queries first: 60.3 us).
 #include "kernels.h"
 #include "kv_q4.cuh"
 
@@ -17,6 +18,7 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 4;
+constexpr int kHeads = 2;  // heads of a token that a group of lanes goes through
 
 __device__ __forceinline__ uint32_t add_bf2(uint32_t a, uint32_t b) {
     uint32_t d;
@@ -137,82 +139,99 @@ __device__ __forceinline__ Eight values_of(uint32_t word, const Group& q) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kWarps * 32) rope_kv_q4_kernel(const RopeKvQ4Params a, int q_blocks, int kv_blocks) {
+__global__ void __launch_bounds__(kWarps * 32) rope_kv_q4_kernel(const RopeKvQ4Params a, int kv_blocks) {
     using Rec = q4::Record<HD>;
-    constexpr int L = HD / 16;  // lanes of a head
+    constexpr int L = HD / 16, R = kHeads;  // L lanes a head
     const RopeKvParams& p = a.rope;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     pdl_wait();
-    const int kind = blockIdx.x < q_blocks ? 0 : blockIdx.x < q_blocks + kv_blocks ? 1 : 2;  // queries, keys, values
-    const int block = blockIdx.x - (kind == 0 ? 0 : kind == 1 ? q_blocks : q_blocks + kv_blocks);
+    // keys, values, queries: those that take longest come first
+    const int kind = blockIdx.x < kv_blocks ? 1 : blockIdx.x < 2 * kv_blocks ? 2 : 0;
+    const int block = blockIdx.x - (kind == 1 ? 0 : kind == 2 ? kv_blocks : 2 * kv_blocks);
     const int lane = threadIdx.x & 31, j = lane % L;
-    const int heads = kind == 0 ? p.hq : p.hkv;
-    const int item = (block * kWarps + (threadIdx.x >> 5)) * (32 / L) + lane / L;
-    const bool real = item < p.T * heads;  // (lanes without a head go through the motions of the last one)
-    const int tok = (real ? item : p.T * heads - 1) / heads, head = (real ? item : p.T * heads - 1) - tok * heads;
-    const uint16_t* src = p.qkv + (size_t)tok * p.ld + (size_t)(head + (kind == 0 ? 0 : kind == 1 ? p.hq : p.hq + p.hkv)) * HD + 8 * j;
-    Eight x = load8(src), y = load8(src + HD / 2);
+    const int heads = kind == 0 ? p.hq : p.hkv, chunks = (heads + R - 1) / R;  // of R heads of a token
+    const int chunk = (block * kWarps + (threadIdx.x >> 5)) * (32 / L) + lane / L, last = p.T * chunks - 1;
+    const int tok = min(chunk, last) / chunks, head0 = (min(chunk, last) - tok * chunks) * R;  // (lanes without heads go through the motions of the last)
+    const int real_heads = chunk <= last ? min(heads - head0, R) : 0;
+    const uint16_t* src = p.qkv + (size_t)tok * p.ld + (size_t)(head0 + (kind == 0 ? 0 : kind == 1 ? p.hq : p.hq + p.hkv)) * HD + 8 * j;
+    Eight xs[R], ys[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const uint16_t* at = src + min(r, heads - 1 - head0) * HD;
+        xs[r] = load8(at), ys[r] = load8(at + HD / 2);
+    }
+    const uint16_t* nw = kind == 0 ? p.q_norm : p.k_norm;
+    Eight c, s, wa, wb;
     if (kind < 2) {
         const size_t at = (size_t)p.positions[tok] * (HD / 2) + 8 * j;
-        const Eight c = load8(p.cos_table + at), s = load8(p.sin_table + at);
-        const uint16_t* nw = kind == 0 ? p.q_norm : p.k_norm;
-        if (nw) {
-            const Eight wa = load8(nw + 8 * j), wb = load8(nw + HD / 2 + 8 * j);
-            if (kind == 0)
-                norm_query<HD>(x, y, wa, wb, p.eps);
-            else
-                norm_key<HD>(x, y, wa, wb, p.eps);
-        }
+        c = load8(p.cos_table + at), s = load8(p.sin_table + at);
+        if (nw) wa = load8(nw + 8 * j), wb = load8(nw + HD / 2 + 8 * j);
+    }
+    auto rotate = [&](Eight& x, Eight& y) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t u = sub_bf2(mul_bf2(x.w[i], c.w[i]), mul_bf2(y.w[i], s.w[i])), v = add_bf2(mul_bf2(y.w[i], c.w[i]), mul_bf2(x.w[i], s.w[i]));
             x.w[i] = u, y.w[i] = v;
         }
-    }
+    };
     if (kind == 0) {
-        if (real) {
-            uint16_t* dst = p.q_out + ((size_t)tok * p.hq + head) * HD + 8 * j;
-            store8(dst, x);
-            store8(dst + HD / 2, y);
+        uint16_t* dst = p.q_out + ((size_t)tok * p.hq + head0) * HD + 8 * j;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if (nw) norm_query<HD>(xs[r], ys[r], wa, wb, p.eps);
+            rotate(xs[r], ys[r]);
+            if (r < real_heads) {
+                store8(dst + r * HD, xs[r]);
+                store8(dst + r * HD + HD / 2, ys[r]);
+            }
         }
         return;
     }
     const bool is_k = kind == 1;
-    float lo1, hi1, lo2, hi2;
-    ends_of(x, lo1, hi1);
-    ends_of(y, lo2, hi2);
-    if (Rec::kGroups == 1) lo1 = lo2 = min_nan(lo1, lo2), hi1 = hi2 = max_nan(hi1, hi2);
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) {
-        lo1 = min_nan(lo1, __shfl_xor_sync(kFull, lo1, o)), hi1 = max_nan(hi1, __shfl_xor_sync(kFull, hi1, o));
-        if (Rec::kGroups == 2) lo2 = min_nan(lo2, __shfl_xor_sync(kFull, lo2, o)), hi2 = max_nan(hi2, __shfl_xor_sync(kFull, hi2, o));
-    }
-    const Group q1 = group_of(lo1, hi1), q2 = Rec::kGroups == 2 ? group_of(lo2, hi2) : q1;
-    const uint32_t c1 = codes_of(x, q1), c2 = codes_of(y, q2);
     const int slot = p.slot_mapping[tok];
-    if (real && slot >= 0 && slot < a.n_slots) {
-        const int page = slot / p.page_size, off = slot - page * p.page_size, t = off & 15;
-        uint8_t* rec = a.pool + (((size_t)page * p.hkv + head) * (p.page_size >> 4) + (off >> 4)) * Rec::kBytes;
-        if (is_k) {  // a word has eight dims
-            uint32_t* row = reinterpret_cast<uint32_t*>(rec) + t * (HD / 8) + j;
-            row[0] = c1;
-            row[HD / 16] = c2;
-        } else {  // a half word has four: word d of block g, for dims 8 j + 4 i and HD/2 + 8 j + 4 i
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int d = (i >> 1) * (HD / 2) + 8 * j + 4 * (i & 1);
-                const int word = (((t >> 3) * 8 + d / (HD / 8)) * 4 + ((t & 7) >> 1)) * (HD / 32) + d % (HD / 8) / 4;
-                reinterpret_cast<uint16_t*>(rec + Rec::kV)[2 * word + (t & 1)] = (uint16_t)((i >> 1 ? c2 : c1) >> (16 * (i & 1)));
-            }
+    for (int r = 0; r < R; r++) {
+        Eight &x = xs[r], &y = ys[r];
+        const int head = head0 + r;
+        if (is_k) {
+            if (nw) norm_key<HD>(x, y, wa, wb, p.eps);
+            rotate(x, y);
         }
-        if (j < Rec::kGroups)
-            reinterpret_cast<uint32_t*>(rec + (is_k ? Rec::kKsb : Rec::kVsb))[j * 16 + t] = pack_bf2(j ? q2.scale : q1.scale, j ? q2.edge : q1.edge);
-    }
-    uint16_t* dst = is_k ? a.k_out : a.v_out;
-    if (dst && real) {
-        dst += ((size_t)tok * p.hkv + head) * HD + 8 * j;
-        store8(dst, values_of(c1, q1));
-        store8(dst + HD / 2, values_of(c2, q2));
+        float lo1, hi1, lo2, hi2;
+        ends_of(x, lo1, hi1);
+        ends_of(y, lo2, hi2);
+        if (Rec::kGroups == 1) lo1 = lo2 = min_nan(lo1, lo2), hi1 = hi2 = max_nan(hi1, hi2);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) {
+            lo1 = min_nan(lo1, __shfl_xor_sync(kFull, lo1, o)), hi1 = max_nan(hi1, __shfl_xor_sync(kFull, hi1, o));
+            if (Rec::kGroups == 2) lo2 = min_nan(lo2, __shfl_xor_sync(kFull, lo2, o)), hi2 = max_nan(hi2, __shfl_xor_sync(kFull, hi2, o));
+        }
+        const Group q1 = group_of(lo1, hi1), q2 = Rec::kGroups == 2 ? group_of(lo2, hi2) : q1;
+        const uint32_t c1 = codes_of(x, q1), c2 = codes_of(y, q2);
+        if (r < real_heads && slot >= 0 && slot < a.n_slots) {
+            const int page = slot / p.page_size, off = slot - page * p.page_size, t = off & 15;
+            uint8_t* rec = a.pool + (((size_t)page * p.hkv + head) * (p.page_size >> 4) + (off >> 4)) * Rec::kBytes;
+            if (is_k) {  // a word has eight dims
+                uint32_t* row = reinterpret_cast<uint32_t*>(rec) + t * (HD / 8) + j;
+                row[0] = c1;
+                row[HD / 16] = c2;
+            } else {  // a half word has four: word d of block g, for dims 8 j + 4 i and HD/2 + 8 j + 4 i
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int d = (i >> 1) * (HD / 2) + 8 * j + 4 * (i & 1);
+                    const int word = (((t >> 3) * 8 + d / (HD / 8)) * 4 + ((t & 7) >> 1)) * (HD / 32) + d % (HD / 8) / 4;
+                    reinterpret_cast<uint16_t*>(rec + Rec::kV)[2 * word + (t & 1)] = (uint16_t)((i >> 1 ? c2 : c1) >> (16 * (i & 1)));
+                }
+            }
+            if (j < Rec::kGroups)
+                reinterpret_cast<uint32_t*>(rec + (is_k ? Rec::kKsb : Rec::kVsb))[j * 16 + t] = pack_bf2(j ? q2.scale : q1.scale, j ? q2.edge : q1.edge);
+        }
+        uint16_t* dst = is_k ? a.k_out : a.v_out;
+        if (dst && r < real_heads) {
+            dst += ((size_t)tok * p.hkv + head) * HD + 8 * j;
+            store8(dst, values_of(c1, q1));
+            store8(dst + HD / 2, values_of(c2, q2));
+        }
     }
 }
 
@@ -221,10 +240,11 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kv_q4_kernel(const RopeKvQ4P
 int32_t b2_rope_kv_q4_launch(b2_ctx* ctx, const RopeKvQ4Params& a) {
     const RopeKvParams& p = a.rope;
     if (p.T <= 0) return B2_OK;
-    const int per = kWarps * 512 / p.hd;  // heads of a block
-    const int q_blocks = (int)(((long)p.T * p.hq + per - 1) / per), kv_blocks = (int)(((long)p.T * p.hkv + per - 1) / per);
+    const int per = kWarps * 512 / p.hd;  // chunks of a block
+    auto blocks = [&](int heads) { return (int)(((long)p.T * ((heads + kHeads - 1) / kHeads) + per - 1) / per); };
+    const int q_blocks = blocks(p.hq), kv_blocks = blocks(p.hkv);
     auto kernel = p.hd == 128 ? rope_kv_q4_kernel<128> : rope_kv_q4_kernel<64>;
-    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kernel, dim3(q_blocks + 2 * kv_blocks), dim3(kWarps * 32), 0, ctx->stream, a, q_blocks, kv_blocks));
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kernel, dim3(q_blocks + 2 * kv_blocks), dim3(kWarps * 32), 0, ctx->stream, a, kv_blocks));
     B2_LAUNCHED(ctx);
     B2_CUDA(cudaGetLastError());
     return B2_OK;
