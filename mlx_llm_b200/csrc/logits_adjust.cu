@@ -4,9 +4,9 @@
 // A token's value v, in f32, each step with one rounding:  seen before: v / r where v > 0, else v r;  n times in the answer: (v - n f) - p;
 // with a bias: v + b;  not allowed: -inf.  The choice is made among these; written out they are rounded to the logits' type.
 //
-// Bound by the bytes of the logits for many rows and by the latency of its phases for few.  A cluster of eight blocks takes a row, each
-// block one eighth of the vocabulary.  A block reads the row's whole history and biases (from L2, but for the first block) and marks what
-// falls into its eighth: a bit per token that a rule names.  The pass over the logits leaves these out; they are listed, counted by their
+// Bound by the bytes of the logits for many rows and by the latency of its phases for few.  A cluster of blocks takes a row, each
+// block its share of the vocabulary.  A block reads the row's whole history and biases (from L2, but for the first block) and marks what
+// falls into its share: a bit per token that a rule names.  The pass over the logits leaves these out; they are listed, counted by their
 // rank among the bits, and dealt out to the threads one by one, so that a history's favourites, which lie close together in a vocabulary,
 // hold no warp up.  Shared memory does not grow with the vocabulary that way, and several blocks fit an SM, one's phases behind another's
 // loads.  The first logits, mask words and tokens of the history are on their way before the first phase.  Counters are integers, so the
@@ -301,13 +301,15 @@ int32_t b2_logits_adjust_launch(b2_ctx* ctx, const b2_logit_rules& rules, const 
     p.argmax = argmax;
     p.ld = ld;
     p.vocab = vocab;
-    // Few rows: as many threads and loads as a row can use.  Many: fewer blocks, each of which reads the history, so that all rows' phases overlap.
-    const bool few = rows * 8 <= ctx->sm_count;
+    // Few rows: as many blocks, threads and loads as a row can use.  More: fewer blocks, each of which reads the history, so that all rows'
+    // phases overlap.  More blocks than SMs hold at once: smaller ones, of which a last wave leaves less idle.  128256 tokens, bf16, 18 / 48 /
+    // 256 rows: eight blocks 10.1 / 16.4 / 56 us, four of 512 threads 10.4 / 13.0 / 37.9, four of 256 12.3 / 14.8 / 34.1.
+    const bool few = (int64_t)rows * 8 <= ctx->sm_count, many = (int64_t)rows * 4 > 3 * ctx->sm_count;
     const int blocks = few ? 8 : 4;
     p.slice = std::min(kMaxSlice, ((vocab + blocks - 1) / blocks + 31) / 32 * 32);
-    auto kernel = f32 ? few ? logits_adjust_kernel<float, 8, 512, 4, 1> : logits_adjust_kernel<float, 4, 512, 2, 3>
-                      : few ? logits_adjust_kernel<uint16_t, 8, 512, 4, 1> : logits_adjust_kernel<uint16_t, 4, 512, 2, 3>;
-    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kernel, dim3(rows * blocks), dim3(512), 0, ctx->stream, p));
+    auto kernel = f32 ? few ? logits_adjust_kernel<float, 8, 512, 4, 2> : many ? logits_adjust_kernel<float, 4, 256, 4, 4> : logits_adjust_kernel<float, 4, 512, 2, 3>
+                  : few ? logits_adjust_kernel<uint16_t, 8, 512, 4, 2> : many ? logits_adjust_kernel<uint16_t, 4, 256, 4, 4> : logits_adjust_kernel<uint16_t, 4, 512, 2, 3>;
+    B2_CUDA(b2_launch_pdl(ctx->pdl_consumers, kernel, dim3(rows * blocks), dim3(many ? 256 : 512), 0, ctx->stream, p));
     B2_LAUNCHED(ctx);
     B2_CUDA(cudaGetLastError());
     return B2_OK;

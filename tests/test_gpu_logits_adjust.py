@@ -89,6 +89,13 @@ def test_all_rules(env, f32, rows, vocab, history, bias):
 
 
 @pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("rows, vocab, history, bias", [(40, 4099, 300, 20), (40, 170001, 700, 20), (150, 1003, 60, 9), (150, 40000, 900, 30)])
+def test_many_rows(env, f32, rows, vocab, history, bias):
+    rng, c = case(rows + vocab, rows, vocab, history, bias)
+    check(env, f32=f32, allowed=rng.random((rows, vocab)) < rng.choice([0.02, 0.5, 0.98], (rows, 1)), **c)
+
+
+@pytest.mark.parametrize("f32", [False, True])
 def test_vocabulary_of_several_rounds(env, f32):
     rng, c = case(5, 2, 420001, 5000, 400)
     check(env, f32=f32, allowed=rng.random((2, 420001)) < 0.5, **c)
