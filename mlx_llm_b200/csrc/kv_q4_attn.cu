@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         return p.out + ((size_t)row * p.hq + (size_t)kvh * group + (col - query * group)) * HD;
     };
 
-    Cursor use, ask;
+    Cursor use;
     int pos, end;
     {
         const int want = by_unit ? blockIdx.x : min(block_start + warp * run, total - 1);
@@ -292,33 +292,39 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         }
     }
     if (pos < end) {
-        ask = use;
+        // The records of a run are looked up 32 at a time, a lane each, whatever units they belong to, and a window ahead: a look into the
+        // block table is not waited for.
         const int begin = pos;
-        int asked = pos, window = -1, record = -1;  // lane i holds the record number of tile window + i of ask's unit, -1 for none
-        uint32_t absent = 0;                         // bit s: the record of stage s lies on a page outside of the pool
+        int asked = pos, look_seq = use.seq, look_at = (use.kvh * use.len.blocks + use.block) * use.len.tiles + use.tile;
+        uint32_t absent = 0;  // bit s: the record of stage s lies on a page outside of the pool
+        auto look = [&](int from) {  // record number of place from + lane of the run, -1 for none
+            int seq = look_seq, at = look_at + lane, record = -1;  // `at`: in the line of the sequence
+            if (from + lane < end) {
+                Lengths l = lengths_of(p, seq);
+                for (int all = l.tiles * l.blocks * p.hkv; at >= all; all = l.tiles * l.blocks * p.hkv) {
+                    at -= all;
+                    l = lengths_of(p, ++seq);
+                }
+                const int unit = at / l.tiles, tile = at - unit * l.tiles, index = tile / p.page_tiles;
+                const int page = p.block_tables[(size_t)(p.bt_rows ? p.bt_rows[seq] : seq) * p.max_blocks + index];
+                if (page >= 0 && page < p.n_pages) record = (page * p.hkv + unit / l.blocks) * p.page_tiles + tile - index * p.page_tiles;
+            }
+            look_seq = __shfl_sync(kFull, seq, 31), look_at = __shfl_sync(kFull, at, 31) + 1;
+            return record;
+        };
+        int record = look(begin), later = look(begin + 32);
         auto ask_until = [&](int upto) {
             for (; asked < upto; asked++) {
-                if (window < 0 || ask.tile - window >= 32) {
-                    window = ask.tile;
-                    const int tile = window + lane, index = tile / p.page_tiles;
-                    record = -1;
-                    if (tile < ask.len.tiles) {
-                        const int page = p.block_tables[(size_t)(p.bt_rows ? p.bt_rows[ask.seq] : ask.seq) * p.max_blocks + index];
-                        if (page >= 0 && page < p.n_pages) record = (page * p.hkv + ask.kvh) * p.page_tiles + tile - index * p.page_tiles;
-                    }
-                }
-                const int rec = __shfl_sync(kFull, record, ask.tile - window), stage = (asked - begin) % kStages;
+                const int i = asked - begin, stage = i % kStages;
+                if (i > 0 && i % 32 == 0) record = later, later = look(asked + 32);
+                const int rec = __shfl_sync(kFull, record, i % 32);
                 absent = (absent & ~(1u << stage)) | (rec < 0 ? 1u << stage : 0u);
                 if (rec >= 0) {
                     const uint8_t* src = p.pool + (size_t)rec * Rec::kBytes + lane * 16;
                     const uint32_t dst = ring + stage * Rec::kBytes + lane * 16;
 #pragma unroll
-                    for (int i = 0; i < kChunks; i += 32)
-                        if (i + 32 <= kChunks || i + lane < kChunks) cp_async16(dst + i * 16, src + i * 16);
-                }
-                if (++ask.tile == ask.len.tiles) {
-                    ask.next_unit(p);
-                    window = -1;
+                    for (int k = 0; k < kChunks; k += 32)
+                        if (k + 32 <= kChunks || k + lane < kChunks) cp_async16(dst + k * 16, src + k * 16);
                 }
             }
             cp_async_commit();
