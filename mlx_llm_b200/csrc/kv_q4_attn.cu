@@ -352,6 +352,21 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
             const int start = pos - t0;
             const int cols = min(8, use.len.columns - use.block * 8);
             if (!first_of_run) load_q();
+            if (pos + use.len.tiles - use.tile < end) {  // the next unit's queries, into L1, where its columns begin in this sequence or the next one
+                int seq = use.seq, kvh = use.kvh, block = use.block + 1;
+                if (block == use.len.blocks) block = 0, kvh++;
+                if (kvh == p.hkv) kvh = 0, seq++;
+                if (seq == use.seq || (!p.q_rows && seq < p.num_seqs)) {
+                    constexpr int kLines = HD / 64;
+                    const int col = block * 8 + lane / kLines, query = col / group;
+                    if (lane < (kNarrow ? 4 : 8) * kLines && col < use.len.columns) {
+                        const size_t row = (p.q_rows ? p.q_rows[seq] : seq) + query;
+                        const uint16_t* q = p.q + (row * p.hq + (size_t)kvh * group + (col - query * group)) * HD + lane % kLines * 64;
+                        uint32_t x;
+                        asm volatile("ld.global.ca.u32 %0, [%1];\n" : "=r"(x) : "l"(q));
+                    }
+                }
+            }
             // keys that columns 2c and 2c + 1 see; all columns see those before `sure`
             int lim0 = use.len.ctx, lim1 = lim0, sure = lim0;
             if (p.q_lens) {
