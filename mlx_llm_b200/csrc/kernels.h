@@ -240,8 +240,7 @@ struct Q4AttnParams {
     int* counters;
 };
 int32_t b2_kv_q4_attn_launch(b2_ctx* ctx, const Q4AttnParams& p, int head_dim);
-// Any number of query tokens per sequence, lengths known on the host: a plan (integers that have to be on the device before the launch,
-// `at` says where each list begins), made once for all layers of a step.
+// Any number of query tokens per sequence, lengths known on the host: a plan, integers that have to be on the device before the launch.
 struct Q4Seq {
     int32_t bt_row, q_row, q_len, ctx;  // block-table row, first query row, query tokens (the last ones of the context), tokens in the cache
 };

@@ -767,6 +767,7 @@ extern "C" int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, 
         B2_REQUIRE(cu_seqlens_host[i] >= 0 && n >= 0 && ctx_len >= n, B2_ERR_MSG, "b2_paged_attn_prefill_q4: ctx_lens must include the new tokens, and cu_seqlens ascend");
         B2_REQUIRE(((int64_t)ctx_len + page_size - 1) / page_size <= max_blocks, B2_ERR_MSG,
                    "b2_paged_attn_prefill_q4: a context needs more blocks than a block-table row holds");
+        B2_REQUIRE(ctx_len <= 0x7fffff00, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: a context of more than 2^31 - 256 tokens");
         seqs.push_back(Q4Seq{i, cu_seqlens_host[i], n, ctx_len});
     }
     B2_CUDA(cudaSetDevice(ctx->device));

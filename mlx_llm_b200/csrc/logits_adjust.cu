@@ -322,6 +322,7 @@ extern "C" int32_t b2_logits_adjust(b2_ctx* ctx, const void* logits_dev, int32_t
     B2_REQUIRE(!rules->history_dev || rules->history_off_dev, B2_ERR_MSG, "b2_logits_adjust: a history needs its rows' offsets");
     B2_REQUIRE(!rules->bias_id_dev || (rules->bias_off_dev && rules->bias_value_dev), B2_ERR_MSG, "b2_logits_adjust: biases need their values and their rows' offsets");
     B2_REQUIRE(!rules->mask_dev || rules->mask_words >= ((int64_t)vocab + 31) / 32, B2_ERR_MSG, "b2_logits_adjust: a mask's row must hold a bit for every token");
+    B2_REQUIRE(vocab <= 1 << 30, B2_ERR_UNSUPPORTED, "b2_logits_adjust: a vocabulary of more than 2^30 tokens");
     const uintptr_t size = f32 ? 4 : 2;
     B2_REQUIRE((uintptr_t)logits_dev % size == 0 && (uintptr_t)out_dev % size == 0, B2_ERR_UNSUPPORTED, "b2_logits_adjust: logits and out must be aligned to their elements");
     B2_CUDA(cudaSetDevice(ctx->device));

@@ -514,3 +514,80 @@ def test_prefill_keeps_a_bad_token_from_earlier_queries(env, hd, what, new, cach
     check_rows(got[:before], q[:before], cache, 0, 0.1, many=new * hq // hkv > 32)
     got = H.bf16_to_f32_np(got[before:])
     assert np.isnan(got[:, :2, :64]).all() and np.isfinite(got[:, 2:]).all()
+
+
+# ---- calls next to one another, and caches past 32 bits -------------------------------------------------------------------
+def test_pool_past_four_gigabytes(env):
+    """Pages whose bytes lie beyond 2^32: what is appended there is what attention reads, by single tokens, few and many."""
+    ctx, K = env
+    hq, hkv, hd, page, n = 8, 1, 128, 16, 700
+    pages = (1 << 21) + 64
+    pool = ctx.empty((K.kv_q4_pool_bytes(pages, hkv, hd, page),), np.uint8)
+    assert pool.nbytes > 1 << 32
+    tables = (pages - 1 - np.arange(44, dtype=np.int32))[None]
+    pos = np.arange(n, dtype=np.int32)
+    slots = (tables[0, pos // page] * page + pos % page).astype(np.int32)
+    rng = np.random.default_rng(8)
+    qkv = O.bf16(rng.standard_normal((n, hq + 2 * hkv, hd)))
+    cos, sin = O.bf16(np.ones((n, hd // 2))), O.bf16(np.zeros((n, hd // 2)))
+    q, k, v = ctx.empty((n, hq, hd), np.uint16), ctx.empty((n, hkv, hd), np.uint16), ctx.empty((n, hkv, hd), np.uint16)
+    K.rope_kv_append_q4(ctx, ctx.buf(as_bf16(qkv)), n, hq, hkv, hd, ctx.buf(pos), ctx.buf(slots), ctx.buf(as_bf16(cos)), ctx.buf(as_bf16(sin)), None, None, 1e-6,
+                        page, pool, pages, q, k, v)
+    ctx.sync()
+    cache = Cache.__new__(Cache)
+    cache.pool, cache.pages, cache.max_blocks, cache.dev_tables = pool, pages, 44, ctx.buf(tables)
+    cache.k, cache.v = ([H.bf16_to_f32_np(x.download()).astype(np.float64).transpose(1, 0, 2)] for x in (k, v))
+    rows = qkv[:, :hq]
+    check_rows(run_decode(env, cache, [n], rows[-1:], hq, hkv, hd, page, 0.1), rows[-1:], cache, 0, 0.1)
+    for new in (3, n):
+        out = ctx.empty((new, hq, hd), np.uint16)
+        K.paged_attn_prefill_q4(ctx, ctx.buf(as_bf16(rows[-new:])), pool, pages, cache.dev_tables, 44, [0, new], [n], hq, hkv, hd, page, 0.1, out)
+        ctx.sync()
+        check_rows(out.download(), rows[-new:], cache, 0, 0.1, many=True)
+        out.free()
+    pool.free()
+
+
+def attention_calls(env, ctx):
+    """Calls of every kind and size on `ctx`, and where their results are."""
+    _, K = env
+    calls = []
+    for seed, lengths, new in ((1, [700], None), (2, [3000, 5, 900, 64], None), (3, [16] * 20, None), (4, [900, 33], [200, 33]), (5, [2500], [300]),
+                               (6, [400, 40, 1500], [2, 1, 4])):
+        cache = Cache((ctx, K), seed, lengths, 2, 128, 16)
+        cu = None if new is None else np.concatenate([[0], np.cumsum(new)])
+        q = ctx.buf(as_bf16(queries(seed, len(lengths) if new is None else int(cu[-1]), 8, 128)))
+        out, n = ctx.empty(q.shape, np.uint16), ctx.buf(np.asarray(lengths, np.int32))
+        if new is None:
+            calls.append((out, lambda q=q, c=cache, n=n, l=lengths, o=out: K.paged_attn_decode_q4(ctx, q, c.pool, c.pages, c.dev_tables, n, len(l), 8, 2, 128, 16,
+                                                                                                  0.1, o, c.max_blocks)))
+        else:
+            calls.append((out, lambda q=q, c=cache, u=cu, l=lengths, o=out: K.paged_attn_prefill_q4(ctx, q, c.pool, c.pages, c.dev_tables, c.max_blocks, u, l, 8, 2,
+                                                                                                    128, 16, 0.1, o)))
+    return calls
+
+
+def test_calls_one_after_the_other_and_two_contexts_at_once(env):
+    from mlx_llm_b200 import _lib
+
+    ctx, _ = env
+    other = _lib.Context(0)
+    try:
+        here, there = attention_calls(env, ctx), attention_calls(env, other)
+        alone = []
+        for out, call in here:
+            call()
+            ctx.sync()
+            alone.append(out.download())
+        for _ in range(5):
+            for out, _ in here + there:
+                out.upload(np.full(out.shape, 0x7FC1, np.uint16))
+            for i in np.random.default_rng(3).permutation(len(here) * 4) % len(here):  # nothing waits in between
+                here[i][1]()
+                there[len(here) - 1 - i][1]()
+            ctx.sync()
+            other.sync()
+            for i, want in enumerate(alone):
+                assert np.array_equal(here[i][0].download(), want) and np.array_equal(there[i][0].download(), want)
+    finally:
+        other.close()

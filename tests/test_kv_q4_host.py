@@ -62,7 +62,7 @@ def test_pool_and_heads(kernels, call, bad, code):
     (decode, dict(out=AT + 4), -5), (decode, dict(n=1 << 20, blocks=1 << 12), -5),
     (decode, dict(scale=0.0), -7), (decode, dict(scale=float("nan")), -7), (prefill, dict(scale=-1.0), -7), (prefill, dict(scale=float("inf")), -7),
     (prefill, dict(q=None), -7), (prefill, dict(cu=(0, 2)), -7), (prefill, dict(cu=(3, 1), ctx=(9,)), -7), (prefill, dict(cu=(-1, 1), ctx=(9,)), -7),
-    (prefill, dict(ctx=(65,)), -7), (prefill, dict(out=AT + 8), -5),
+    (prefill, dict(ctx=(65,)), -7), (prefill, dict(out=AT + 8), -5), (prefill, dict(ctx=(0x7fffff01,), blocks=1 << 27), -5),
 ])
 def test_arguments(kernels, call, bad, code):
     refused(lambda: call(kernels, **bad), code)
@@ -75,7 +75,7 @@ def test_calls_without_work(kernels):
 @pytest.mark.parametrize("rules, kw, code", [
     ({}, dict(logits=None), -7), ({}, dict(argmax=None), -7), ({}, dict(vocab=0), -7), ({}, dict(rows=-1), -7), ({}, dict(ld=63), -7),
     (dict(history=AT), {}, -7), (dict(bias_id=AT, bias_off=AT), {}, -7), (dict(bias_id=AT, bias_value=AT), {}, -7),
-    (dict(mask=AT, mask_words=1), {}, -7), ({}, dict(logits=AT + 1), -5), ({}, dict(logits=AT + 2, f32=True), -5), ({}, dict(out=AT + 1), -5),
+    (dict(mask=AT, mask_words=1), {}, -7), ({}, dict(vocab=(1 << 30) + 1, ld=1 << 31), -5), ({}, dict(logits=AT + 1), -5), ({}, dict(logits=AT + 2, f32=True), -5), ({}, dict(out=AT + 1), -5),
 ])
 def test_rules_on_logits(kernels, rules, kw, code):
     args = dict(dict(logits=AT, rows=1, vocab=64, argmax=AT), **kw)
