@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         }
     // few short units: each is a block's, and no block shares one with another.  Else equal runs.
     const bool by_unit = units <= (int)gridDim.x && longest <= kWarps * kUnitRun;
-    const int run = max(kMinRun, (total + (int)gridDim.x * kWarps - 1) / ((int)gridDim.x * kWarps));
+    const int run = max(min(kMinRun, longest), (total + (int)gridDim.x * kWarps - 1) / ((int)gridDim.x * kWarps));
     const int block_start = blockIdx.x * kWarps * run;
     if (by_unit ? blockIdx.x >= units : block_start >= total) return;
     const uint32_t ring = smem_u32(smem) + warp * kStages * Rec::kBytes;
