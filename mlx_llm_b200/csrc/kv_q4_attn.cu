@@ -6,7 +6,8 @@
 //   unit    = (sequence, kv head, block of 8 columns); a column is one (query token, q head of the group).  Its work is the sequence's
 //             16-token records.
 //   split   = all units' records form one line, which is cut into equal runs, one per warp: every warp streams the same number of
-//             records whatever the lengths of the sequences, and no warp of a block waits for another before its run is done.
+//             records whatever the lengths of the sequences, and no warp of a block waits for another before its run is done.  Short
+//             units of much the same length have 1, 2, 4 or 8 warps of a block to themselves instead, and no blocks share one.
 //             A unit inside one run is written out at once.  Runs that share a unit leave (maximum, sum, unnormalised output): first
 //             in shared memory, where the block adds up its warps', then in global memory, where the block that arrives last adds up
 //             the blocks', both in the order of the line, so that results do not depend on timing.
@@ -31,7 +32,9 @@ constexpr int kEntries = 512;        // entries of the line's index in shared me
 constexpr float kFloor = -1e30f;     // reference of a column that has seen nothing: exp2(-inf - floor) is 0
 constexpr float kSlack = 8.f;
 constexpr int kMinRun = 4;           // records of a run at least
-constexpr int kUnitRun = 8;          // ... and at most, where a block has a unit of its own
+// Where units have warps to themselves: the records that the longest may have beyond an equal run, and the longest such run.  64 sequences
+// of 16-128 tokens 10.9 us (equal runs: 19.0), of 128 11.1 (13.6), of 512 18.1 (21.1), of 1024 27.4 (29.0), of 2048 47.7 (47.0).
+constexpr int kUnitSlack = 8, kUnitRun = 20;
 constexpr int kBlocksPerSm = 2;
 
 template <int HD>
@@ -240,11 +243,14 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
             const int n = (p.q_lens ? p.q_lens[s] : 1) * p.hq * HD;
             for (int e = threadIdx.x; e < n; e += kThreads) p.out[row * p.hq * HD + e] = 0;
         }
-    // few short units: each is a block's, and no block shares one with another.  Else equal runs.
-    const bool by_unit = units <= (int)gridDim.x && longest <= kWarps * kUnitRun;
-    const int run = max(min(kMinRun, longest), (total + (int)gridDim.x * kWarps - 1) / ((int)gridDim.x * kWarps));
+    const int warps = (int)gridDim.x * kWarps, run = max(min(kMinRun, longest), (total + warps - 1) / warps);
+    // Units of much the same length, as many as there are warps or fewer: each has `team` warps of a block to itself, and no block shares one
+    // with another.  Else equal runs.
+    int team = kWarps;
+    while (team > 1 && units > warps / team) team >>= 1;
+    const bool by_unit = units <= warps / team && run <= kUnitRun && (longest + team - 1) / team <= run + kUnitSlack;
     const int block_start = blockIdx.x * kWarps * run;
-    if (by_unit ? blockIdx.x >= units : block_start >= total) return;
+    if (by_unit ? blockIdx.x * (kWarps / team) >= units : block_start >= total) return;
     const uint32_t ring = smem_u32(smem) + warp * kStages * Rec::kBytes;
     float4* const parts = reinterpret_cast<float4*>(smem + ring_bytes<HD>());
     const float to_log2 = p.scale_log2 * q4::kUnscale;
@@ -259,7 +265,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     Cursor use;
     int pos, end;
     {
-        const int want = by_unit ? blockIdx.x : min(block_start + warp * run, total - 1);
+        const int want = by_unit ? min((int)blockIdx.x * (kWarps / team) + warp / team, units - 1) : min(block_start + warp * run, total - 1);
         const int* first = by_unit ? s_unit : s_off;
         int lo = 0, hi = p.entries - 1;  // the last entry that begins at or before it; of equal ones all but the last are empty
         while (lo < hi) {
@@ -279,10 +285,10 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         }
         if (by_unit) {
             use.at_unit(left);
-            const int each = (use.len.tiles + kWarps - 1) / kWarps;
-            use.tile = min(warp * each, use.len.tiles);
-            pos = use.tile;  // (the unit's own line)
-            end = min(pos + each, use.len.tiles);
+            const int each = (use.len.tiles + team - 1) / team, line = warp / team * longest;  // (every unit of the block has a line of its own)
+            use.tile = min(warp % team * each, use.len.tiles);
+            pos = line + use.tile;
+            end = (int)blockIdx.x * (kWarps / team) + warp / team < units ? line + min(use.tile + each, use.len.tiles) : pos;
         } else {
             const int unit = left / use.len.tiles;
             use.tile = left - unit * use.len.tiles;
