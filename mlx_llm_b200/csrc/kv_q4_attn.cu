@@ -31,10 +31,12 @@ constexpr int kStages = 4;             // records of a warp in shared memory: th
 constexpr int kEntries = 512;        // entries of the line's index in shared memory; each covers num_seqs / kEntries sequences
 constexpr float kFloor = -1e30f;     // reference of a column that has seen nothing: exp2(-inf - floor) is 0
 constexpr float kSlack = 8.f;
-constexpr int kMinRun = 4;           // records of a run at least
+constexpr int kMinRun = 4;           // records of a run at least (one sequence of 4000: 18.0 us, 2 records 18.1, 8 records 20.3)
 // Where units have warps to themselves: the records that the longest may have beyond an equal run, and the longest such run.  64 sequences
 // of 16-128 tokens 10.9 us (equal runs: 19.0), of 128 11.1 (13.6), of 512 18.1 (21.1), of 1024 27.4 (29.0), of 2048 47.7 (47.0).
-constexpr int kUnitSlack = 8, kUnitRun = 20;
+// Less of it where a unit would have a whole block, which is where warps are not short of units: 8 sequences of 1500 17.1 us (21.0 with 8),
+// 32 of 50-1000 17.0 (18.1 with 3).
+constexpr int kUnitSlack = 8, kBlockSlack = 4, kUnitRun = 20;
 constexpr int kBlocksPerSm = 2;
 
 template <int HD>
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     // with another.  Else equal runs.
     int team = kWarps;
     while (team > 1 && units > warps / team) team >>= 1;
-    const bool by_unit = units <= warps / team && run <= kUnitRun && (longest + team - 1) / team <= run + kUnitSlack;
+    const bool by_unit = units <= warps / team && run <= kUnitRun && (longest + team - 1) / team <= run + (team == kWarps ? kBlockSlack : kUnitSlack);
     const int block_start = blockIdx.x * kWarps * run;
     if (by_unit ? blockIdx.x * (kWarps / team) >= units : block_start >= total) return;
     const uint32_t ring = smem_u32(smem) + warp * kStages * Rec::kBytes;
