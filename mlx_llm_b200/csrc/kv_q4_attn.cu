@@ -248,11 +248,14 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     const int warps = (int)gridDim.x * kWarps, run = max(min(kMinRun, longest), (total + warps - 1) / warps);
     // Units of much the same length, as many as there are warps or fewer: each has `team` warps of a block to itself, and no block shares one
     // with another.  Else equal runs.
-    int team = kWarps;
-    while (team > 1 && units > warps / team) team >>= 1;
-    const bool by_unit = units <= warps / team && run <= kUnitRun && (longest + team - 1) / team <= run + (team == kWarps ? kBlockSlack : kUnitSlack);
+    int team_log2 = 3;
+    static_assert(kWarps == 8, "a team is 1, 2, 4 or 8 of a block's warps");
+    while (team_log2 > 0 && units > warps >> team_log2) team_log2--;
+    const int team = 1 << team_log2, block_units = kWarps >> team_log2;
+    const bool by_unit = units <= warps >> team_log2 && run <= kUnitRun &&
+                         (longest + team - 1) >> team_log2 <= run + (team == kWarps ? kBlockSlack : kUnitSlack);
     const int block_start = blockIdx.x * kWarps * run;
-    if (by_unit ? blockIdx.x * (kWarps / team) >= units : block_start >= total) return;
+    if (by_unit ? (int)blockIdx.x * block_units >= units : block_start >= total) return;
     const uint32_t ring = smem_u32(smem) + warp * kStages * Rec::kBytes;
     float4* const parts = reinterpret_cast<float4*>(smem + ring_bytes<HD>());
     const float to_log2 = p.scale_log2 * q4::kUnscale;
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     Cursor use;
     int pos, end;
     {
-        const int want = by_unit ? min((int)blockIdx.x * (kWarps / team) + warp / team, units - 1) : min(block_start + warp * run, total - 1);
+        const int want = by_unit ? min((int)blockIdx.x * block_units + (warp >> team_log2), units - 1) : min(block_start + warp * run, total - 1);
         const int* first = by_unit ? s_unit : s_off;
         int lo = 0, hi = p.entries - 1;  // the last entry that begins at or before it; of equal ones all but the last are empty
         while (lo < hi) {
@@ -287,10 +290,10 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         }
         if (by_unit) {
             use.at_unit(left);
-            const int each = (use.len.tiles + team - 1) / team, line = warp / team * longest;  // (every unit of the block has a line of its own)
-            use.tile = min(warp % team * each, use.len.tiles);
+            const int each = (use.len.tiles + team - 1) >> team_log2, line = (warp >> team_log2) * longest;  // (a line for every unit of the block)
+            use.tile = min((warp & (team - 1)) * each, use.len.tiles);
             pos = line + use.tile;
-            end = (int)blockIdx.x * (kWarps / team) + warp / team < units ? line + min(use.tile + each, use.len.tiles) : pos;
+            end = (int)blockIdx.x * block_units + (warp >> team_log2) < units ? line + min(use.tile + each, use.len.tiles) : pos;
         } else {
             const int unit = left / use.len.tiles;
             use.tile = left - unit * use.len.tiles;
@@ -303,11 +306,11 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
         // The records of a run are looked up 32 at a time, a lane each, whatever units they belong to, and a window ahead: a look into the
         // block table is not waited for.
         const int begin = pos;
-        int asked = pos, look_seq = use.seq, look_at = (use.kvh * use.len.blocks + use.block) * use.len.tiles + use.tile;
+        int asked = pos, look_from = pos, look_seq = use.seq, look_at = (use.kvh * use.len.blocks + use.block) * use.len.tiles + use.tile;
         uint32_t absent = 0;  // bit s: the record of stage s lies on a page outside of the pool
-        auto look = [&](int from) {  // record number of place from + lane of the run, -1 for none
+        auto look = [&] {  // record number of place look_from + lane, -1 for none
             int seq = look_seq, at = look_at + lane, record = -1;  // `at`: in the line of the sequence
-            if (from + lane < end) {
+            if (look_from + lane < end) {
                 Lengths l = lengths_of(p, seq);
                 for (int all = l.tiles * l.blocks * p.hkv; at >= all; all = l.tiles * l.blocks * p.hkv) {
                     at -= all;
@@ -317,14 +320,15 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
                 const int page = p.block_tables[(size_t)(p.bt_rows ? p.bt_rows[seq] : seq) * p.max_blocks + index];
                 if (page >= 0 && page < p.n_pages) record = (page * p.hkv + unit / l.blocks) * p.page_tiles + tile - index * p.page_tiles;
             }
-            look_seq = __shfl_sync(kFull, seq, 31), look_at = __shfl_sync(kFull, at, 31) + 1;
+            look_seq = __shfl_sync(kFull, seq, 31), look_at = __shfl_sync(kFull, at, 31) + 1, look_from += 32;
             return record;
         };
-        int record = look(begin), later = look(begin + 32);
+        int record = look(), later = -1;
         auto ask_until = [&](int upto) {
             for (; asked < upto; asked++) {
                 const int i = asked - begin, stage = i % kStages;
-                if (i > 0 && i % 32 == 0) record = later, later = look(asked + 32);
+                if (i > 0 && i % 32 == 0) record = later;
+                if (i % 32 == kStages && look_from < end) later = look();
                 const int rec = __shfl_sync(kFull, record, i % 32);
                 absent = (absent & ~(1u << stage)) | (rec < 0 ? 1u << stage : 0u);
                 if (rec >= 0) {
