@@ -235,7 +235,7 @@ struct Q4AttnParams {
     float scale_log2;             // softmax scale * log2(e)
     uint16_t* out;                // [rows, hq, hd] bf16
     // filled in by the launch
-    int group, max_ctx, entries, per_entry;
+    int group, max_ctx;
     float* parts;
     int* counters;
 };

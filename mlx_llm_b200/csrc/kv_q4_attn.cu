@@ -28,7 +28,6 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 8;
 constexpr int kStages = 4;             // records of a warp in shared memory: the two that it works on, the two that are on their way
-constexpr int kEntries = 512;        // entries of the line's index in shared memory; each covers num_seqs / kEntries sequences
 constexpr float kFloor = -1e30f;     // reference of a column that has seen nothing: exp2(-inf - floor) is 0
 constexpr float kSlack = 8.f;
 constexpr int kMinRun = 4;           // records of a run at least (one sequence of 4000: 18.0 us, 2 records 18.1, 8 records 20.3)
@@ -195,8 +194,6 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     constexpr int kChunks = Rec::kBytes / 16;
     constexpr int kThreads = kWarps * 32, kParts = 2 * kWarps;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int s_off[kEntries + 1], s_unit[kEntries + 1];  // first record, first unit of every entry
-    __shared__ int4 s_scan[kWarps];
     __shared__ Part s_part[kParts];
     __shared__ float s_m[kParts][8], s_l[kParts][8], s_weight[kParts][8], s_sum[kParts][8], s_max[kParts][8];
     __shared__ int s_last[2];
@@ -205,12 +202,17 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int group = p.group;
 
-    // the line: first record and unit of every entry, the longest unit, and whether there are empty contexts
-    int total = 0, units = 0, longest = 0, empty = 0;
-    for (int base = 0; base < p.entries; base += kThreads) {
-        const int e = base + threadIdx.x;
-        int n = 0, u = 0, most = 0, none = 0;
-        for (int s = e * p.per_entry; s < min(p.num_seqs, (e + 1) * p.per_entry); s++) {
+    if (lane < 2) s_part[2 * warp + lane].tiles = 0;
+    // Where this warp's run begins.  Every warp finds out for itself, without waiting for others: its lanes add up what 1/32 of the sequences
+    // have each, and then the same of the lane that holds the place, until that is one sequence.
+    int run = 0, team_log2 = 0, team = 1, block_units = kWarps, block_start = 0, longest = 0, total = 0, units = 0;
+    bool by_unit = false;
+    int lo = 0, span = p.num_seqs, left = 0;  // sequences that hold the place, and the place among theirs
+    for (bool all = true;; all = false) {
+        const int per = (span + 31) >> 5, from = lo + lane * per;
+        int n = 0, u = 0, most = 0, none = 0;  // records, units, the longest unit, an empty context
+#pragma unroll 1
+        for (int s = from; s < min(from + per, lo + span); s++) {
             const Lengths l = lengths_of(p, s);
             u += l.blocks * p.hkv;
             n += l.tiles * l.blocks * p.hkv;
@@ -223,39 +225,38 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
             const int a = __shfl_up_sync(kFull, ni, o), b = __shfl_up_sync(kFull, ui, o);
             if (lane >= o) ni += a, ui += b;
         }
-        most = __reduce_max_sync(kFull, most);
-        none = __any_sync(kFull, none);
-        if (lane == 31) s_scan[warp] = make_int4(ni, ui, most, none);
-        if (base == 0 && threadIdx.x < kParts) s_part[threadIdx.x].tiles = 0;
-        __syncthreads();
-        int nb = total, ub = units;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            const int4 v = s_scan[w];
-            if (w < warp) nb += v.x, ub += v.y;
-            total += v.x, units += v.y, longest = max(longest, v.z), empty |= v.w;
+        if (all) {
+            total = __shfl_sync(kFull, ni, 31), units = __shfl_sync(kFull, ui, 31), longest = __reduce_max_sync(kFull, most);
+            if (__builtin_expect(__any_sync(kFull, none), 0))  // an empty context attends to nothing: rows of zeros
+#pragma unroll 1
+                for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
+                    if (lengths_of(p, s).tiles > 0) continue;
+                    const size_t row = p.q_rows ? p.q_rows[s] : s;
+                    const int count = (p.q_lens ? p.q_lens[s] : 1) * p.hq * HD;
+#pragma unroll 1
+                    for (int e = threadIdx.x; e < count; e += kThreads) p.out[row * p.hq * HD + e] = 0;
+                }
+            // Units of much the same length, as many as there are warps or fewer: each has a team of warps of a block to itself, and no block
+            // shares one with another.  Else equal runs.
+            const int warps = (int)gridDim.x * kWarps;
+            run = max(min(kMinRun, longest), (total + warps - 1) / warps);
+            team_log2 = 3;
+            static_assert(kWarps == 8, "a team is 1, 2, 4 or 8 of a block's warps");
+#pragma unroll 1
+            while (team_log2 > 0 && units > warps >> team_log2) team_log2--;
+            team = 1 << team_log2, block_units = kWarps >> team_log2;
+            by_unit = units <= warps >> team_log2 && run <= kUnitRun &&
+                      (longest + team - 1) >> team_log2 <= run + (team == kWarps ? kBlockSlack : kUnitSlack);
+            block_start = blockIdx.x * kWarps * run;
+            if (by_unit ? (int)blockIdx.x * block_units >= units : block_start >= total) return;
+            left = by_unit ? min((int)blockIdx.x * block_units + (warp >> team_log2), units - 1) : min(block_start + warp * run, total - 1);
         }
-        if (e < p.entries) s_off[e] = nb + ni - n, s_unit[e] = ub + ui - u;
-        __syncthreads();
+        const int size = by_unit ? u : n, before = (by_unit ? ui : ni) - size;
+        const int owner = __ffs(__ballot_sync(kFull, left >= before && left - before < size)) - 1;
+        left -= __shfl_sync(kFull, before, owner);
+        lo += owner * per, span = min(per, span - owner * per);
+        if (per == 1) break;
     }
-    if (empty)  // an empty context attends to nothing: rows of zeros
-        for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
-            if (lengths_of(p, s).tiles > 0) continue;
-            const size_t row = p.q_rows ? p.q_rows[s] : s;
-            const int n = (p.q_lens ? p.q_lens[s] : 1) * p.hq * HD;
-            for (int e = threadIdx.x; e < n; e += kThreads) p.out[row * p.hq * HD + e] = 0;
-        }
-    const int warps = (int)gridDim.x * kWarps, run = max(min(kMinRun, longest), (total + warps - 1) / warps);
-    // Units of much the same length, as many as there are warps or fewer: each has `team` warps of a block to itself, and no block shares one
-    // with another.  Else equal runs.
-    int team_log2 = 3;
-    static_assert(kWarps == 8, "a team is 1, 2, 4 or 8 of a block's warps");
-    while (team_log2 > 0 && units > warps >> team_log2) team_log2--;
-    const int team = 1 << team_log2, block_units = kWarps >> team_log2;
-    const bool by_unit = units <= warps >> team_log2 && run <= kUnitRun &&
-                         (longest + team - 1) >> team_log2 <= run + (team == kWarps ? kBlockSlack : kUnitSlack);
-    const int block_start = blockIdx.x * kWarps * run;
-    if (by_unit ? (int)blockIdx.x * block_units >= units : block_start >= total) return;
     const uint32_t ring = smem_u32(smem) + warp * kStages * Rec::kBytes;
     float4* const parts = reinterpret_cast<float4*>(smem + ring_bytes<HD>());
     const float to_log2 = p.scale_log2 * q4::kUnscale;
@@ -270,24 +271,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     Cursor use;
     int pos, end;
     {
-        const int want = by_unit ? min((int)blockIdx.x * block_units + (warp >> team_log2), units - 1) : min(block_start + warp * run, total - 1);
-        const int* first = by_unit ? s_unit : s_off;
-        int lo = 0, hi = p.entries - 1;  // the last entry that begins at or before it; of equal ones all but the last are empty
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (first[mid] <= want)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
-        int left = want - first[lo];
-        use.at_seq(p, lo * p.per_entry);
-        while (true) {  // (sequences of the entry)
-            const int all = (by_unit ? 1 : use.len.tiles) * use.len.blocks * p.hkv;
-            if (left < all) break;
-            left -= all;
-            use.at_seq(p, use.seq + 1);
-        }
+        use.at_seq(p, lo);
         if (by_unit) {
             use.at_unit(left);
             const int each = (use.len.tiles + team - 1) >> team_log2, line = (warp >> team_log2) * longest;  // (a line for every unit of the block)
@@ -626,8 +610,6 @@ int32_t launch(b2_ctx* ctx, Q4AttnParams p) {
     }
     p.group = p.hq / p.hkv;
     p.max_ctx = (int)std::min<int64_t>((int64_t)p.max_blocks * p.page_tiles * 16, 0x7ffffff0);
-    p.per_entry = (p.num_seqs + kEntries - 1) / kEntries;
-    p.entries = (p.num_seqs + p.per_entry - 1) / p.per_entry;
     p.parts = ctx->q4_parts;
     p.counters = reinterpret_cast<int*>(ctx->q4_parts + (size_t)grid * 2 * part_floats<128>());
     const auto kernel = kv_q4_attn_kernel<HD, kNarrow>;
