@@ -94,6 +94,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, kPer
     auto take = [&](float ov, int oi) {
         if (ov > best || (ov == best && oi < bi)) best = ov, bi = oi;
     };
+#pragma unroll 1
     for (int base = 0; base < p.vocab; base += kBlocks * p.slice) {
         const int first = base + block * p.slice, n = max(0, min(p.slice, p.vocab - first));  // this block's tokens
         const int whole = vec ? n / V * V : 0;
@@ -123,6 +124,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, kPer
         auto each_seen = [&](auto f) {
 #pragma unroll
             for (int k = 0; k < kAhead; k++) in_slice(head[k], h0 + tid + k * kThreads, f);
+#pragma unroll 1
             for (int i = h0 + tid + kAhead * kThreads; i < h1; i += 4 * kThreads) {
                 int id[4];
 #pragma unroll
@@ -132,10 +134,12 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, kPer
             }
         };
         auto each_bias = [&](auto f) {
+#pragma unroll 1
             for (int i = b0 + tid; i < b1; i += kThreads) in_slice(r.bias_id_dev[i], i, f);
         };
         uint32_t total = 0;  // named tokens
         if (h1 > h0 || b1 > b0) {
+#pragma unroll 1
             for (int i = tid; i < p.slice / 32; i += kThreads) named[i] = 0;
             __syncthreads();
             auto mark = [&](uint32_t t, int) {  // (a look first: atomics on one word wait for one another, and favourites come in crowds)
@@ -202,6 +206,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, kPer
                 for (int j = 0; j < 4; j++) keep[j] = u[j];
             }
         };
+#pragma unroll 1
         for (int from = 0; from * V < whole; from += kAhead * kThreads) {
             if (from > 0) ask(from);
 #pragma unroll
@@ -210,6 +215,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, kPer
                 if (at < whole) piece(ahead[k], at, allow[k]);
             }
         }
+#pragma unroll 1
         for (int t = whole + tid; t < n; t += kThreads) {
             if (total && (named[t >> 5] >> (t & 31) & 1)) continue;
             const float v = allowed(first + t) ? Elt<T>::ld(in + first + t) : -INFINITY;
@@ -229,8 +235,10 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, kPer
             take(top, found);
         }
         // the named ones, kNamed at a time
+#pragma unroll 1
         for (uint32_t from = 0; from < total; from += kNamed) {
             const uint32_t kept = min((uint32_t)kNamed, total - from);
+#pragma unroll 1
             for (uint32_t i = tid; i < kept; i += kThreads) counts[i] = 0, biases[i] = 0.f;
             __syncthreads();
             auto rank = [&](uint32_t t) { return rank_of[t >> 5] + __popc(named[t >> 5] & ((1u << (t & 31)) - 1)) - from; };
@@ -250,6 +258,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads, kPer
                 if (i == b0 || r.bias_id_dev[i - 1] != r.bias_id_dev[i]) biases[at] = r.bias_value_dev[i];
             });
             __syncthreads();
+#pragma unroll 1
             for (uint32_t at = tid; at < kept; at += kThreads) {
                 const int i = first + ids[at];
                 float v = Elt<T>::ld(in + i);
