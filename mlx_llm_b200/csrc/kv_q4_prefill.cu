@@ -413,17 +413,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
                 tc_fence_after();
                 // The upper 64 scores are read for the maximum and, once the lower ones have become P, again: a thread has 128 registers.
                 const int key0 = (w.first_tile + j) * KT;
-                const bool masked = key0 + KT - 1 > sees;
+                if (__any_sync(0xffffffffu, key0 + KT - 1 > sees)) {  // in place, so that the code for other tiles is without it
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t v[32];
+                        tc_ld32(ts + c * 32u, v);
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (key0 + c * 32 + i > sees) v[i] = 0xff800000u;
+                        tc_st32(ts + c * 32u, v);
+                    }
+                }
                 uint32_t s[2][32];
                 auto read = [&](int half) {
 #pragma unroll
                     for (int c = 0; c < 2; c++) tc_ld32_nowait(ts + half * 64u + c * 32u, s[c]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < 64; i++)
-                            if (key0 + half * 64 + i > sees) s[i >> 5][i & 31] = 0xff800000u;
-                    }
                 };
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
