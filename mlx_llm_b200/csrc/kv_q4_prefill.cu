@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
                 }
                 const uint64_t sc = twice(p.scale_log2), neg = twice(-m);
                 uint64_t sum[2] = {0, 0};
-#pragma unroll
+#pragma unroll 1
                 for (int half = 0; half < 2; half++) {
                     if (half == 1) read(1);
 #pragma unroll
