@@ -38,19 +38,22 @@ __device__ __forceinline__ uint32_t tile_at(int row, int dim) {  // of 8 dims
 // A CTA fills an SM and goes through segments: two blocks of 128 query rows, a kv head, and tiles of their keys.  A row is a (query token,
 // q head of the group) pair, the heads of a token next to one another, so that a group shares every tile of K and V, and the two blocks share
 // them again.  The host, which knows all lengths, deals the segments out (b2_kv_q4_plan).  The warps that convert are at the next segment's
-// keys, and the other block at its products, while a block writes its rows out: three prompts of ~1049 took 65 us, with a CTA for each
-// segment 72.
+// keys, and the other block at its products, while a block writes its rows out: three prompts of ~1049 took 65 us (now 60), with a CTA for
+// each segment 72.
 //   warps 0-3, 4-7  softmax of block A, B: thread = row = TMEM lane.  exp2 against a running reference that is raised only when a tile exceeds
 //                   it by more than 2^8 (O is touched only then); P goes as bf16 over the scores' columns.
 //   warps 8-11      codes to operands: a warp has two of the eight records of a tile, reads the next tile's while it converts this one's, and
 //                   fills a ring of five tiles K0 V0 K1 V1 ...  K keeps the order that nibbles come out in, 0 4 1 5 2 6 3 7 of eight dims, and Q is
 //                   put in the same; both carry the conversion's 2^-64 (kv_q4.cuh), which the softmax scale and the division take back.
 //   warp 12         one thread issues S = Q K^T and O += P V with P from tensor memory, for A and B in turn: while one block's softmax runs,
-//                   the tensor cores have the other's products.  S(j + 1) of a block goes over P(j), which the in-order pipe has read by then;
-//                   and when S(j) is there, P V of j - 1 has completed, so O may be rescaled.
+//                   the tensor cores have the other's products.  P comes by halves of the keys, and the first half's product runs beside the
+//                   second half's exponentials.  S(j + 1) of a block goes over P(j), which the in-order pipe has read by then; and when S(j) is
+//                   there, P V of j - 1 has completed, so O may be rescaled.
 // Bound by a block's chain of product, softmax, product (two thirds of it are the tensor cores').  Converting in here costs each CTA what an
 // own kernel would do once per 128 keys, in warps that the chain leaves idle: 512 tokens behind 11800 that read bf16 tiles, made by such a
-// kernel, from L2 took 210 us instead of 234, but 64 tokens behind 12000 took 60 instead of 42, and eight sequences of 16 behind 1500 took 47 instead of 33.
+// kernel, from L2 took 210 us where this took 236, but 64 tokens behind 12000 took 60 instead of 45, and eight sequences of 16 behind 1500 took 47
+// instead of 33.  The three roles' code competes for the SM's instruction cache: loops that could be unrolled are not (512 behind 11800: masks in
+// place 234 -> 228 us, exponentials 222, the maximum and P by halves 218), but for the issuing thread's, whose latency counts (229).
 // A value that is NaN must reach the rows that see it and no others, but a row that does not still multiplies it, with zero: it goes into the
 // token's keys, whose scores are masked by choice and not by multiplication, and the value becomes zero.
 // P carries 8 bits (one rounding of each weight, relative 2^-9; their sum is taken before the rounding, whose errors have no sign of their
@@ -237,13 +240,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
     auto full = [&](int s) { return bar + 8u * s; };
     auto empty = [&](int s) { return bar + 8u * (5 + s); };
     auto s_ready = [&](int x) { return bar + 8u * (10 + x); };
-    auto p_ready = [&](int x) { return bar + 8u * (12 + x); };
-    auto q_full = [&](int x) { return bar + 8u * (14 + x); };   // once a segment: Q is there, and O of the last one has been read
-    auto o_ready = [&](int x) { return bar + 8u * (16 + x); };  // once a segment
-    const uint32_t gone = bar + 8u * 18, slot_addr = bar + 8u * 19;
+    auto p_ready = [&](int x, int half) { return bar + 8u * (12 + 2 * x + half); };
+    auto q_full = [&](int x) { return bar + 8u * (16 + x); };   // once a segment: Q is there, and O of the last one has been read
+    auto o_ready = [&](int x) { return bar + 8u * (18 + x); };  // once a segment
+    const uint32_t gone = bar + 8u * 20, slot_addr = bar + 8u * 21;
     if (tid == 0) {
         for (int s = 0; s < kSlots; s++) mbar_init(full(s), 4), mbar_init(empty(s), 1);
-        for (int x = 0; x < 2; x++) mbar_init(s_ready(x), 1), mbar_init(p_ready(x), 4), mbar_init(q_full(x), 4), mbar_init(o_ready(x), 1);
+        for (int x = 0; x < 2; x++) mbar_init(s_ready(x), 1), mbar_init(p_ready(x, 0), 4), mbar_init(p_ready(x, 1), 4), mbar_init(q_full(x), 4), mbar_init(o_ready(x), 1);
         mbar_init(gone, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -310,11 +313,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
                 }
                 tc_commit(s_ready(x));
             };
-            auto issue_o = [&](int x, int slot, uint32_t add) {  // O of block x
+            auto issue_o = [&](int x, int half, int slot, uint32_t add) {  // O of block x, by half of the keys
                 const uint32_t at = v_lo + slot * (TILE >> 4);
 #pragma unroll
-                for (int k = 0; k < KT / 16; k++)
+                for (int i = 0; i < KT / 32; i++) {
+                    const int k = half * (KT / 32) + i;
                     tc_mma_ts(tmem + 256u + x * 128u, tmem + x * 128u + k * 8u, two(at + k * (2048 >> 4), v_hi), idesc_pv<HD>(), k > 0 ? 1u : add);
+                }
             };
             int slot = 0;
             uint32_t parity = 0;
@@ -336,10 +341,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
                 advance();
                 for (int j = 0; j < n; j++, phase ^= 1u) {
                     const int v = slot;
-                    alive = mbar_wait(full(v), parity) && mbar_wait(p_ready(0), phase);
+                    alive = mbar_wait(full(v), parity) && mbar_wait(p_ready(0, 0), phase);
                     if (!alive) break;
                     tc_fence_after();
-                    issue_o(0, v, j > 0);
+                    issue_o(0, 0, v, j > 0);
+                    alive = mbar_wait(p_ready(0, 1), phase);
+                    if (!alive) break;
+                    tc_fence_after();
+                    issue_o(0, 1, v, 1);
                     advance();
                     const int k = slot;
                     if (j + 1 < n) {
@@ -350,10 +359,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
                     } else {
                         tc_commit(o_ready(0));
                     }
-                    alive = mbar_wait(p_ready(1), phase);
+                    alive = mbar_wait(p_ready(1, 0), phase);
                     if (!alive) break;
                     tc_fence_after();
-                    issue_o(1, v, j > 0);
+                    issue_o(1, 0, v, j > 0);
+                    alive = mbar_wait(p_ready(1, 1), phase);
+                    if (!alive) break;
+                    tc_fence_after();
+                    issue_o(1, 1, v, 1);
                     tc_commit(empty(v));
                     if (j + 1 < n) {
                         issue_s(1, k);
@@ -396,23 +409,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full(x));
         };
-        Segment w = p.segments[begin];
-        copy_q(w);
+        copy_q(p.segments[begin]);
         q_there();
         uint32_t phase = 0, seg_phase = 0;
         for (int segment = begin; segment < end; segment++, seg_phase ^= 1u) {
             // last key that the row sees; rows without a query see all (nothing comes of them)
-            const bool row_ok = in_block && query < w.queries;
-            const int sees = row_ok ? w.sees + query : 0x3fffffff;
+            const Segment* const work = p.segments + segment;
+            const int n = work->n_tiles, first_key = work->first_tile * KT, sees = in_block && query < work->queries ? work->sees + query : 0x3fffffff;
             float m = kFloor, l = 0.f;
-            for (int j = 0; j < w.n_tiles; j++, phase ^= 1u) {
+            for (int j = 0; j < n; j++, phase ^= 1u) {
                 if (!__all_sync(0xffffffffu, mbar_wait(s_ready(x), phase))) {
                     alive = false;
                     break;
                 }
                 tc_fence_after();
                 // The upper 64 scores are read for the maximum and, once the lower ones have become P, again: a thread has 128 registers.
-                const int key0 = (w.first_tile + j) * KT;
+                const int key0 = first_key + j * KT;
                 if (__any_sync(0xffffffffu, key0 + KT - 1 > sees)) {  // in place, so that the code for other tiles is without it
 #pragma unroll 1
                     for (int c = 0; c < 4; c++) {
@@ -431,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
                     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
                 };
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
+#pragma unroll 1
                 for (int half = 1; half >= 0; half--) {
                     read(half);
 #pragma unroll
@@ -476,24 +488,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
                         }
                         tc_st16_nowait(ts + (half * 2 + c) * 16u, h);
                     }
+                    asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready(x, half));
                 }
                 const uint64_t both = add2(sum[0], sum[1]);
                 l += low(both) + high(both);
-                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready(x));
             }
             if (!alive) break;
-            const size_t row = row_of(w);
-            const int part = w.part;
-            if (segment + 1 < end) {  // (all of this segment's scores are there, so its Q is not read any more)
-                w = p.segments[segment + 1];
-                copy_q(w);
-            }
+            if (segment + 1 < end) copy_q(work[1]);  // (all of this segment's scores are there, so its Q is not read any more)
             alive = __all_sync(0xffffffffu, mbar_wait(o_ready(x), seg_phase));
             if (!alive) break;
             tc_fence_after();
+            const bool row_ok = in_block && query < work->queries;
+            const size_t row = row_of(*work);
+            const int part = work->part;
             const float inv = l == 0.f ? 0.f : q4::kUnscale / l;
             const size_t at = (size_t)part * (2 * kRows) + x * kRows + r;
 #pragma unroll 1
