@@ -17,10 +17,11 @@ namespace {
 using namespace tc5;
 
 // Which of the two, for all sequences of a call, by what they cost in records x blocks of 8 columns.  Both kernels at work on 64 sequences
-// behind 2000 tokens, 4 q heads a kv head: 8 new tokens (~36 columns) 160 and 186 us, 16 new 300 and 189 us; so a tile of 128 keys counts
-// like 41.  The second kernel has ~6 us more of start and end (64 tokens behind 100: 14 and 21 us), and two kernels, one after the other,
-// cost the shorter one's latency (8 sequences of 4 to 12 new tokens behind 1500: 31 us with either kernel, 49 with both).
-constexpr double kTileCost = 41, kStartCost = 8e3, kBothCost = 2e4;
+// behind 2000 tokens, 4 q heads a kv head: 8 new tokens (~36 columns) 155 and 168 us, 16 new 292 and 172 us; so a tile of 128 keys counts
+// like 41.  The second kernel has 5 to 9 us more of start and end (32 tokens behind 1500: 20.7 and 28.8 us; but 16 behind 12000 42.0 and
+// 36.0), and two kernels, one after the other, cost the shorter one's latency (8 sequences of 4 to 12 new tokens behind 1500: 31 us with
+// either kernel, 49 with both, before both became faster).
+constexpr double kTileCost = 41, kStartCost = 1.4e4, kBothCost = 2e4;
 // In tiles (2.4 us): what a segment costs besides its tiles, what joining parts does, and the shortest run worth a CTA.
 constexpr double kSegmentCost = 2, kJoinCost = 4, kShortRun = 4;
 constexpr int KT = 128;  // keys of a tile

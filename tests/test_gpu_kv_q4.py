@@ -493,7 +493,7 @@ def test_prompt_then_tokens_then_choices(env, hd, hq, hkv):
 
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("what", ["key", "value"])
-@pytest.mark.parametrize("new, cached", [(3, 37), (60, 37), (400, 700)])
+@pytest.mark.parametrize("new, cached", [(3, 37), (60, 37), (400, 700), (900, 700)])
 def test_prefill_keeps_a_bad_token_from_earlier_queries(env, hd, what, new, cached):
     """A token whose key or value is NaN: queries before it are as if it were not there, those that see it are NaN."""
     ctx, K = env
