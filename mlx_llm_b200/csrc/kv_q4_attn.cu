@@ -196,6 +196,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     constexpr int kThreads = kWarps * 32, kParts = 2 * kWarps;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Part s_part[kParts];
+    __shared__ int4 s_scan[kWarps];
+    __shared__ int s_first[2][kThreads];  // records, units of the sequences before a thread's
     __shared__ float s_m[kParts][8], s_l[kParts][8], s_weight[kParts][8], s_sum[kParts][8], s_max[kParts][8];
     __shared__ int s_last[2];
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
@@ -204,53 +206,91 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
     const int group = p.group;
 
     if (lane < 2) s_part[2 * warp + lane].tiles = 0;
-    // Where this warp's run begins.  Every warp finds out for itself, without waiting for others: its lanes add up what 1/32 of the sequences
-    // have each, and then the same of the lane that holds the place, until that is one sequence.
     int run = 0, team_log2 = 0, team = 1, block_units = kWarps, block_start = 0, longest = 0, total = 0, units = 0;
     bool by_unit = false;
-    int lo = 0, span = p.num_seqs, left = 0;  // sequences that hold the place, and the place among theirs
-    for (bool all = true;; all = false) {
-        const int per = (span + 31) >> 5, from = lo + lane * per;
-        int n = 0, u = 0, most = 0, none = 0;  // records, units, the longest unit, an empty context
+    int lo = 0, span = p.num_seqs, left = 0;  // sequences that hold the place where this warp's run begins, and the place among theirs
+    auto add_up = [&](int from, int to, int& n, int& u, int& most, int& none) {  // records, units, the longest unit, an empty context
 #pragma unroll 1
-        for (int s = from; s < min(from + per, lo + span); s++) {
+        for (int s = from; s < to; s++) {
             const Lengths l = lengths_of(p, s);
             u += l.blocks * p.hkv;
             n += l.tiles * l.blocks * p.hkv;
             most = max(most, l.tiles);
             none |= l.tiles == 0;
         }
-        int ni = n, ui = u;
+    };
+    auto scan = [&](int& n, int& u) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int a = __shfl_up_sync(kFull, ni, o), b = __shfl_up_sync(kFull, ui, o);
-            if (lane >= o) ni += a, ui += b;
+            const int a = __shfl_up_sync(kFull, n, o), b = __shfl_up_sync(kFull, u, o);
+            if (lane >= o) n += a, u += b;
         }
+    };
+    auto deal = [&](bool none) {  // false: nothing for this block
+        if (__builtin_expect(none, 0))  // an empty context attends to nothing: rows of zeros
+#pragma unroll 1
+            for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
+                if (lengths_of(p, s).tiles > 0) continue;
+                const size_t row = p.q_rows ? p.q_rows[s] : s;
+                const int count = (p.q_lens ? p.q_lens[s] : 1) * p.hq * HD;
+#pragma unroll 1
+                for (int e = threadIdx.x; e < count; e += kThreads) p.out[row * p.hq * HD + e] = 0;
+            }
+        // Units of much the same length, as many as there are warps or fewer: each has a team of warps of a block to itself, and no block
+        // shares one with another.  Else equal runs.
+        const int warps = (int)gridDim.x * kWarps;
+        run = max(min(kMinRun, longest), (total + warps - 1) / warps);
+        team_log2 = 3;
+        static_assert(kWarps == 8, "a team is 1, 2, 4 or 8 of a block's warps");
+#pragma unroll 1
+        while (team_log2 > 0 && units > warps >> team_log2) team_log2--;
+        team = 1 << team_log2, block_units = kWarps >> team_log2;
+        by_unit = units <= warps >> team_log2 && run <= kUnitRun &&
+                  (longest + team - 1) >> team_log2 <= run + (team == kWarps ? kBlockSlack : kUnitSlack);
+        block_start = blockIdx.x * kWarps * run;
+        left = by_unit ? min((int)blockIdx.x * block_units + (warp >> team_log2), units - 1) : min(block_start + warp * run, total - 1);
+        return by_unit ? (int)blockIdx.x * block_units < units : block_start < total;
+    };
+    // With many sequences a block looks at all of them together, a thread at 1/256 (4096 sequences of 100: 160 us; each warp by itself 191) ...
+    const bool many = p.num_seqs > kThreads;
+    if (__builtin_expect(many, 0)) {
+        const int per = (span + kThreads - 1) / kThreads;
+        int n = 0, u = 0, most = 0, none = 0;
+        add_up(threadIdx.x * per, min((int)(threadIdx.x + 1) * per, span), n, u, most, none);
+        int ni = n, ui = u;
+        scan(ni, ui);
+        most = __reduce_max_sync(kFull, most);
+        none = __any_sync(kFull, none);
+        if (lane == 31) s_scan[warp] = make_int4(ni, ui, most, none);
+        __syncthreads();
+#pragma unroll 1
+        for (int w = 0; w < kWarps; w++) {
+            const int4 v = s_scan[w];
+            if (w < warp) ni += v.x, ui += v.y;
+            total += v.x, units += v.y, longest = max(longest, v.z), none |= v.w;
+        }
+        s_first[0][threadIdx.x] = ni - n, s_first[1][threadIdx.x] = ui - u;
+        __syncthreads();
+        if (!deal(none)) return;
+        const int* first = s_first[by_unit];
+        int at = 0;  // the last thread whose sequences begin at or before the place; of equal ones all but the last have nothing
+#pragma unroll 1
+        for (int step = kThreads / 2; step > 0; step >>= 1)
+            if (first[at + step] <= left) at += step;
+        left -= first[at];
+        lo = at * per, span = min(per, span - lo);
+    }
+    // ... and else every warp finds its place by itself, without waiting for others: its lanes add up what 1/32 of the sequences have each, and
+    // then the same of the lane that holds the place, until that is one sequence.
+    for (bool all = !many;; all = false) {
+        const int per = (span + 31) >> 5, from = lo + lane * per;
+        int n = 0, u = 0, most = 0, none = 0;
+        add_up(from, min(from + per, lo + span), n, u, most, none);
+        int ni = n, ui = u;
+        scan(ni, ui);
         if (all) {
             total = __shfl_sync(kFull, ni, 31), units = __shfl_sync(kFull, ui, 31), longest = __reduce_max_sync(kFull, most);
-            if (__builtin_expect(__any_sync(kFull, none), 0))  // an empty context attends to nothing: rows of zeros
-#pragma unroll 1
-                for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
-                    if (lengths_of(p, s).tiles > 0) continue;
-                    const size_t row = p.q_rows ? p.q_rows[s] : s;
-                    const int count = (p.q_lens ? p.q_lens[s] : 1) * p.hq * HD;
-#pragma unroll 1
-                    for (int e = threadIdx.x; e < count; e += kThreads) p.out[row * p.hq * HD + e] = 0;
-                }
-            // Units of much the same length, as many as there are warps or fewer: each has a team of warps of a block to itself, and no block
-            // shares one with another.  Else equal runs.
-            const int warps = (int)gridDim.x * kWarps;
-            run = max(min(kMinRun, longest), (total + warps - 1) / warps);
-            team_log2 = 3;
-            static_assert(kWarps == 8, "a team is 1, 2, 4 or 8 of a block's warps");
-#pragma unroll 1
-            while (team_log2 > 0 && units > warps >> team_log2) team_log2--;
-            team = 1 << team_log2, block_units = kWarps >> team_log2;
-            by_unit = units <= warps >> team_log2 && run <= kUnitRun &&
-                      (longest + team - 1) >> team_log2 <= run + (team == kWarps ? kBlockSlack : kUnitSlack);
-            block_start = blockIdx.x * kWarps * run;
-            if (by_unit ? (int)blockIdx.x * block_units >= units : block_start >= total) return;
-            left = by_unit ? min((int)blockIdx.x * block_units + (warp >> team_log2), units - 1) : min(block_start + warp * run, total - 1);
+            if (!deal(__any_sync(kFull, none))) return;
         }
         const int size = by_unit ? u : n, before = (by_unit ? ui : ni) - size;
         const int owner = __ffs(__ballot_sync(kFull, left >= before && left - before < size)) - 1;

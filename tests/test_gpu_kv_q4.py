@@ -248,6 +248,9 @@ DECODE = [
     ([70, 1000], 32, 2, 128, 16),  # 16
     ([64, 3], 40, 2, 64, 16),      # 20: three
     (list(range(1, 90)), 8, 2, 128, 16),
+    ([(5 * i) % 23 for i in range(300)], 8, 2, 128, 16),       # each unit a warp's
+    ([(37 * i) % 500 for i in range(300)], 4, 1, 64, 16),
+    ([300 + i % 60 for i in range(60)], 16, 8, 128, 16),       # ... two warps'
     ([9000, 20000], 2, 1, 64, 16),
 ]
 
