@@ -142,7 +142,8 @@ int32_t b2_paged_attn_prefill(b2_ctx* ctx, const uint16_t* q_dev, const uint16_t
 /* ---- 4-bit key/value cache --------------------------------------------------------------------
  * The same cache in 4-bit codes with a bf16 scale and bias for each 64 dims of a token's head: 144 bytes per token and kv
  * head at head size 128, 72 at 64, against 512 and 256 (the reference caches bf16 only, src/primitives/kv_cache.rs:30-64).
- * A code c stands for bf16(c * scale + bias).
+ * A code c stands for bf16(c * scale + bias).  Scales are less than 2^59, or NaN for a group without values: a pool that holds a
+ * larger one gives those who see that token no defined result.  Attention takes values below 2^-62 as multiples of 2^-69.
  * Pool: [n_pages, hkv, page_size / 16, record] bytes, a record being the keys and values of 16 tokens of one kv head:
  *   K codes  [16 tokens][head_dim / 2] bytes: a token's dims in order, the lower of two in the low nibble
  *   V codes  u32 [2][8][4][head_dim / 32]: word (h, g, c, d) holds token 8h + 2c in its low and token 8h + 2c + 1 in its high
@@ -156,7 +157,8 @@ int64_t b2_kv_q4_pool_bytes(int64_t n_pages, int32_t hkv, int32_t head_dim, int3
 /* b2_rope_kv_append into such a pool: [per-head q/k RMSNorm ->] NeoX RoPE -> quantization -> append.  The rotation and its
  * roundings are the same.  Per 64 values: e = the one farthest from zero (the largest in a tie), n = round(15 |e| / (max - min)),
  * scale = bf16(-e / n), bias = e, code = clamp(round((x - bias) / scale), 0, 15), halves away from zero; equal values: scale 0.
- * Values that are infinite, NaN or beyond 2^100 make their group NaN.  A slot outside of the pool skips the cache write; of
+ * A group becomes NaN if one of its values is infinite or NaN, if its scale would be 2^59 or more (values that lie 2^63 or so
+ * apart), or if its values differ and 15 |e| is 2^128 or more.  A slot outside of the pool skips the cache write; of
  * tokens with the same slot in one call the last write is any of them.  k_out_dev / v_out_dev (nullable) [T, hkv, head_dim]
  * receive the bf16 values that the codes stand for, for a caller that goes on with them. */
 int32_t b2_rope_kv_append_q4(b2_ctx* ctx, const uint16_t* qkv_dev, int32_t T, int32_t hq, int32_t hkv, int32_t head_dim,

@@ -24,7 +24,9 @@ inline int record_bytes(int hd) { return hd == 128 ? Record<128>::kBytes : Recor
 
 // Codes become numbers as the weights' codes do (dequant.cuh): a nibble in the low bits of a bf16 is the number c 2^-133, so one fma with
 // scale 2^69 and bias 2^-64 gives the value times 2^-64 with one rounding: bf16(c scale + bias) 2^-64, wherever that is no subnormal
-// (values from 2^-62 on; smaller ones lose bits beside what the 4 bits lose).  Scales stay finite up to 2^58.
+// (values from 2^-62 on; smaller ones lose bits beside what the 4 bits lose).  A scale times 2^69 is finite below 2^59; the append writes
+// none from there on.
+constexpr float kScaleEnd = 576460752303423488.f;  // 2^59
 constexpr float kUnscale = 18446744073709551616.f;  // 2^64
 struct Scales {
     uint32_t lo, hi, bias;  // for nibbles 0, 2 (bits 0-3 of a half word), for nibbles 1, 3 (bits 4-7), and the biases
@@ -35,8 +37,8 @@ __device__ __forceinline__ Scales scales_of(uint32_t s2, uint32_t b2) {
 // one token's, for both halves of a word, and two tokens', one for each half
 __device__ __forceinline__ Scales scales_twice(uint32_t sb) { return scales_of(prmt(sb, 0u, 0x1010u), prmt(sb, 0u, 0x3232u)); }
 __device__ __forceinline__ Scales scales_pair(uint32_t sb0, uint32_t sb1) { return scales_of(prmt(sb0, sb1, 0x5410u), prmt(sb0, sb1, 0x7632u)); }
-// whether a scale or a bias is infinite or NaN
-__device__ __forceinline__ bool poisoned(uint32_t sb) { return (sb & 0x7f80u) == 0x7f80u || (sb & 0x7f800000u) == 0x7f800000u; }
+// whether values of this scale and bias may be infinite or NaN: a scale from 2^59 (0x5d00) on, a bias that is one
+__device__ __forceinline__ bool poisoned(uint32_t sb) { return (sb & 0x7fffu) >= 0x5d00u || (sb & 0x7f800000u) == 0x7f800000u; }
 // nibble i of the low half word beside nibble i of the high one
 __device__ __forceinline__ void values(uint32_t w, const Scales& s, uint32_t (&out)[4]) { scaled_q4_paired(w, s.lo, s.hi, s.bias, out); }
 

@@ -4,7 +4,8 @@
 // scale and a bias such that the value farthest from zero, e, and zero itself are codes:
 //   n = round(15 |e| / (max - min)),  scale = bf16(-e / n),  bias = e,  code = clamp(round((x - bias) / scale), 0, 15)
 // (e the maximum in a tie; halves away from zero).  Codes are taken for the scale as it is stored, so that its rounding costs nothing
-// again; all values equal: scale 0.  A NaN or an infinity makes the scale a NaN, and with it the group's values, as they would be in bf16.
+// again; all values equal: scale 0.  A NaN or an infinity makes the scale a NaN, and with it the group's values, as they would be in bf16;
+// so do values that are too large for 15 |e| or for a scale that attention takes (q4::kScaleEnd), so that all readers have the same values.
 //
 // Bound by HBM (6151 tokens of 64 + 16 heads with norms: 261 MB in 58.6 us, 4.5 TB/s) once the instructions are few: HD / 16 lanes take a
 // head, each 8 adjacent dims of either half, so that reads and writes are 16 bytes, the rotation's roundings come with bf16x2 instructions
@@ -89,8 +90,8 @@ struct Group {
 __device__ __forceinline__ Group group_of(float lo, float hi) {
     const float edge = fabsf(lo) > fabsf(hi) ? lo : hi, span = hi - lo;
     if (span == 0.f) return {0.f, edge};
-    const float scale = rbf(__fdiv_rn(-edge, roundf(__fdiv_rn(15.f * fabsf(edge), span))));
-    return {isfinite(span) ? scale : __int_as_float(0x7fc00000), edge};
+    const float most = 15.f * fabsf(edge), scale = rbf(__fdiv_rn(-edge, roundf(__fdiv_rn(most, span))));
+    return {most < INFINITY && fabsf(scale) < q4::kScaleEnd ? scale : __int_as_float(0x7fc00000), edge};
 }
 // smallest and largest of a lane's eight; NaN where one is NaN or infinite (0 x is, then)
 __device__ __forceinline__ void ends_of(const Eight& v, float& lo, float& hi) {

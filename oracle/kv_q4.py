@@ -28,9 +28,9 @@ def quantize(x):
     with np.errstate(all="ignore"):
         n = away(15 * np.abs(edge) / span)
         scale = np.where(span == 0, 0.0, bf16(-edge / n))
-        scale = np.where(np.isfinite(span), scale, np.nan)
+        scale = np.where((span == 0) | (15 * np.abs(edge) < 2.0 ** 128) & (np.abs(scale) < 2.0 ** 59), scale, np.nan)
         codes = np.clip(away((x - edge[..., None]) / scale[..., None]), 0, 15)
-    codes = np.where(scale[..., None] == 0, 0, codes)
+    codes = np.where((scale[..., None] == 0) | np.isnan(scale[..., None]), 0, codes)
     return codes.reshape(codes.shape[:-2] + (codes.shape[-2] * 64,)), scale, edge
 
 
