@@ -156,6 +156,10 @@ class LogitRules(C.Structure):
 def logit_rules(mask_words=0, **arrays):
     """Rules for logits_adjust: history, history_off, n_prompt, repetition, presence, frequency, bias_id, bias_value, bias_off, mask, mask_row as device
     buffers (None: not used), and the words of a mask's row."""
+    names = [name for name, _ in LogitRules._fields_ if name != "mask_words"]
+    unknown = sorted(set(arrays) - set(names))
+    if unknown:  # (a structure takes any attribute, and the call would go without the rule)
+        raise TypeError(f"logit_rules: no rule is called {', '.join(unknown)}; there are {', '.join(names)}")
     rules = LogitRules()
     rules.mask_words = mask_words
     for name, a in arrays.items():

@@ -1,0 +1,17 @@
+"""What the Python side of the 4-bit cache and of the rules on logits checks before anything reaches the library."""
+import pytest
+
+from tests.test_kv_q4_host import AT, kernels  # noqa: F401
+
+
+@pytest.mark.parametrize("wrong", ["masks", "repetiton", "bias_ids", "history_dev", "h"])
+def test_a_rule_that_is_not_there(kernels, wrong):
+    with pytest.raises(TypeError, match=wrong):
+        kernels.logit_rules(history=AT, history_off=AT, **{wrong: AT})
+
+
+def test_rules_reach_their_fields(kernels):
+    names = ["history", "history_off", "n_prompt", "repetition", "presence", "frequency", "bias_id", "bias_value", "bias_off", "mask", "mask_row"]
+    rules = kernels.logit_rules(mask_words=5, **{n: 16 * (i + 1) for i, n in enumerate(names)})
+    assert [getattr(rules, n) for n in names] == [16 * (i + 1) for i in range(len(names))] and rules.mask_words == 5
+    assert kernels.logit_rules(mask=None).mask is None
