@@ -117,11 +117,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // The eight codes of a lane, lowest nibble first.  The quotient comes from a reciprocal; what it misses is put right by the sign of an fma:
 // (x - edge) / scale is never negative, and halves go up.
 __device__ __forceinline__ uint32_t codes_of(const Eight& v, const Group& q) {
-    const float s = fabsf(q.scale), inv = s > 0.f ? __fdividef(1.f, s) : 0.f, half = 0.5f * s;
+    // (a scale below 2^-126 has no reciprocal: such a group, whose values are below 2^-87, is taken 2^64 times as large, exactly)
+    const float up = fabsf(q.scale) < 0x1p-100f ? 0x1p64f : 1.f, edge = q.edge * up;
+    const float s = fabsf(q.scale) * up, inv = s > 0.f ? __fdividef(1.f, s) : 0.f, half = 0.5f * s;
     uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float d = fabsf(v[i] - q.edge);
+        const float d = fabsf(fmaf(v[i], up, -edge));
         const float magic = fminf(d * inv, 15.f) + 8388608.f;  // 2^23: the sum's low bits are the whole number
         const float r = fmaf(8388608.f - magic, s, d);         // d - code s
         int code = (__float_as_int(magic) & 31) + (r >= half) - (r < -half);

@@ -29,7 +29,7 @@ def stored(pool, page, hkv, hd, slot, kvh, is_v):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("power", [-100, -64, 50, 58, 59, 60, 61, 62, 63, 64, 70, 100, 120, 122, 123, 124, 125, 126])
+@pytest.mark.parametrize("power", [-133, -131, -129, -128, -127, -126, -120, -100, -64, 50, 58, 59, 60, 61, 62, 63, 64, 70, 100, 120, 122, 123, 124, 125, 126])
 def test_append_of_large_and_small_values(env, hd, power):
     """Normal numbers times 2^power, groups on one side of zero, and groups of equal values."""
     n, hq, hkv, page, pages = 24, 1, 1, 16, 2
