@@ -64,6 +64,9 @@ constexpr float kRaise = 8.f, kFloor = -1e30f;
 template <int HD>
 struct Smem {
     static constexpr int kQ = 0, kRing = 2 * tile_bytes<HD>(), kBar = kRing + kSlots * tile_bytes<HD>(), kBytes = kBar + 256;
+    // Records of a tile that are not there, a bit each: a byte per converting warp, a word per tile, of the last four tiles.  (The ring has
+    // room for K of tile t when P V of t - 3 is done, and with it all that the softmax reads of that tile.)
+    static constexpr int kAbsent = kBar + 192;
 };
 constexpr uint32_t kIdesc128 = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 template <int HD>
@@ -137,7 +140,7 @@ struct Source {  // the two records of a converting warp in a tile
             if (left[i] <= 0) continue;
             const int index = r / p.page_tiles, page = p.block_tables[(size_t)w.bt_row * p.max_blocks + index];
             if (page < 0 || page >= p.n_pages)
-                left[i] = 0;  // nothing there: zeros
+                left[i] = 0;  // nothing there: zeros, which the softmax leaves out
             else
                 rec[i] += (((size_t)page * p.hkv + w.kvh) * p.page_tiles + r - index * p.page_tiles) * q4::Record<HD>::kBytes;
         }
@@ -278,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
         from.find(p, w, w.first_tile, warp - kConvert);
         from.read(keys, false, lane);
         from.read(vals, true, lane);
-        int slot = 0;
+        int slot = 0, tile = 0;
         uint32_t parity = 0;  // of the slot's present use
         auto fill = [&](auto put) {
             alive = __all_sync(0xffffffffu, mbar_wait(empty(slot), parity ^ 1u));
@@ -291,10 +294,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
         };
         for (bool more = true; more;) {
             more = next();
-            fill([&](uint8_t* tile) { put_keys<HD>(tile, row0, keys, lane); });
+            fill([&](uint8_t* at) {
+                put_keys<HD>(at, row0, keys, lane);
+                if (lane == 0) smem[S::kAbsent + (tile & 3) * 4 + warp - kConvert] = (uint8_t)((keys.left[0] <= 0) | (keys.left[1] <= 0) << 1);
+            });
             if (!alive) break;
+            tile++;
             if (more) from.read(keys, false, lane);
-            fill([&](uint8_t* tile) { put_values<HD>(tile, row0, vals, lane); });
+            fill([&](uint8_t* at) { put_values<HD>(at, row0, vals, lane); });
             if (!alive) break;
             if (more) from.read(vals, true, lane);
         }
@@ -412,13 +419,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
         };
         copy_q(p.segments[begin]);
         q_there();
-        uint32_t phase = 0, seg_phase = 0;
+        uint32_t phase = 0, seg_phase = 0, tile = 0;
         for (int segment = begin; segment < end; segment++, seg_phase ^= 1u) {
             // last key that the row sees; rows without a query see all (nothing comes of them)
             const Segment* const work = p.segments + segment;
             const int n = work->n_tiles, first_key = work->first_tile * KT, sees = in_block && query < work->queries ? work->sees + query : 0x3fffffff;
             float m = kFloor, l = 0.f;
-            for (int j = 0; j < n; j++, phase ^= 1u) {
+            for (int j = 0; j < n; j++, tile++, phase ^= 1u) {
                 if (!__all_sync(0xffffffffu, mbar_wait(s_ready(x), phase))) {
                     alive = false;
                     break;
@@ -426,14 +433,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv_q4_prefill_kernel(const Produc
                 tc_fence_after();
                 // The upper 64 scores are read for the maximum and, once the lower ones have become P, again: a thread has 128 registers.
                 const int key0 = first_key + j * KT;
-                if (__any_sync(0xffffffffu, key0 + KT - 1 > sees)) {  // in place, so that the code for other tiles is without it
+                const uint32_t absent = *reinterpret_cast<volatile uint32_t*>(smem + S::kAbsent + (tile & 3) * 4);
+                if (__any_sync(0xffffffffu, key0 + KT - 1 > sees || absent != 0)) {  // in place, so that the code for other tiles is without it
 #pragma unroll 1
                     for (int c = 0; c < 4; c++) {
                         uint32_t v[32];
                         tc_ld32(ts + c * 32u, v);
+                        const int sees0 = absent >> (8 * c) & 1 ? -1 : sees, sees1 = absent >> (8 * c) & 2 ? -1 : sees;  // of two records
 #pragma unroll
                         for (int i = 0; i < 32; i++)
-                            if (key0 + c * 32 + i > sees) v[i] = 0xff800000u;
+                            if (key0 + c * 32 + i > (i < 16 ? sees0 : sees1)) v[i] = 0xff800000u;
                         tc_st32(ts + c * 32u, v);
                     }
                 }
