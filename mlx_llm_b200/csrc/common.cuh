@@ -87,6 +87,13 @@ enum { B2_CLS_GEMM = 0, B2_CLS_ATTN_DECODE = 1, B2_CLS_ATTN_PREFILL = 2, B2_CLS_
 void b2_prof_mark(b2_ctx* ctx, int cls);
 // After the stream has been synchronised: folds the recorded stretches into class_ms.
 void b2_prof_collect(b2_ctx* ctx);
+// Makes a buffer of the context hold `bytes` at least, a quarter more and `spare` if it has to be made anew; what it held is lost then.  If that
+// fails the buffer is gone and its size is 0, so that no later call takes the size for what is there.
+int32_t b2_ctx_grow_bytes(b2_ctx* ctx, void** buf, size_t* have, size_t bytes, size_t spare);
+template <typename T>
+inline int32_t b2_ctx_grow(b2_ctx* ctx, T** buf, size_t* have, size_t bytes, size_t spare = 0) {
+    return b2_ctx_grow_bytes(ctx, reinterpret_cast<void**>(buf), have, bytes, spare);
+}
 int32_t b2_ctx_scratch(b2_ctx* ctx, size_t bytes, void** out);
 int32_t b2_ctx_stage(b2_ctx* ctx, size_t bytes, void** out);
 #define B2_LAUNCHED(ctx) ((ctx)->launches++)

@@ -261,27 +261,24 @@ void b2_prof_collect(b2_ctx* ctx) {
     ctx->prof_launch.clear();
 }
 
+int32_t b2_ctx_grow_bytes(b2_ctx* ctx, void** buf, size_t* have, size_t bytes, size_t spare) {
+    if (bytes <= *have) return B2_OK;
+    B2_CUDA(cudaStreamSynchronize(ctx->stream));
+    void* old = *buf;
+    *buf = nullptr, *have = 0;
+    if (old) B2_CUDA(cudaFree(old));
+    const size_t want = bytes + (bytes >> 2) + spare;
+    B2_CUDA(cudaMalloc(buf, want));
+    *have = want;
+    return B2_OK;
+}
 int32_t b2_ctx_scratch(b2_ctx* ctx, size_t bytes, void** out) {
-    if (bytes > ctx->scratch_bytes) {
-        B2_CUDA(cudaStreamSynchronize(ctx->stream));
-        if (ctx->scratch) B2_CUDA(cudaFree(ctx->scratch));
-        ctx->scratch = nullptr;
-        size_t want = bytes + (bytes >> 2) + (1 << 20);
-        B2_CUDA(cudaMalloc(&ctx->scratch, want));
-        ctx->scratch_bytes = want;
-    }
+    B2_CHECK(b2_ctx_grow(ctx, &ctx->scratch, &ctx->scratch_bytes, bytes, 1 << 20));
     *out = ctx->scratch;
     return B2_OK;
 }
 int32_t b2_ctx_stage(b2_ctx* ctx, size_t bytes, void** out) {
-    if (bytes > ctx->stage_bytes) {
-        B2_CUDA(cudaStreamSynchronize(ctx->stream));
-        if (ctx->stage) B2_CUDA(cudaFree(ctx->stage));
-        ctx->stage = nullptr;
-        size_t want = bytes + (bytes >> 2) + (1 << 16);
-        B2_CUDA(cudaMalloc(&ctx->stage, want));
-        ctx->stage_bytes = want;
-    }
+    B2_CHECK(b2_ctx_grow(ctx, &ctx->stage, &ctx->stage_bytes, bytes, 1 << 16));
     *out = ctx->stage;
     return B2_OK;
 }

@@ -381,13 +381,7 @@ int32_t launch_stream(b2_ctx* ctx, const GemmParams& p) {
     StreamExtra ex{splits, cut.k_per_range, nullptr, nullptr};
     if (splits > 1) {
         const size_t bytes = (size_t)splits * p.M * p.N * sizeof(float);
-        if (bytes > ctx->tc_partial_bytes) {
-            B2_CUDA(cudaStreamSynchronize(ctx->stream));
-            if (ctx->tc_partial) B2_CUDA(cudaFree(ctx->tc_partial));
-            ctx->tc_partial = nullptr;
-            B2_CUDA(cudaMalloc((void**)&ctx->tc_partial, bytes + (bytes >> 2)));
-            ctx->tc_partial_bytes = bytes + (bytes >> 2);
-        }
+        B2_CHECK(b2_ctx_grow(ctx, &ctx->tc_partial, &ctx->tc_partial_bytes, bytes));
         ex.partial = ctx->tc_partial;
         constexpr int kMaxTiles = 8192;  // row tiles of 128: up to N = 1 M features
         B2_REQUIRE(row_tiles <= kMaxTiles, B2_ERR_UNSUPPORTED, "gemm: output too wide for the split-K streaming kernel");

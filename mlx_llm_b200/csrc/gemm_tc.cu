@@ -829,13 +829,7 @@ int32_t launch_pair(b2_ctx* ctx, const GemmParams& p, int* err) {
     plan.partial = nullptr;
     if (best > 1) {
         const size_t bytes = (size_t)best * p.M * p.N * sizeof(float);
-        if (bytes > ctx->tc_partial_bytes) {
-            B2_CUDA(cudaStreamSynchronize(ctx->stream));
-            if (ctx->tc_partial) B2_CUDA(cudaFree(ctx->tc_partial));
-            ctx->tc_partial = nullptr;
-            B2_CUDA(cudaMalloc((void**)&ctx->tc_partial, bytes + (bytes >> 2)));
-            ctx->tc_partial_bytes = bytes + (bytes >> 2);
-        }
+        B2_CHECK(b2_ctx_grow(ctx, &ctx->tc_partial, &ctx->tc_partial_bytes, bytes));
         plan.partial = ctx->tc_partial;
     }
     const int units = plan.total_blocks * best;

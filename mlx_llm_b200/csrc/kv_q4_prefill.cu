@@ -730,14 +730,7 @@ static int32_t launch_many(b2_ctx* ctx, const Q4PrefillParams& p, const Q4Plan& 
     a.err = ctx->dev_err;
     if (plan.parts > 0) {
         const size_t rows = (size_t)plan.parts * 2 * kRows, bytes = rows * (HD + 2) * sizeof(float);
-        if (bytes > ctx->pf_part_bytes) {
-            B2_CUDA(cudaStreamSynchronize(ctx->stream));
-            if (ctx->pf_part) B2_CUDA(cudaFree(ctx->pf_part));
-            ctx->pf_part = nullptr;
-            ctx->pf_part_bytes = 0;
-            B2_CUDA(cudaMalloc((void**)&ctx->pf_part, bytes + (bytes >> 2)));
-            ctx->pf_part_bytes = bytes + (bytes >> 2);
-        }
+        B2_CHECK(b2_ctx_grow(ctx, &ctx->pf_part, &ctx->pf_part_bytes, bytes));
         a.part_o = ctx->pf_part;
         a.part_ml = ctx->pf_part + rows * HD;
     }

@@ -491,7 +491,7 @@ int32_t b2_decode_attn_counters(b2_ctx* ctx, int num_seqs, int hkv, int** out) {
     if (need > ctx->attn_counters_cap) {
         B2_CUDA(cudaStreamSynchronize(ctx->stream));
         if (ctx->attn_counters) B2_CUDA(cudaFree(ctx->attn_counters));
-        ctx->attn_counters = nullptr;
+        ctx->attn_counters = nullptr, ctx->attn_counters_cap = 0;
         const size_t cap = need + need / 4 + 1024;
         B2_CUDA(cudaMalloc((void**)&ctx->attn_counters, cap * sizeof(int)));
         B2_CUDA(cudaMemsetAsync(ctx->attn_counters, 0, cap * sizeof(int), ctx->stream));

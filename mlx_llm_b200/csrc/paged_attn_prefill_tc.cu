@@ -739,13 +739,7 @@ int32_t b2_prefill_attn_tc_launch(b2_ctx* ctx, const PrefillAttnParams& p, int g
     if (splits > 1) {
         const size_t slots = (size_t)grid_work * p.hq * splits * QT;
         const size_t bytes = slots * (HD + 2) * sizeof(float);
-        if (bytes > ctx->pf_part_bytes) {
-            B2_CUDA(cudaStreamSynchronize(ctx->stream));
-            if (ctx->pf_part) B2_CUDA(cudaFree(ctx->pf_part));
-            ctx->pf_part = nullptr;
-            B2_CUDA(cudaMalloc((void**)&ctx->pf_part, bytes + (bytes >> 2)));
-            ctx->pf_part_bytes = bytes + (bytes >> 2);
-        }
+        B2_CHECK(b2_ctx_grow(ctx, &ctx->pf_part, &ctx->pf_part_bytes, bytes));
         ex.splits = splits;
         ex.part_o = ctx->pf_part;
         ex.part_ml = ctx->pf_part + slots * HD;
