@@ -16,8 +16,10 @@ int32_t b2_fail(int32_t code, const std::string& msg);
 #define B2_CUDA(call)                                                                             \
     do {                                                                                          \
         cudaError_t e__ = (call);                                                                 \
-        if (e__ != cudaSuccess)                                                                   \
+        if (e__ != cudaSuccess) {                                                                 \
+            cudaGetLastError(); /* told here: the check behind the next launch must not find it */ \
             return b2_fail(B2_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e__));     \
+        }                                                                                         \
     } while (0)
 #define B2_CHECK(call)            \
     do {                          \

@@ -91,6 +91,16 @@ static int32_t GET(b2_ctx* ctx, size_t bytes, void** out) {
     return B2_OK;
 }
 int main() {""" + BUFFER + "}",
+    # the error belongs to the call that failed: a kernel's launch after it asks for the last error
+    "last error": r"""
+int main() {
+    b2_ctx ctx;
+    void* at = nullptr;
+    SAY(b2_malloc(&ctx, 1 << 10, &at) == B2_ERR_CUDA);
+    SAY(std::string(b2_last_error()).find("out of memory") != std::string::npos);
+    SAY(cudaGetLastError() == cudaSuccess);
+    return 0;
+}""",
 }
 
 
