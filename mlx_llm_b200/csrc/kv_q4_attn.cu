@@ -436,12 +436,12 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) kv_q4_attn_kernel(c
                 else
                     s1[0] = s1[1] = s1[2] = s1[3] = -INFINITY;
                 const int tok0 = t * 16;
-                const bool some = tok0 + 32 > sure && p.q_lens;
+                const bool edge = tok0 > sure - 32, some = edge && p.q_lens;  // (tok0 + 32 may be 2^31)
                 if (some) {
                     if (one) hidden_values<HD>(rec0, lane, s0);
                     if (two) hidden_values<HD>(rec1, lane, s1);
                 }
-                if (tok0 + 32 > sure) {
+                if (edge) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const int lim = j & 1 ? lim1 : lim0, tok = tok0 + g + (j >> 1) * 8;
