@@ -150,9 +150,9 @@ int32_t b2_paged_attn_prefill(b2_ctx* ctx, const uint16_t* q_dev, const uint16_t
  *            half, each the dims g * head_dim / 8 + 4d .. + 3 from the lowest nibble on
  *   K, then V scales and biases: u32 [head_dim / 64][16 tokens], scale in the low half, bias in the high one (both bf16)
  * b2_kv_q4_pool_bytes gives the pool's size; a pool needs no initial contents.  Any hq / hkv that is whole, head_dim 64 or 128,
- * page_size a multiple of 16, a positive softmax scale, pool and bf16 arrays 16-byte aligned.  A block table may name pages in
- * any order; of a page number outside of 0 .. n_pages - 1 nothing is read: attention leaves its tokens out, and a query that sees
- * no others gets zeros. */
+ * page_size a multiple of 16, a softmax scale above 0 and below 2^62, pool and bf16 arrays 16-byte aligned.  A block table may
+ * name pages in any order; of a page number outside of 0 .. n_pages - 1 nothing is read: attention leaves its tokens out, and a
+ * query that sees no others gets zeros. */
 int64_t b2_kv_q4_pool_bytes(int64_t n_pages, int32_t hkv, int32_t head_dim, int32_t page_size); /* 0 for sizes that are refused */
 /* b2_rope_kv_append into such a pool: [per-head q/k RMSNorm ->] NeoX RoPE -> quantization -> append.  The rotation and its
  * roundings are the same.  Per 64 values: e = the one farthest from zero (the largest in a tie), n = round(15 |e| / (max - min)),

@@ -213,6 +213,8 @@ int32_t b2_prefill_attn_tc_launch(b2_ctx* ctx, const PrefillAttnParams& p, int g
 // ---- 4-bit key/value cache (kv_q4_append.cu, kv_q4_attn.cu, kv_q4_prefill.cu; the records: kv_q4.cuh) -----------------------
 // What every entry point over such a pool refuses.
 int32_t b2_kv_q4_check(const char* who, const void* pool, int64_t n_pages, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size);
+// Softmax scales are less: times log2 e and the 2^64 that values are short of (kv_q4.cuh) they are finite.
+constexpr float kQ4SoftmaxScaleEnd = 4611686018427387904.f;  // 2^62
 struct RopeKvQ4Params {
     RopeKvParams rope;   // (its pools are not used)
     uint8_t* pool;       // [pages, hkv, page_size / 16, record]

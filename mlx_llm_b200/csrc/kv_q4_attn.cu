@@ -693,7 +693,7 @@ extern "C" int32_t b2_paged_attn_decode_q4(b2_ctx* ctx, const uint16_t* q_dev, c
     B2_REQUIRE(num_seqs >= 0 && max_blocks > 0, B2_ERR_MSG, "b2_paged_attn_decode_q4: bad sizes");
     B2_REQUIRE((double)num_seqs * max_blocks * (page_size / 16) * hkv * ((hq / hkv + 7) / 8) < 1073741824.0, B2_ERR_UNSUPPORTED,
                "b2_paged_attn_decode_q4: the block tables reach more than 2^30 records; make fewer sequences a call");
-    B2_REQUIRE(scale > 0.f && scale < INFINITY, B2_ERR_MSG, "b2_paged_attn_decode_q4: the scale must be positive");
+    B2_REQUIRE(scale > 0.f && scale < kQ4SoftmaxScaleEnd, B2_ERR_MSG, "b2_paged_attn_decode_q4: the scale must be positive and below 2^62");
     B2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & 15) == 0, B2_ERR_UNSUPPORTED, "b2_paged_attn_decode_q4: q and out must be 16-byte aligned");
     B2_CUDA(cudaSetDevice(ctx->device));
     Q4AttnParams p{};

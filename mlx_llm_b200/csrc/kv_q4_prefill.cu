@@ -776,7 +776,7 @@ extern "C" int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, 
     B2_REQUIRE(ctx && q_dev && kv_pool_dev && block_tables_dev && cu_seqlens_host && ctx_lens_host && out_dev, B2_ERR_MSG, "b2_paged_attn_prefill_q4: null argument");
     B2_CHECK(b2_kv_q4_check("b2_paged_attn_prefill_q4", kv_pool_dev, n_pages, hq, hkv, head_dim, page_size));
     B2_REQUIRE(num_seqs >= 0 && max_blocks > 0, B2_ERR_MSG, "b2_paged_attn_prefill_q4: bad sizes");
-    B2_REQUIRE(scale > 0.f && scale < INFINITY, B2_ERR_MSG, "b2_paged_attn_prefill_q4: the scale must be positive");
+    B2_REQUIRE(scale > 0.f && scale < kQ4SoftmaxScaleEnd, B2_ERR_MSG, "b2_paged_attn_prefill_q4: the scale must be positive and below 2^62");
     B2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & 15) == 0, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: q and out must be 16-byte aligned");
     if (num_seqs == 0) return B2_OK;
     std::vector<Q4Seq> seqs;

@@ -1,7 +1,7 @@
 """What the Python side of the 4-bit cache and of the rules on logits checks before anything reaches the library."""
 import pytest
 
-from tests.test_kv_q4_host import AT, kernels  # noqa: F401
+from tests.test_kv_q4_host import AT, decode, kernels, prefill, refused  # noqa: F401
 
 
 @pytest.mark.parametrize("wrong", ["masks", "repetiton", "bias_ids", "history_dev", "h"])
@@ -15,3 +15,9 @@ def test_rules_reach_their_fields(kernels):
     rules = kernels.logit_rules(mask_words=5, **{n: 16 * (i + 1) for i, n in enumerate(names)})
     assert [getattr(rules, n) for n in names] == [16 * (i + 1) for i in range(len(names))] and rules.mask_words == 5
     assert kernels.logit_rules(mask=None).mask is None
+
+
+@pytest.mark.parametrize("call", [decode, prefill])
+@pytest.mark.parametrize("scale", [2.0 ** 62, 2.0 ** 63, 3e38, -2.0 ** 62])
+def test_softmax_scales_that_attention_cannot_take(kernels, call, scale):
+    refused(lambda: call(kernels, scale=scale), -7)
