@@ -48,12 +48,14 @@ class _Entry:
 
 
 def _at(a):
-    """Address of a device buffer (DevBuf, or a number), a host array, or nothing."""
+    """Address of a device buffer (DevBuf, or a number), or nothing."""
     if a is None or type(a) is int:
         return a
-    if type(a) is DevBuf:
+    if isinstance(a, DevBuf):
         return a.ptr
-    return a.ctypes.data if isinstance(a, np.ndarray) else int(a)
+    if isinstance(a, np.ndarray):  # (a kernel that reads host memory faults)
+        raise TypeError("a host array where a device buffer is needed: upload it with Context.buf")
+    return int(a)
 
 
 _append_q4 = _Entry("b2_rope_kv_append_q4", "ppiiiippppppfipippp")

@@ -1,7 +1,8 @@
 """What the Python side of the 4-bit cache and of the rules on logits checks before anything reaches the library."""
+import numpy as np
 import pytest
 
-from tests.test_kv_q4_host import AT, decode, kernels, prefill, refused  # noqa: F401
+from tests.test_kv_q4_host import AT, CTX, append, decode, kernels, prefill, refused  # noqa: F401
 
 
 @pytest.mark.parametrize("wrong", ["masks", "repetiton", "bias_ids", "history_dev", "h"])
@@ -21,3 +22,13 @@ def test_rules_reach_their_fields(kernels):
 @pytest.mark.parametrize("scale", [2.0 ** 62, 2.0 ** 63, 3e38, -2.0 ** 62])
 def test_softmax_scales_that_attention_cannot_take(kernels, call, scale):
     refused(lambda: call(kernels, scale=scale), -7)
+
+
+@pytest.mark.parametrize("call", [
+    lambda K, a: decode(K, q=a), lambda K, a: decode(K, tables=a), lambda K, a: prefill(K, pool=a), lambda K, a: prefill(K, out=a), lambda K, a: append(K, pos=a),
+    lambda K, a: K.logit_rules(mask=a), lambda K, a: K.logits_adjust(CTX, a, 1, 64, K.logit_rules(), argmax=AT),
+    lambda K, a: K.logits_adjust(CTX, AT, 1, 64, K.logit_rules(), argmax=a),
+])
+def test_host_arrays_are_no_device_buffers(kernels, call):
+    with pytest.raises(TypeError, match="host array"):
+        call(kernels, np.zeros(64, np.int32))
