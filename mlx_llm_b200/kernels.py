@@ -83,6 +83,8 @@ def paged_attn_decode_q4(ctx, q, kv_pool, n_pages, block_tables, ctx_lens, num_s
 def paged_attn_prefill_q4(ctx, q, kv_pool, n_pages, block_tables, max_blocks, cu_seqlens, ctx_lens, hq, hkv, head_dim, page_size, scale, out):
     cu = np.ascontiguousarray(cu_seqlens, np.int32)
     cl = np.ascontiguousarray(ctx_lens, np.int32)
+    if cu.ndim != 1 or cl.ndim != 1 or cu.size != cl.size + 1:  # (the library reads one more of the first)
+        raise ValueError(f"paged_attn_prefill_q4: {cl.size} contexts need {cl.size + 1} cu_seqlens, not {cu.size}")
     _prefill_q4(ctx.h, _at(q), _at(kv_pool), n_pages, _at(block_tables), max_blocks, cu.ctypes.data, cl.ctypes.data, cl.size, hq, hkv, head_dim, page_size,
                 scale, _at(out))
 

@@ -32,3 +32,9 @@ def test_softmax_scales_that_attention_cannot_take(kernels, call, scale):
 def test_host_arrays_are_no_device_buffers(kernels, call):
     with pytest.raises(TypeError, match="host array"):
         call(kernels, np.zeros(64, np.int32))
+
+
+@pytest.mark.parametrize("cu, ctx", [((0,), (1,)), ((0, 1), (1, 1)), ((), ()), ((0, 1, 2), (4,)), (((0, 1), (1, 2)), (4, 4, 4))])
+def test_one_more_offset_than_sequences(kernels, cu, ctx):
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        prefill(kernels, cu=cu, ctx=ctx)
