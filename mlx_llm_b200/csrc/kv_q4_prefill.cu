@@ -780,13 +780,17 @@ extern "C" int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, 
     B2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & 15) == 0, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: q and out must be 16-byte aligned");
     if (num_seqs == 0) return B2_OK;
     std::vector<Q4Seq> seqs;
+    double segments = 0;  // of 256 rows, about: the plan's lists would outgrow the host's memory long before a GPU holds such queries
     for (int i = 0; i < num_seqs; i++) {
-        const int n = cu_seqlens_host[i + 1] - cu_seqlens_host[i], ctx_len = ctx_lens_host[i];
+        const int64_t n = (int64_t)cu_seqlens_host[i + 1] - cu_seqlens_host[i];
+        const int ctx_len = ctx_lens_host[i];
         B2_REQUIRE(cu_seqlens_host[i] >= 0 && n >= 0 && ctx_len >= n, B2_ERR_MSG, "b2_paged_attn_prefill_q4: ctx_lens must include the new tokens, and cu_seqlens ascend");
         B2_REQUIRE(((int64_t)ctx_len + page_size - 1) / page_size <= max_blocks, B2_ERR_MSG,
                    "b2_paged_attn_prefill_q4: a context needs more blocks than a block-table row holds");
         B2_REQUIRE(ctx_len <= 0x7fffff00, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: a context of more than 2^31 - 256 tokens");
-        seqs.push_back(Q4Seq{i, cu_seqlens_host[i], n, ctx_len});
+        segments += std::ceil((double)n * (hq / hkv) / (2 * kRows)) * hkv;
+        B2_REQUIRE(segments < 16777216.0, B2_ERR_UNSUPPORTED, "b2_paged_attn_prefill_q4: more than 2^24 x 256 queries of q heads; make fewer sequences a call");
+        seqs.push_back(Q4Seq{i, cu_seqlens_host[i], (int32_t)n, ctx_len});
     }
     B2_CUDA(cudaSetDevice(ctx->device));
     Q4Plan plan;

@@ -38,3 +38,11 @@ def test_host_arrays_are_no_device_buffers(kernels, call):
 def test_one_more_offset_than_sequences(kernels, cu, ctx):
     with pytest.raises(ValueError, match="cu_seqlens"):
         prefill(kernels, cu=cu, ctx=ctx)
+
+
+def test_more_queries_than_a_plan_holds(kernels):
+    """Refused before a list of them is made: memory that runs out would be an exception that no C caller can catch."""
+    n = 0x7fffff00
+    refused(lambda: prefill(kernels, cu=(0, n), ctx=(n,), blocks=1 << 27, hq=16, hkv=8), -5)
+    refused(lambda: prefill(kernels, cu=(0, n), ctx=(n,), blocks=1 << 27, hq=1024, hkv=2), -5)
+    refused(lambda: prefill(kernels, cu=(9, -(1 << 31)), ctx=(n,), blocks=1 << 27), -7)  # (a difference that 32 bits do not hold)
