@@ -158,9 +158,9 @@ int64_t b2_kv_q4_pool_bytes(int64_t n_pages, int32_t hkv, int32_t head_dim, int3
  * roundings are the same.  Per 64 values: e = the one farthest from zero (the largest in a tie), n = round(15 |e| / (max - min)),
  * scale = bf16(-e / n), bias = e, code = clamp(round((x - bias) / scale), 0, 15), halves away from zero; equal values: scale 0.
  * A group becomes NaN if one of its values is infinite or NaN, if its scale would be 2^59 or more (values that lie 2^63 or so
- * apart), or if its values differ and 15 |e| is 2^128 or more.  A slot outside of the pool skips the cache write; of
- * tokens with the same slot in one call the last write is any of them.  k_out_dev / v_out_dev (nullable) [T, hkv, head_dim]
- * receive the bf16 values that the codes stand for, for a caller that goes on with them. */
+ * apart), or if its values differ and 15 |e| is 2^128 or more.  A slot outside of the pool skips the cache write.  Slots inside
+ * of it must differ within a call: two tokens with the same one leave a mix of both there.  k_out_dev / v_out_dev (nullable)
+ * [T, hkv, head_dim] receive the bf16 values that the codes stand for, for a caller that goes on with them. */
 int32_t b2_rope_kv_append_q4(b2_ctx* ctx, const uint16_t* qkv_dev, int32_t T, int32_t hq, int32_t hkv, int32_t head_dim,
                              const int32_t* positions_dev, const int32_t* slot_mapping_dev, const uint16_t* cos_dev,
                              const uint16_t* sin_dev, const uint16_t* q_norm_dev, const uint16_t* k_norm_dev, float eps,
@@ -168,14 +168,16 @@ int32_t b2_rope_kv_append_q4(b2_ctx* ctx, const uint16_t* qkv_dev, int32_t T, in
                              uint16_t* k_out_dev, uint16_t* v_out_dev);
 /* b2_paged_attn_decode over such a pool: one query token per sequence.  Work is split evenly over the GPU whatever the
  * lengths; the results do not depend on timing.  A ctx_lens[i] above max_blocks * page_size is read as that maximum; 0 gives
- * rows of zeros.  What a page holds behind a sequence's end is not looked at. */
+ * rows of zeros.  What a page holds behind a sequence's end is not looked at.  The lengths being on the device, a call is measured
+ * by its tables: num_seqs * max_blocks * page_size / 16 * hkv * ceil(hq / hkv / 8) must be below 2^30. */
 int32_t b2_paged_attn_decode_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_t* kv_pool_dev, int32_t n_pages,
                                 const int32_t* block_tables_dev, int32_t max_blocks, const int32_t* ctx_lens_dev,
                                 int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size, float scale,
                                 uint16_t* out_dev);
 /* b2_paged_attn_prefill over such a pool: any number of query tokens per sequence, causal as there.  A query that does not see a
- * token is not touched by it, whatever it holds.  Which of two kernels a sequence goes through, and with it how P is rounded
- * (16 or 8 bits), depends on all the lengths of the call. */
+ * token is not touched by it, whatever it holds.  Which of two kernels a sequence goes through, and with it how the softmax's
+ * weights are rounded (16 or 8 bits: errors of up to 2^-8 of a row's values, of the size of the result's own rounding), depends on
+ * all the lengths of the call; a sequence's results may so differ by that with its neighbours. */
 int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, const uint8_t* kv_pool_dev, int32_t n_pages,
                                  const int32_t* block_tables_dev, int32_t max_blocks, const int32_t* cu_seqlens_host,
                                  const int32_t* ctx_lens_host, int32_t num_seqs, int32_t hq, int32_t hkv, int32_t head_dim,

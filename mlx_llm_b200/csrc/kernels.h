@@ -264,7 +264,7 @@ struct Q4PrefillParams {
     float scale_log2;
     uint16_t* out;
 };
-int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int hkv, int head_dim, Q4Plan& plan);
+int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int hkv, Q4Plan& plan);
 // `plan_dev`: plan.host on the device
 int32_t b2_kv_q4_prefill_launch(b2_ctx* ctx, const Q4PrefillParams& p, int head_dim, const Q4Plan& plan, const int32_t* plan_dev);
 

@@ -7,8 +7,9 @@
 // again; all values equal: scale 0.  A NaN or an infinity makes the scale a NaN, and with it the group's values, as they would be in bf16;
 // so do values that are too large for 15 |e| or for a scale that attention takes (q4::kScaleEnd), so that all readers have the same values.
 //
-// Bound by HBM (6151 tokens of 64 + 16 heads with norms: 261 MB in 58.6 us, 4.5 TB/s) once the instructions are few: HD / 16 lanes take a
-// head, each 8 adjacent dims of either half, so that reads and writes are 16 bytes, the rotation's roundings come with bf16x2 instructions
+// Bound by instructions and by the wait for its loads, not by HBM alone (6151 tokens of 64 + 16 heads with norms: 261 MB in 59 us, 4.4 TB/s, while
+// 68 % of the issue slots are taken and a warp, one of 26 on an SM, waits for what it loads a third of its time).  So instructions are few: HD / 16
+// lanes take a head, each 8 adjacent dims of either half, so that reads and writes are 16 bytes, the rotation's roundings come with bf16x2 instructions
 // (a product or a sum of two bf16 numbers rounded once is what they give), and a lane's codes of a group are one word.  The lanes go through
 // two heads of a token with one set of positions and norm weights (one head: 65.7 us, four: 60.5 us, and few tokens wait longer: 608 take
 // 6.5, 6.8 and 12.9 us).  Queries, keys and values are warps of their own, keys first, since they take longest (queries first: 60.3 us).
@@ -41,7 +42,7 @@ __device__ __forceinline__ Eight load8(const uint16_t* p) {
 }
 __device__ __forceinline__ void store8(uint16_t* p, const Eight& v) { *reinterpret_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]); }
 
-// Per-head RMSNorm of queries: rope_kv.cu's sum, term for term (its lane l has dims HD/32 l of either half, and it adds lanes 16, 8, ... 1
+// Per-head RMSNorm of queries: rope_kv.cu's sum, term for term (its lane l has HD / 64 dims of either half, from HD / 64 l on, and it adds lanes 16, 8, ... 1
 // apart), so that a model's queries do not depend on what holds its cache.
 template <int HD>
 __device__ __forceinline__ void norm_query(Eight& a, Eight& b, const Eight& wa, const Eight& wb, float eps) {

@@ -17,10 +17,12 @@ namespace {
 using namespace tc5;
 
 // Which of the two, for all sequences of a call, by what they cost in records x blocks of 8 columns.  Both kernels at work on 64 sequences
-// behind 2000 tokens, 4 q heads a kv head: 8 new tokens (~36 columns) 155 and 168 us, 16 new 292 and 172 us; so a tile of 128 keys counts
-// like 41.  The second kernel has 5 to 9 us more of start and end (32 tokens behind 1500: 20.7 and 28.8 us; but 16 behind 12000 42.0 and
-// 36.0), and two kernels, one after the other, cost the shorter one's latency (8 sequences of 4 to 12 new tokens behind 1500: 31 us with
-// either kernel, 49 with both, before both became faster).
+// behind 2000 tokens, 4 q heads a kv head: 8 new tokens (32 columns) 156 and 173 us, 16 new 292 and 175 us; so a tile of 128 keys counts
+// like 41.  The second kernel has 5 to 8 us more of start and end (32 tokens behind 1500: 20.8 and 28.2 us; but 16 behind 12000 42.9 and
+// 37.3), and two kernels, one after the other, cost the shorter one's latency (8 sequences of 4 to 12 new tokens behind 1500: 25 and 31 us,
+// 48 with both; 31 of 4 and one of 512 behind 2000: 226, 122 and 101 with both).  The same rule serves head size 64, where both kernels save
+// alike (64 of 8 behind 2000: 112 and 136 us, of 16 206 and 136, 32 behind 1500 17.6 and 23.1, 16 behind 12000 33.2 and 30.4).  Where it is
+// off: short prompts with nothing before them, of which the second kernel takes only what the mask leaves (200 tokens: 22 us for 19).
 constexpr double kTileCost = 41, kStartCost = 1.4e4, kBothCost = 2e4;
 // In tiles (2.4 us): what a segment costs besides its tiles, what joining parts does, and the shortest run worth a CTA.
 constexpr double kSegmentCost = 2, kJoinCost = 4, kShortRun = 4;
@@ -53,12 +55,14 @@ __device__ __forceinline__ uint32_t tile_at(int row, int dim) {  // of 8 dims
 // Bound by a block's chain of product, softmax, product (two thirds of it are the tensor cores').  Converting in here costs each CTA what an
 // own kernel would do once per 128 keys, in warps that the chain leaves idle: 512 tokens behind 11800 that read bf16 tiles, made by such a
 // kernel, from L2 took 210 us where this took 236, but 64 tokens behind 12000 took 60 instead of 45, and eight sequences of 16 behind 1500 took 47
-// instead of 33.  The three roles' code competes for the SM's instruction cache: loops that could be unrolled are not (512 behind 11800: masks in
-// place 234 -> 228 us, exponentials 222, the maximum and P by halves 218), but for the issuing thread's, whose latency counts (229).
+// instead of 33.  The three roles' code competes for the SM's instruction cache: loops that could be unrolled are not (512 behind 11800, each step
+// timed on the same inputs again and again: masks in place 234 -> 228 us, exponentials 222, the maximum and P by halves 218; on new inputs each
+// time 237 in the end), but for the issuing thread's, whose latency counts.
 // A value that is NaN must reach the rows that see it and no others, but a row that does not still multiplies it, with zero: it goes into the
 // token's keys, whose scores are masked by choice and not by multiplication, and the value becomes zero.
-// P carries 8 bits (one rounding of each weight, relative 2^-9; their sum is taken before the rounding, whose errors have no sign of their
-// own): a second product for the rest of P would cost half as much again.
+// P carries 8 bits (one rounding of each weight, 2^-8 of it at most; their sum is taken before the rounding, whose errors have no sign of their
+// own).  A second product for the rest of P brings the error to that of the other kernels (512 behind 11800: 0.0023 to 0.0017 of the values'
+// size, most of it the result's rounding) and takes a third more time (239 -> 315 us, three prompts 63 -> 77).
 constexpr int kRows = 128, kSlots = 5, kConvert = 8, kIssuer = 12, kThreads = 416;
 constexpr float kRaise = 8.f, kFloor = -1e30f;
 template <int HD>
@@ -609,8 +613,7 @@ __global__ void __launch_bounds__(256) kv_q4_prefill_merge_kernel(const ProductP
 
 }  // namespace
 
-int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int hkv, int head_dim, Q4Plan& plan) {
-    (void)head_dim;
+int32_t b2_kv_q4_plan(b2_ctx* ctx, const std::vector<Q4Seq>& seqs, int hq, int hkv, Q4Plan& plan) {
     plan = Q4Plan{};
     const int group = hq / hkv, step = 2 * (kRows / group);  // query tokens of an item
     auto few_cost = [&](const Q4Seq& s) { return (double)((s.ctx + 15) / 16) * hkv * (((int64_t)s.q_len * group + 7) / 8); };
@@ -794,7 +797,7 @@ extern "C" int32_t b2_paged_attn_prefill_q4(b2_ctx* ctx, const uint16_t* q_dev, 
     }
     B2_CUDA(cudaSetDevice(ctx->device));
     Q4Plan plan;
-    B2_CHECK(b2_kv_q4_plan(ctx, seqs, hq, hkv, head_dim, plan));
+    B2_CHECK(b2_kv_q4_plan(ctx, seqs, hq, hkv, plan));
     if (plan.host.empty()) return B2_OK;
     void* dev = nullptr;
     B2_CHECK(b2_ctx_stage(ctx, plan.host.size() * 4, &dev));
