@@ -64,7 +64,7 @@ __device__ __forceinline__ uint32_t tile_at(int row, int dim) {  // of 8 dims
 // own).  A second product for the rest of P brings the error to that of the other kernels (512 behind 11800: 0.0023 to 0.0017 of the values'
 // size, most of it the result's rounding) and takes a third more time (239 -> 315 us, three prompts 63 -> 77).
 constexpr int kRows = 128, kSlots = 5, kConvert = 8, kIssuer = 12, kThreads = 416;
-constexpr float kRaise = 8.f, kFloor = -1e30f;
+constexpr float kRaise = 8.f, kFloor = -3e38f;
 template <int HD>
 struct Smem {
     static constexpr int kQ = 0, kRing = 2 * tile_bytes<HD>(), kBar = kRing + kSlots * tile_bytes<HD>(), kBytes = kBar + 256;

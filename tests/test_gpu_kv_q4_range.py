@@ -102,3 +102,32 @@ def test_prefill_keeps_a_scale_that_is_too_large_from_earlier_queries(env, hd, s
     assert np.isfinite(H.bf16_to_f32_np(got[:, 2:])).all()  # the other kv head
     cache.k[0], cache.v[0] = cache.k[0][:, :cached + before], cache.v[0][:, :cached + before]
     T.check_rows(got[:before], q[:before], cache, 0, 0.1, many=new * hq // hkv > 32)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new, cached", [(1, 20), (1, 3000), (3, 37), (400, 700), (100, 6000)])
+def test_scores_far_below_zero(env, hd, new, cached):
+    """All scores are the same number of some -2^113: the result is the mean of the values, not nothing.  Tolerance: equal weights are 1 each, which is
+    exact, so what is left are sums in f32 of at most n terms and the result's rounding."""
+    ctx, K = env
+    n, hq, hkv, page = cached + new, 4, 1, 16
+    pages = (n + page - 1) // page
+    rng = np.random.default_rng(hd + n)
+    qkv = rng.standard_normal((n, hq + 2, hd))
+    qkv[:, :hq], qkv[:, hq] = 2.0 ** 90, -2.0 ** 20
+    qkv = O.bf16(qkv)
+    slots, order = np.arange(n, dtype=np.int32), np.arange(pages, dtype=np.int32)
+    cos, sin = np.ones((1, hd // 2)), np.zeros((1, hd // 2))
+    _, pool, _, (k, v) = T.run_append(env, qkv, np.zeros(n, np.int32), slots, cos, sin, None, None, page, pages, hq, hkv, hd)
+    assert (H.bf16_to_f32_np(k) == -2.0 ** 20).all()
+    v = H.bf16_to_f32_np(v).astype(np.float64)[:, 0]
+    q, out = ctx.buf(T.as_bf16(qkv[-new:, :hq])), ctx.empty((new, hq, hd), np.uint16)
+    K.paged_attn_prefill_q4(ctx, q, ctx.buf(pool), pages, ctx.buf(order[None]), pages, [0, new], [n], hq, hkv, hd, page, 0.125, out)
+    ctx.sync()
+    ref = (np.cumsum(v, 0) / np.arange(1, n + 1)[:, None])[-new:, None]
+    tol = 2 * n * 2.0 ** -24 * np.abs(v).max() + 2.0 ** -8 * np.abs(ref)
+    assert (np.abs(H.bf16_to_f32_np(out.download()) - ref) <= tol).all()
+    if new == 1:
+        K.paged_attn_decode_q4(ctx, q, ctx.buf(pool), pages, ctx.buf(order[None]), ctx.buf(np.array([n], np.int32)), 1, hq, hkv, hd, page, 0.125, out, pages)
+        ctx.sync()
+        assert (np.abs(H.bf16_to_f32_np(out.download()) - ref) <= tol).all()
