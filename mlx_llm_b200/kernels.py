@@ -1,6 +1,7 @@
 """Kernel-level entry points of the C ABI as Python callables (device buffers in, device buffers
 out).  Used by the parity tests and the microbenchmarks; the engine API lives in engine.py."""
 import ctypes as C
+import operator
 
 import numpy as np
 
@@ -42,7 +43,10 @@ class _Entry:
         if self.fn is None:
             self.fn = getattr(load(), self.name)
             self.fn.argtypes = self.types
-        rc = self.fn(*args)
+        try:
+            rc = self.fn(*args)
+        except C.ArgumentError:  # numbers that are not Python's own, an array's length in numpy for one
+            rc = self.fn(*[a if a is None or isinstance(a, C.c_void_p) else float(a) if t is C.c_float else operator.index(a) for t, a in zip(self.types, args)])
         if rc:
             check(rc)
 
@@ -165,7 +169,7 @@ def logit_rules(mask_words=0, **arrays):
     if unknown:  # (a structure takes any attribute, and the call would go without the rule)
         raise TypeError(f"logit_rules: no rule is called {', '.join(unknown)}; there are {', '.join(names)}")
     rules = LogitRules()
-    rules.mask_words = mask_words
+    rules.mask_words = operator.index(mask_words)
     for name, a in arrays.items():
         setattr(rules, name, _at(a))
     return rules

@@ -46,3 +46,16 @@ def test_more_queries_than_a_plan_holds(kernels):
     refused(lambda: prefill(kernels, cu=(0, n), ctx=(n,), blocks=1 << 27, hq=16, hkv=8), -5)
     refused(lambda: prefill(kernels, cu=(0, n), ctx=(n,), blocks=1 << 27, hq=1024, hkv=2), -5)
     refused(lambda: prefill(kernels, cu=(9, -(1 << 31)), ctx=(n,), blocks=1 << 27), -7)  # (a difference that 32 bits do not hold)
+
+
+def test_numbers_of_numpy(kernels):
+    """They go through to the library, whose refusal comes back; what is no number does not."""
+    refused(lambda: decode(kernels, n=np.int64(-1)), -7)
+    refused(lambda: decode(kernels, hd=np.int32(96)), -5)
+    refused(lambda: append(kernels, T=np.int64(-1)), -7)
+    refused(lambda: prefill(kernels, scale=np.float32(-1)), -7)
+    refused(lambda: kernels.logits_adjust(CTX, AT, np.int64(-1), 64, kernels.logit_rules(mask_words=np.int64(4)), argmax=AT), -7)
+    with pytest.raises(TypeError):
+        decode(kernels, n=1.5)
+    with pytest.raises(TypeError):
+        decode(kernels, n="3")
