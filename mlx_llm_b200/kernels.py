@@ -157,6 +157,8 @@ def argmax(ctx, logits, rows, vocab, out):
 class LogitRules(C.Structure):
     """b2_logit_rules: device pointers, null where a rule is not used."""
 
+    __slots__ = ()  # no attributes but the fields: a misspelt rule must not vanish in one
+
     _fields_ = [(n, C.c_void_p) for n in ("history", "history_off", "n_prompt", "repetition", "presence", "frequency", "bias_id", "bias_value", "bias_off",
                                           "mask")] + [("mask_words", C.c_int64), ("mask_row", C.c_void_p)]
 
@@ -164,14 +166,13 @@ class LogitRules(C.Structure):
 def logit_rules(mask_words=0, **arrays):
     """Rules for logits_adjust: history, history_off, n_prompt, repetition, presence, frequency, bias_id, bias_value, bias_off, mask, mask_row as device
     buffers (None: not used), and the words of a mask's row."""
-    names = [name for name, _ in LogitRules._fields_ if name != "mask_words"]
-    unknown = sorted(set(arrays) - set(names))
-    if unknown:  # (a structure takes any attribute, and the call would go without the rule)
-        raise TypeError(f"logit_rules: no rule is called {', '.join(unknown)}; there are {', '.join(names)}")
     rules = LogitRules()
-    rules.mask_words = operator.index(mask_words)
-    for name, a in arrays.items():
-        setattr(rules, name, _at(a))
+    rules.mask_words = mask_words if type(mask_words) is int else operator.index(mask_words)
+    try:
+        for name, a in arrays.items():
+            setattr(rules, name, _at(a))
+    except AttributeError:
+        raise TypeError(f"logit_rules: no rule is called {name}; there are {', '.join(n for n, _ in LogitRules._fields_ if n != 'mask_words')}") from None
     return rules
 
 

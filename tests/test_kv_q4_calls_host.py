@@ -59,3 +59,9 @@ def test_numbers_of_numpy(kernels):
         decode(kernels, n=1.5)
     with pytest.raises(TypeError):
         decode(kernels, n="3")
+
+
+def test_a_rule_that_is_not_there_set_by_hand(kernels):
+    rules = kernels.logit_rules()
+    with pytest.raises(AttributeError):
+        rules.masks = AT
