@@ -2,8 +2,8 @@
 // verification step checks.
 //
 // Byte streaming, 144 bytes per token and kv head (head size 128), that is bound by its instructions: 377 a record, with 64 % of the issue
-// slots taken; 32 sequences of 8000 to 16000 tokens stream at 3.8 to 4.1 of the 6.5 TB/s that a copy reaches (116 us by itself, 109 in a
-// row of calls).
+// slots taken; 32 sequences of 8000 to 16000 tokens stream at 4.1 of the 6.5 TB/s that a copy reaches (109 us in a row of calls; 116
+// with nothing in the caches, 3.8).
 //
 //   unit    = (sequence, kv head, block of 8 columns); a column is one (query token, q head of the group).  Its work is the sequence's
 //             16-token records.
