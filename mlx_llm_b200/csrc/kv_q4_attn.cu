@@ -30,7 +30,7 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 8;
 constexpr int kStages = 4;             // records of a warp in shared memory: the two that it works on, the two that are on their way
-constexpr float kFloor = -3e38f;     // reference of a column that has seen nothing: exp2(-inf - floor) is 0, and every finite score counts
+constexpr float kFloor = -3e38f;     // reference of a column that has seen nothing: exp2(-inf - floor) is 0; scores down to it count
 constexpr float kSlack = 8.f;
 constexpr int kMinRun = 4;           // records of a run at least (one sequence of 4000: 18.0 us, 2 records 18.1, 8 records 20.3)
 // Where units have warps to themselves: the records that the longest may have beyond an equal run, and the longest such run.  64 sequences

@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t tile_at(int row, int dim) {  // of 8 dims
 // kernel, from L2 took 210 us where this took 236, but 64 tokens behind 12000 took 60 instead of 45, and eight sequences of 16 behind 1500 took 47
 // instead of 33.  The three roles' code competes for the SM's instruction cache: loops that could be unrolled are not (512 behind 11800, each step
 // timed on the same inputs again and again: masks in place 234 -> 228 us, exponentials 222, the maximum and P by halves 218; on new inputs each
-// time 237 in the end), but for the issuing thread's, whose latency counts.
+// time 235 in the end), but for the issuing thread's, whose latency counts.
 // A value that is NaN must reach the rows that see it and no others, but a row that does not still multiplies it, with zero: it goes into the
 // token's keys, whose scores are masked by choice and not by multiplication, and the value becomes zero.
 // P carries 8 bits (one rounding of each weight, 2^-8 of it at most; their sum is taken before the rounding, whose errors have no sign of their
